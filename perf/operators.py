@@ -322,7 +322,7 @@ def _own_scan_train(s):
     gates = (s["x"], s["A_log"], s["a"], s["dt_bias"], s["b"], s["cu"])
     ckpt = rec.empty_checkpoints(s["x"])
     y, ns = rec.launch_scan(*gates, s["state"], checkpoints=ckpt)
-    dx, da, db, dA_log, ddt_bias, dstate = rec.launch_scan_backward(s["dy"], *gates, ckpt, d_new_state=s["dns"])
+    dx, da, db, dA_log, ddt_bias, dstate = rec.launch_scan_backward(s["dy"], *gates, s["state"], ckpt, d_new_state=s["dns"])
     out = {"y": y, "new_state": ns, "dx": dx, "da": da, "db": db, "dA_log": dA_log, "ddt_bias": ddt_bias}
     if s["state"] is not None:
         out["dstate"] = dstate
