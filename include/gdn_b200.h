@@ -10,7 +10,11 @@
  *   gdn_prefill_launch  replaces gdn_prefill_qk4_v8_d128_k_last/solution/triton/kernel.py:56-262
  *                       (launch_gdn, registered as "flashinfer.kernel")
  *
- * Problem constants are those of both definitions: 4 q/k heads, 8 v heads,
+ * and beside them stand the operators that a recurrent layer needs around the
+ * delta rule: the per-channel gated recurrence (gdn_scan_*), the residual and
+ * the gated root-mean-square norm (gdn_add_norm_*, gdn_gated_norm_*).
+ *
+ * Problem constants of the first two are those of both definitions: 4 q/k heads, 8 v heads,
  * head dim 128, k-last fp32 state [.., 8, 128 (V), 128 (K)].
  *
  * Conventions
@@ -48,7 +52,7 @@ typedef enum gdn_status_t {
     GDN_ERR_MISALIGNED = 3,        /* a pointer violates its alignment rule */
     GDN_ERR_WORKSPACE = 4,         /* workspace missing or too small */
     GDN_ERR_CUDA = 5,              /* a CUDA runtime call failed */
-    GDN_ERR_BAD_DTYPE = 6,         /* unsupported cu_seqlens dtype code */
+    GDN_ERR_BAD_DTYPE = 6,         /* unsupported dtype code */
     GDN_ERR_NO_DEVICE = 7,         /* no usable sm_100 device is current */
     GDN_ERR_DEVICE_BAD_SEQLENS = 16,  /* device status bit: cu_seqlens not monotone / out of range */
     GDN_ERR_DEVICE_TIMEOUT = 32       /* device status bit: a bounded wait expired */
@@ -254,6 +258,169 @@ int gdn_prefill_cp_launch(const GdnPrefillArgs* args, void* workspace, size_t wo
  * All calls on a device share the array: calls whose kernels overlap on the
  * GPU (different streams or host threads) race and must be serialised. */
 int gdn_prefill_launch_noalloc(const GdnPrefillArgs* args, void* stream);
+
+/* ---------------------------------------------- per-channel recurrence -- */
+
+/* Element types of the operators below. */
+#define GDN_DTYPE_BF16 0
+#define GDN_DTYPE_F16 1
+#define GDN_DTYPE_F32 2
+
+/* The per-channel gated linear recurrence over packed sequences, with the
+ * gates of the delta-rule kernels:
+ *   h_t = g_t h_{t-1} + sigmoid(b_t) x_t,  g_t = exp(-exp(A_log) softplus(a_t + dt_bias)),  y_t = h_t
+ *   x, a, b     [T, C] of `dtype`; *_stride elements between tokens (>= C),
+ *               channels contiguous: column blocks of one projection's output
+ *               need no copy.  Any alignment; rows on 16-byte boundaries are
+ *               read as vectors.
+ *   A_log, dt_bias fp32 [C]
+ *   state       fp32 [N, C] or NULL (zero); must not alias new_state
+ *   cu_seqlens  int32 or int64 [N + 1], non-decreasing, cu[0] >= 0, cu[N] <= T
+ *   output      [T, C] of `dtype`, output_stride elements between tokens
+ *   new_state   fp32 [N, C]
+ *   checkpoints fp32 [gdn_scan_checkpoint_rows(T), C] or NULL: what the
+ *               backward pass needs of the forward pass
+ * The output must not overlap an input.  State and sums are fp32.  An empty
+ * sequence's new_state row is its state row.  Output rows (and gradients) of
+ * tokens that belong to no sequence are written as zeros.  No reference
+ * counterpart (the reference has the delta rule only). */
+typedef struct GdnScanArgs {
+    const void* x;
+    const void* a;
+    const void* b;
+    int64_t x_stride, a_stride, b_stride;
+    const float* A_log;
+    const float* dt_bias;
+    const float* state;
+    const void* cu_seqlens;
+    int32_t cu_seqlens_dtype;
+    int32_t dtype;
+    int64_t total_tokens;
+    int64_t num_seqs;
+    int64_t channels;
+    void* output;
+    int64_t output_stride;
+    float* new_state;
+    float* checkpoints;
+} GdnScanArgs;
+
+/* Gradients: d_output [T, C] and d_new_state fp32 [N, C] (NULL: zero) in;
+ * dx, da, db [T, C] of `dtype` and dA_log, d_dt_bias fp32 [C], d_state fp32
+ * [N, C] (NULL: not wanted) out. */
+typedef struct GdnScanGradArgs {
+    const void* d_output;
+    int64_t d_output_stride;
+    const float* d_new_state;
+    void* dx;
+    void* da;
+    void* db;
+    int64_t dx_stride, da_stride, db_stride;
+    float* dA_log;
+    float* d_dt_bias;
+    float* d_state;
+} GdnScanGradArgs;
+
+int gdn_scan_launch(const GdnScanArgs* args, void* stream);
+
+/* The backward pass of gdn_scan_launch: the same args (output and new_state
+ * unused) with the checkpoints that the forward call wrote.  The workspace
+ * (16-byte aligned) is free again when the call's kernels have run; calls
+ * that overlap need one each. */
+int64_t gdn_scan_checkpoint_rows(int64_t total_tokens);
+size_t gdn_scan_backward_workspace_size(int64_t total_tokens, int64_t num_seqs, int64_t channels);
+int gdn_scan_backward_launch(const GdnScanArgs* args, const GdnScanGradArgs* grads, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Decode: `tokens` >= 1 tokens for each of num_seqs sequences, total_tokens =
+ * num_seqs * tokens rows in sequence order; cu_seqlens and checkpoints are not
+ * read; state is required and may be new_state. */
+int gdn_scan_step_launch(const GdnScanArgs* args, int64_t tokens, void* stream);
+
+/* ----------------------------------------------------------------- norms -- */
+
+#define GDN_QUANT_NONE 0
+#define GDN_QUANT_ROW 1   /* e4m3 output, one scale per row */
+#define GDN_QUANT_GROUP 2 /* e4m3 output, one scale per 128 channels (gated norm: per head) */
+
+/* r = x + residual; y = r / sqrt(mean(r^2) + eps) * weight over rows of
+ * `width` (1 .. 32768) elements.
+ *   x, residual [rows, width] of `dtype`, *_stride elements between rows;
+ *               residual NULL: r = x, and new_residual is not written
+ *   weight      [width], fp32 or `dtype` (weight_dtype)
+ *   new_residual [rows, width]: r rounded to `dtype`; may be residual or x itself
+ *               (the same rows, contiguous).  The norm is of the unrounded r.
+ *   output      [rows, width] of `dtype`, or e4m3 codes
+ *   scale       fp32 [rows] or [rows, width / 128] (width a multiple of 128):
+ *               max(amax |y|, 1e-12) / 448; code = e4m3(y / scale), saturating;
+ *               NaN stays NaN, in the scale too
+ * No reference counterpart (the reference has the recurrence alone). */
+typedef struct GdnAddNormArgs {
+    const void* x;
+    const void* residual;
+    int64_t x_stride, residual_stride;
+    const void* weight;
+    int32_t weight_dtype;
+    int32_t dtype;
+    int32_t quant;
+    float eps;
+    int64_t rows;
+    int64_t width;
+    void* output;
+    void* new_residual;
+    float* scale;
+} GdnAddNormArgs;
+
+int gdn_add_norm_launch(const GdnAddNormArgs* args, void* stream);
+
+/* y = x / sqrt(mean(x^2) + eps) * weight * z sigmoid(z) over each head of
+ * head_dim (64, 128 or 256) elements: the norm of a recurrence's output
+ * [tokens, heads, head_dim] with its gate.
+ *   x, z    [tokens, heads, head_dim] of `dtype`, *_stride elements between
+ *           tokens, a token's heads contiguous
+ *   weight  [head_dim], fp32 or `dtype`
+ *   output  contiguous, of `dtype` (may be x itself when x is contiguous) or
+ *           e4m3 codes with scale fp32 [tokens, heads] (GDN_QUANT_GROUP) */
+typedef struct GdnGatedNormArgs {
+    const void* x;
+    const void* z;
+    int64_t x_stride, z_stride;
+    const void* weight;
+    int32_t weight_dtype;
+    int32_t dtype;
+    int32_t quant;
+    float eps;
+    int64_t tokens;
+    int32_t heads;
+    int32_t head_dim;
+    void* output;
+    float* scale;
+} GdnGatedNormArgs;
+
+int gdn_gated_norm_launch(const GdnGatedNormArgs* args, void* stream);
+
+/* Gradients of either norm (quant = GDN_QUANT_NONE): d_output in the layout
+ * of x; dx (and dz of the gated norm) contiguous, of `dtype`; d_weight fp32.
+ * For gdn_add_norm args->x is the stored sum (new_residual), residual is not
+ * read, and dx -- the gradient of x and of residual alike -- includes
+ * d_new_residual (NULL: zero).  Sums are taken in a fixed order: the same
+ * call gives the same bits.  The workspace (16-byte aligned) is free again
+ * when the call's kernels have run; calls that overlap need one each. */
+typedef struct GdnNormGradArgs {
+    const void* d_output;
+    int64_t d_output_stride;
+    const void* d_new_residual;
+    int64_t d_new_residual_stride;
+    void* dx;
+    void* dz;
+    float* d_weight;
+} GdnNormGradArgs;
+
+size_t gdn_add_norm_backward_workspace_size(int64_t rows, int64_t width);
+int gdn_add_norm_backward_launch(const GdnAddNormArgs* args, const GdnNormGradArgs* grads, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+size_t gdn_gated_norm_backward_workspace_size(int64_t tokens, int32_t heads, int32_t head_dim);
+int gdn_gated_norm_backward_launch(const GdnGatedNormArgs* args, const GdnNormGradArgs* grads, void* workspace,
+                                   size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- status -- */
 

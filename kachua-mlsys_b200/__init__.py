@@ -9,12 +9,14 @@ romitjain/kachua-mlsys):
 
 * ``decode.launch_gdn``  -- gdn_decode_qk4_v8_d128_k_last
 * ``prefill.launch_gdn`` -- gdn_prefill_qk4_v8_d128_k_last
+* ``recurrence``         -- the per-channel gated recurrence: scan, backward, step
+* ``norm``               -- residual and gated RMS norms, with e4m3 outputs
 * ``inputs``             -- seeded synthetic inputs of the benchmark configs
 * ``shard``              -- sequence sharding across GPUs and the final gather
 """
-from . import _build, _capi, decode, inputs, prefill, shard  # noqa: F401
+from . import _build, _capi, decode, inputs, norm, prefill, recurrence, shard  # noqa: F401
 
-__all__ = ["decode", "prefill", "inputs", "build"]
+__all__ = ["decode", "prefill", "recurrence", "norm", "inputs", "build"]
 
 
 def build(force: bool = False, verbose: bool = False):

@@ -38,8 +38,21 @@ EXPORTED_SYMBOLS = (
     "gdn_prefill_cp_workspace_size",
     "gdn_prefill_cp_summary_offset",
     "gdn_prefill_cp_launch",
+    "gdn_scan_launch",
+    "gdn_scan_checkpoint_rows",
+    "gdn_scan_backward_workspace_size",
+    "gdn_scan_backward_launch",
+    "gdn_scan_step_launch",
+    "gdn_add_norm_launch",
+    "gdn_add_norm_backward_workspace_size",
+    "gdn_add_norm_backward_launch",
+    "gdn_gated_norm_launch",
+    "gdn_gated_norm_backward_workspace_size",
+    "gdn_gated_norm_backward_launch",
 )
-ABI_VERSION = 9
+ABI_VERSION = 10
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+QUANT_NONE, QUANT_ROW, QUANT_GROUP = 0, 1, 2
 PATH_AUTO, PATH_RECURRENT, PATH_CHUNKED, PATH_SEGMENTED = 0, 1, 2, 3
 MMA_KIND_BF16, MMA_KIND_TF32, MMA_KIND_F16 = 1, 2, 3
 MMA_A_MN, MMA_B_MN, MMA_D_LANE16, MMA_A_TMEM, MMA_NO_COMPLETION = 1, 2, 4, 8, 16
@@ -80,6 +93,97 @@ class GdnPrefillArgs(ctypes.Structure):
         ("scale", ctypes.c_float),
         ("output", ctypes.c_void_p),
         ("new_state", ctypes.c_void_p),
+    ]
+
+
+class GdnScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("a_stride", ctypes.c_int64),
+        ("b_stride", ctypes.c_int64),
+        ("A_log", ctypes.c_void_p),
+        ("dt_bias", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("cu_seqlens_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("total_tokens", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("output", ctypes.c_void_p),
+        ("output_stride", ctypes.c_int64),
+        ("new_state", ctypes.c_void_p),
+        ("checkpoints", ctypes.c_void_p),
+    ]
+
+
+class GdnScanGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_output", ctypes.c_void_p),
+        ("d_output_stride", ctypes.c_int64),
+        ("d_new_state", ctypes.c_void_p),
+        ("dx", ctypes.c_void_p),
+        ("da", ctypes.c_void_p),
+        ("db", ctypes.c_void_p),
+        ("dx_stride", ctypes.c_int64),
+        ("da_stride", ctypes.c_int64),
+        ("db_stride", ctypes.c_int64),
+        ("dA_log", ctypes.c_void_p),
+        ("d_dt_bias", ctypes.c_void_p),
+        ("d_state", ctypes.c_void_p),
+    ]
+
+
+class GdnAddNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("quant", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rows", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("output", ctypes.c_void_p),
+        ("new_residual", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+    ]
+
+
+class GdnGatedNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("z", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("z_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("quant", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("output", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+    ]
+
+
+class GdnNormGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("d_output", ctypes.c_void_p),
+        ("d_output_stride", ctypes.c_int64),
+        ("d_new_residual", ctypes.c_void_p),
+        ("d_new_residual_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dz", ctypes.c_void_p),
+        ("d_weight", ctypes.c_void_p),
     ]
 
 
@@ -143,6 +247,23 @@ def load(build_if_needed: bool = True) -> ctypes.CDLL:
         lib.gdn_abi_version.restype = ctypes.c_int
         lib.gdn_mma_selftest.argtypes = [ctypes.c_int] * 5 + [P, P, P, P]
         lib.gdn_mma_selftest.restype = ctypes.c_int
+        i64, size = ctypes.c_int64, ctypes.c_size_t
+        scan, norm, gated = (ctypes.POINTER(t) for t in (GdnScanArgs, GdnAddNormArgs, GdnGatedNormArgs))
+        scan_grad, norm_grad = ctypes.POINTER(GdnScanGradArgs), ctypes.POINTER(GdnNormGradArgs)
+        for name, restype, argtypes in (
+                ("gdn_scan_launch", ctypes.c_int, [scan, P]),
+                ("gdn_scan_checkpoint_rows", i64, [i64]),
+                ("gdn_scan_backward_workspace_size", size, [i64, i64, i64]),
+                ("gdn_scan_backward_launch", ctypes.c_int, [scan, scan_grad, P, size, P]),
+                ("gdn_scan_step_launch", ctypes.c_int, [scan, i64, P]),
+                ("gdn_add_norm_launch", ctypes.c_int, [norm, P]),
+                ("gdn_add_norm_backward_workspace_size", size, [i64, i64]),
+                ("gdn_add_norm_backward_launch", ctypes.c_int, [norm, norm_grad, P, size, P]),
+                ("gdn_gated_norm_launch", ctypes.c_int, [gated, P]),
+                ("gdn_gated_norm_backward_workspace_size", size, [i64, ctypes.c_int32, ctypes.c_int32]),
+                ("gdn_gated_norm_backward_launch", ctypes.c_int, [gated, norm_grad, P, size, P])):
+            getattr(lib, name).restype = restype
+            getattr(lib, name).argtypes = argtypes
         if lib.gdn_abi_version() != ABI_VERSION:
             raise RuntimeError("libgdn_b200.so ABI version mismatch; rebuild it")
         _lib = lib

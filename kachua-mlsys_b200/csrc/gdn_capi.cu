@@ -37,7 +37,7 @@ static float resolve_scale(float s) { return s == 0.0f ? 1.0f / sqrtf((float)kD)
 
 using namespace gdn;
 
-extern "C" int gdn_abi_version(void) { return 9; }
+extern "C" int gdn_abi_version(void) { return 10; }
 
 extern "C" const char* gdn_status_string(int status) {
     switch (status) {
@@ -47,7 +47,7 @@ extern "C" const char* gdn_status_string(int status) {
         case GDN_ERR_MISALIGNED: return "a pointer violates its alignment rule";
         case GDN_ERR_WORKSPACE: return "workspace missing or too small";
         case GDN_ERR_CUDA: return "a CUDA runtime call failed";
-        case GDN_ERR_BAD_DTYPE: return "unsupported cu_seqlens dtype code";
+        case GDN_ERR_BAD_DTYPE: return "unsupported dtype code";
         case GDN_ERR_NO_DEVICE: return "no usable sm_100 device is current";
         case GDN_ERR_DEVICE_BAD_SEQLENS: return "device: cu_seqlens not monotone or out of range";
         case GDN_ERR_DEVICE_TIMEOUT: return "device: a bounded wait expired";
@@ -299,3 +299,7 @@ extern "C" int gdn_mma_selftest(int kind, int flags, int M, int N, int K, const 
 
 // Decode with the state in host memory, transfers pipelined with the kernel.
 #include "gdn_decode_staged.cu"
+
+// The per-channel recurrence and the norms around it.
+#include "gdn_recurrence.cu"
+#include "gdn_norm.cu"

@@ -84,7 +84,7 @@ def _ptr(t: torch.Tensor):
     return ctypes.c_void_p(t.data_ptr())
 
 
-def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, scale=None, output=None, new_state=None):
+def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, scale=None, output=None, new_state=None, out_norm=None):
     """One GDN decode step (destination-passing); returns ``(output, new_state)``.
 
     ``output`` is bf16 ``[B, 8, 128]`` (``[B, 1, 8, 128]`` is accepted too);
@@ -94,6 +94,8 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, scale=None, output=None, ne
     per sequence (q ``[B, T, 4, 128]``: speculative or multi-token decode)
     the tokens are applied in order in one call, ``output`` is
     ``[B, T, 8, 128]`` and ``new_state`` the state after the last token.
+    ``out_norm`` (a ``norm.OutputNorm``) applies the gated per-head norm to
+    ``output`` right behind the step, on the same stream.
     """
     _need(isinstance(q, torch.Tensor) and q.dim() == 4, "q must be a [B, T, 4, 128] tensor")
     T = q.shape[1]
@@ -104,6 +106,7 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, scale=None, output=None, ne
     if new_state is None:
         new_state = torch.empty_like(state)
     B = validate(q, k, v, state, A_log, a, dt_bias, b, output, new_state)
+    norm_output = None if out_norm is None else out_norm.prepare(output)
     lib = _capi.load()
     args = _capi.GdnDecodeArgs(
         _ptr(q), _ptr(k), _ptr(v), _ptr(state), _ptr(A_log), _ptr(a), _ptr(dt_bias), _ptr(b),
@@ -123,6 +126,8 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, scale=None, output=None, ne
         else:
             _capi.check(lib.gdn_decode_launch_tokens(ctypes.byref(args), T, ctypes.c_void_p(stream)),
                         "gdn_decode_launch_tokens")
+    if norm_output is not None:
+        norm_output()
     return output, new_state
 
 

@@ -1,0 +1,301 @@
+"""Root-mean-square norms on either side of a recurrent layer.
+
+``launch_add_norm``    r = x + residual; y = r / sqrt(mean(r^2) + eps) * weight, before a layer's projections
+``launch_gated_norm``  y = x / sqrt(mean(x^2) + eps) * weight * silu(z) over each head of a recurrence's output
+                       (``launch_gdn(..., out_norm=...)`` applies it to its own output)
+
+Both write the inputs' type, or e4m3 codes with fp32 scales for an 8-bit
+product: scale = max(amax |y|, 1e-12) / 448 per row or per 128 channels
+(``launch_add_norm``) or per head (``launch_gated_norm``), code = e4m3(y /
+scale), saturating.  The backward passes and the differentiable ``add_norm``
+and ``gated_norm`` are for training.  Inputs are bf16, fp16 or fp32, all of
+one type, the weight fp32 or that type; statistics and sums are fp32 and every
+output is rounded once.  Everything runs on the current torch stream,
+asynchronously; errors in arguments raise ``ValueError`` before a launch.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _capi
+from .recurrence import DTYPES, _call, _dense, _need, _ptr, _rows
+
+QUANT = {None: _capi.QUANT_NONE, "row": _capi.QUANT_ROW, "group": _capi.QUANT_GROUP}
+GROUP = 128
+MAX_WIDTH = 32768
+HEAD_DIMS = (64, 128, 256)
+
+
+def _weight(weight, width: int, dtype, device) -> int:
+    _need(isinstance(weight, torch.Tensor), "weight must be a torch.Tensor")
+    _need(weight.dtype in (torch.float32, dtype), f"weight must be float32 or {dtype}, got {weight.dtype}")
+    _dense(weight, "weight", weight.dtype, (width,), device)
+    return DTYPES[weight.dtype]
+
+
+def _row_inputs(x, weight, eps) -> tuple[int, int, int]:
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x must be a [rows, width] tensor")
+    _need(x.device.type == "cuda", "x must be a CUDA tensor (there is no CPU path)")
+    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    rows, width = x.shape
+    _need(1 <= width <= MAX_WIDTH, f"rows must have 1 to {MAX_WIDTH} elements, got {width}")
+    _need(eps >= 0, "eps must be >= 0")
+    return rows, width, _weight(weight, width, x.dtype, x.device)
+
+
+def launch_add_norm(x, residual, weight, eps=1e-6, output=None, new_residual=None, scale=None, quant=None):
+    """Returns ``(output, new_residual)``, or with ``quant`` ``(output, new_residual, scale)``.
+
+    ``x`` and ``residual`` are ``[rows, width]`` with a free row stride;
+    ``residual=None`` norms ``x`` alone and returns ``x`` as ``new_residual``.
+    ``new_residual`` is the sum in the inputs' type (the norm is of the
+    unrounded sum) and may be ``residual`` or ``x`` (in place).  ``quant``:
+    ``"row"`` (scale ``[rows, 1]``) or ``"group"`` (one scale per 128
+    channels, scale ``[rows, width / 128]``); ``output`` is then
+    ``float8_e4m3fn``.
+    """
+    rows, width, wdt = _row_inputs(x, weight, eps)
+    dev = x.device
+    _need(quant in QUANT, f"quant must be None, 'row' or 'group', got {quant!r}")
+    _need(quant != "group" or width % GROUP == 0, f"group scales need a width that is a multiple of {GROUP}, got {width}")
+    x_stride = _rows(x, "x", x.dtype, rows, width, dev)
+    res_stride = 0
+    if residual is not None:
+        res_stride = _rows(residual, "residual", x.dtype, rows, width, dev)
+        if new_residual is None:
+            new_residual = torch.empty((rows, width), dtype=x.dtype, device=dev)
+        else:
+            _dense(new_residual, "new_residual", x.dtype, (rows, width), dev)
+    else:
+        _need(new_residual is None, "new_residual needs a residual")
+    odt = torch.float8_e4m3fn if quant else x.dtype
+    if output is None:
+        output = torch.empty((rows, width), dtype=odt, device=dev)
+    else:
+        _dense(output, "output", odt, (rows, width), dev)
+    if quant:
+        scale_shape = (rows, 1 if quant == "row" else width // GROUP)
+        if scale is None:
+            scale = torch.empty(scale_shape, dtype=torch.float32, device=dev)
+        else:
+            _dense(scale, "scale", torch.float32, scale_shape, dev)
+    else:
+        _need(scale is None, "scale needs quant")
+    args = _capi.GdnAddNormArgs(_ptr(x), _ptr(residual), x_stride, res_stride, _ptr(weight), wdt, DTYPES[x.dtype],
+                                QUANT[quant], eps, rows, width, _ptr(output), _ptr(new_residual), _ptr(scale))
+    _call(_capi.load().gdn_add_norm_launch, "gdn_add_norm_launch", dev, ctypes.byref(args))
+    summed = x if residual is None else new_residual
+    return (output, summed, scale) if quant else (output, summed)
+
+
+def launch_add_norm_backward(d_output, new_residual, weight, eps=1e-6, d_new_residual=None, dx=None):
+    """Gradients of ``launch_add_norm``: ``(dx, d_weight)``.
+
+    ``new_residual`` is the sum that the forward call returned (``x`` where it
+    had no residual).  ``dx`` is the gradient of ``x`` and of ``residual``
+    alike, the ``d_new_residual`` that came down the residual stream (``None``:
+    zero) included; ``d_weight`` is fp32.  Sums are taken in a fixed order.
+    """
+    rows, width, wdt = _row_inputs(new_residual, weight, eps)
+    dev, dt = new_residual.device, new_residual.dtype
+    r_stride = _rows(new_residual, "new_residual", dt, rows, width, dev)
+    dy_stride = _rows(d_output, "d_output", dt, rows, width, dev)
+    dr_stride = 0 if d_new_residual is None else _rows(d_new_residual, "d_new_residual", dt, rows, width, dev)
+    if dx is None:
+        dx = torch.empty((rows, width), dtype=dt, device=dev)
+    else:
+        _dense(dx, "dx", dt, (rows, width), dev)
+    d_weight = torch.empty(width, dtype=torch.float32, device=dev)
+    lib = _capi.load()
+    need = int(lib.gdn_add_norm_backward_workspace_size(rows, width))
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = _capi.GdnAddNormArgs(_ptr(new_residual), None, r_stride, 0, _ptr(weight), wdt, DTYPES[dt], 0, eps, rows, width,
+                                None, None, None)
+    g = _capi.GdnNormGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_residual), dr_stride, _ptr(dx), None, _ptr(d_weight))
+    _call(lib.gdn_add_norm_backward_launch, "gdn_add_norm_backward_launch", dev, ctypes.byref(args), ctypes.byref(g),
+          _ptr(workspace), need)
+    return dx, d_weight
+
+
+def _heads(t, name: str, dtype, shape, device) -> int:
+    """Checks a [tokens, heads, dim] tensor whose tokens are contiguous; returns the token stride."""
+    _need(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
+    _need(t.shape == shape, f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    tokens, heads, dim = shape
+    s = t.stride()
+    _need(s[2] == 1 and (heads == 1 or s[1] == dim), f"{name} must have contiguous heads, got strides {s}")
+    _need(tokens <= 1 or s[0] >= heads * dim, f"{name} must not have overlapping tokens, got strides {s}")
+    return s[0] if tokens > 1 else heads * dim
+
+
+def _gated_inputs(x, z, weight, eps):
+    """x and z as [tokens, heads, dim] with their token strides, and the weight's type."""
+    _need(isinstance(x, torch.Tensor) and x.dim() >= 3, "x must be a [tokens, heads, dim] tensor")
+    _need(x.device.type == "cuda", "x must be a CUDA tensor (there is no CPU path)")
+    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    _need(isinstance(z, torch.Tensor) and z.shape == x.shape, f"z must have the shape of x, {tuple(x.shape)}")
+    heads, dim = x.shape[-2:]
+    _need(dim in HEAD_DIMS, f"the head dim must be one of {HEAD_DIMS}, got {dim}")
+    _need(1 <= heads <= 4096, f"x must have 1 to 4096 heads, got {heads}")
+    _need(eps >= 0, "eps must be >= 0")
+    if x.dim() > 3:  # [batch, tokens, heads, dim]
+        _need(x.is_contiguous() and z.is_contiguous(), "x and z must be contiguous with more than three dimensions")
+        x, z = x.view(-1, heads, dim), z.view(-1, heads, dim)
+    _need(x.shape[0] * heads <= 0x7FFF0000, "too many heads in one call")
+    xs, zs = _heads(x, "x", x.dtype, x.shape, x.device), _heads(z, "z", x.dtype, x.shape, x.device)
+    return x, z, xs, zs, _weight(weight, dim, x.dtype, x.device)
+
+
+def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):
+    """Checks the arguments and makes the C ones; returns ``(launch, output, scale)``."""
+    shape = x.shape if isinstance(x, torch.Tensor) else None
+    x, z, xs, zs, wdt = _gated_inputs(x, z, weight, eps)
+    tokens, heads, dim = x.shape
+    dev = x.device
+    odt = torch.float8_e4m3fn if quant else x.dtype
+    if output is None:
+        output = torch.empty(shape, dtype=odt, device=dev)
+    else:
+        _dense(output, "output", odt, shape, dev)
+    _need(tokens == 0 or output.data_ptr() != z.data_ptr(), "output must not be z")
+    if quant:
+        if scale is None:
+            scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+        else:
+            _dense(scale, "scale", torch.float32, shape[:-1], dev)
+    else:
+        _need(scale is None, "scale needs quant")
+    args = _capi.GdnGatedNormArgs(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype],
+                                  _capi.QUANT_GROUP if quant else _capi.QUANT_NONE, eps, tokens, heads, dim,
+                                  _ptr(output), _ptr(scale))
+
+    def launch():
+        _call(_capi.load().gdn_gated_norm_launch, "gdn_gated_norm_launch", dev, ctypes.byref(args))
+
+    return launch, output, scale
+
+
+def launch_gated_norm(x, z, weight, eps=1e-6, output=None, scale=None, quant: bool = False):
+    """The gated per-head norm; returns ``output``, or with ``quant`` ``(output, scale)``.
+
+    ``x`` and ``z`` are ``[tokens, heads, dim]`` (dim 64, 128 or 256) with a
+    free token stride, or contiguous with more leading dimensions; ``weight``
+    is ``[dim]``.  ``output`` has ``x``'s shape, contiguous, and may be a
+    contiguous ``x`` itself.  With ``quant`` it is ``float8_e4m3fn`` with one
+    fp32 scale per head, ``scale`` ``[..., heads]``.
+    """
+    launch, output, scale = _prepare_gated_norm(x, z, weight, eps, output, scale, quant)
+    launch()
+    return (output, scale) if quant else output
+
+
+def launch_gated_norm_backward(d_output, x, z, weight, eps=1e-6, dx=None, dz=None):
+    """Gradients of ``launch_gated_norm``: ``(dx, dz, d_weight)``; ``d_weight`` is fp32."""
+    shape = x.shape if isinstance(x, torch.Tensor) else None
+    x, z, xs, zs, wdt = _gated_inputs(x, z, weight, eps)
+    tokens, heads, dim = x.shape
+    dev = x.device
+    _need(isinstance(d_output, torch.Tensor) and d_output.shape == shape, f"d_output must have shape {tuple(shape)}")
+    if d_output.dim() > 3:
+        _need(d_output.is_contiguous(), "d_output must be contiguous with more than three dimensions")
+        d_output = d_output.view(-1, heads, dim)
+    dys = _heads(d_output, "d_output", x.dtype, x.shape, dev)
+    if dx is None:
+        dx = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        _dense(dx, "dx", x.dtype, shape, dev)
+    if dz is None:
+        dz = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        _dense(dz, "dz", x.dtype, shape, dev)
+    d_weight = torch.empty(dim, dtype=torch.float32, device=dev)
+    lib = _capi.load()
+    need = int(lib.gdn_gated_norm_backward_workspace_size(tokens, heads, dim))
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = _capi.GdnGatedNormArgs(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype], 0, eps, tokens, heads, dim,
+                                  None, None)
+    g = _capi.GdnNormGradArgs(_ptr(d_output), dys, None, 0, _ptr(dx), _ptr(dz), _ptr(d_weight))
+    _call(lib.gdn_gated_norm_backward_launch, "gdn_gated_norm_backward_launch", dev, ctypes.byref(args),
+          ctypes.byref(g), _ptr(workspace), need)
+    return dx, dz, d_weight
+
+
+@dataclass
+class OutputNorm:
+    """The gated norm that ``launch_gdn(..., out_norm=)`` applies to its output:
+    ``z`` in the output's shape, ``weight`` ``[128]``.  With ``codes``
+    (``float8_e4m3fn``, the output's shape) and ``scale`` (fp32, the shape
+    without its last dimension) the e4m3 form is written there and ``output``
+    keeps the recurrence's own values; without them ``output`` is normed in
+    place."""
+
+    z: torch.Tensor
+    weight: torch.Tensor
+    eps: float = 1e-6
+    codes: torch.Tensor | None = None
+    scale: torch.Tensor | None = None
+
+    def prepare(self, output):
+        """Checks the norm against the ``output`` it will be applied to and
+        returns the call that launches it."""
+        _need((self.codes is None) == (self.scale is None), "codes and scale go together")
+        z = self.z
+        _need(isinstance(z, torch.Tensor) and z.numel() == output.numel(), f"z must have the output's shape {tuple(output.shape)}")
+        if z.shape != output.shape:  # [B, 1, heads, 128] for an output [B, heads, 128], or the other way round
+            _need(z.is_contiguous(), "z must be contiguous unless it has the output's shape")
+            z = z.view(output.shape)
+        if self.codes is None:
+            return _prepare_gated_norm(output, z, self.weight, self.eps, output, None, False)[0]
+        _need(z.numel() == 0 or output.data_ptr() != z.data_ptr(), "z must not be the output")
+        return _prepare_gated_norm(output, z, self.weight, self.eps, self.codes, self.scale, True)[0]
+
+
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        output, summed = launch_add_norm(x, residual, weight, eps)
+        ctx.save_for_backward(summed, weight)
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        return (output, summed) if ctx.has_residual else output
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_output, d_summed=None):
+        summed, weight = ctx.saved_tensors
+        if d_summed is not None:
+            d_summed = d_summed.contiguous()
+        dx, dw = launch_add_norm_backward(d_output.contiguous(), summed, weight, ctx.eps, d_summed)
+        return dx, dx if ctx.has_residual else None, dw.to(weight.dtype), None
+
+
+def add_norm(x, residual, weight, eps=1e-6):
+    """Differentiable ``launch_add_norm``: ``(output, new_residual)``, with
+    gradients for ``x``, ``residual`` and ``weight``."""
+    if residual is None:
+        return _AddNorm.apply(x, None, weight, eps), x
+    return _AddNorm.apply(x, residual, weight, eps)
+
+
+class _GatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, z, weight, eps):
+        ctx.save_for_backward(x, z, weight)
+        ctx.eps = eps
+        return launch_gated_norm(x, z, weight, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_output):
+        x, z, weight = ctx.saved_tensors
+        dx, dz, dw = launch_gated_norm_backward(d_output.contiguous(), x, z, weight, ctx.eps)
+        return dx, dz, dw.to(weight.dtype), None
+
+
+def gated_norm(x, z, weight, eps=1e-6):
+    """Differentiable ``launch_gated_norm``, with gradients for ``x``, ``z`` and ``weight``."""
+    return _GatedNorm.apply(x, z, weight, eps)

@@ -31,7 +31,8 @@ PKG = Path(__file__).resolve().parent
 FIB = PKG / "fib"
 INCLUDE = PKG.parent / "include"
 PACKED_PKG = "kachua_mlsys_b200"  # the package directory's name inside a solution
-MODULES = ("__init__.py", "_build.py", "_capi.py", "decode.py", "prefill.py", "inputs.py", "shard.py")
+MODULES = ("__init__.py", "_build.py", "_capi.py", "decode.py", "prefill.py", "recurrence.py", "norm.py", "inputs.py",
+           "shard.py")
 DEFINITIONS = ("gdn_decode_qk4_v8_d128_k_last", "gdn_prefill_qk4_v8_d128_k_last")
 
 

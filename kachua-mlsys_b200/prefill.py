@@ -106,7 +106,7 @@ PATHS = {"auto": 0, "recurrent": 1, "chunked": 2, "segmented": 3}
 
 def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale=None, output=None,
                new_state=None, workspace: torch.Tensor | None = None, check_seqlens: bool = False,
-               path: str = "auto"):
+               path: str = "auto", out_norm=None):
     """Varlen GDN prefill (destination-passing); returns ``(output, new_state)``.
 
     ``path`` selects the algorithm: ``"auto"`` (token-recurrent kernel for
@@ -115,7 +115,8 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale=None, out
     device buffer of at least ``workspace_bytes(T, N)`` bytes (other head
     counts: ``workspace_bytes(T, N, hv)``).  Head counts other than 4 q/k /
     8 v (q ``[T, HQK, 128]``, v ``[T, HV, 128]``, HV a multiple of HQK) take
-    the same paths.
+    the same paths.  ``out_norm`` (a ``norm.OutputNorm``) applies the gated
+    per-head norm to ``output`` behind the prefill, on the same stream.
     """
     _need(path in PATHS, f"path must be one of {sorted(PATHS)}")
     _need(isinstance(q, torch.Tensor), "q must be a torch.Tensor")
@@ -128,6 +129,7 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale=None, out
     if new_state is None:
         new_state = torch.empty((N, hv, D, D), dtype=torch.float32, device=q.device)
     T, N = validate(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, output, new_state, check_seqlens)
+    norm_output = None if out_norm is None else out_norm.prepare(output)
     lib = _capi.load()
     other_heads = (hqk, hv) != (HQK, HV)
     need = workspace_bytes(T, N, hv)
@@ -148,6 +150,8 @@ def launch_gdn(q, k, v, state, A_log, a, dt_bias, b, cu_seqlens, scale=None, out
         else:
             _capi.check(lib.gdn_prefill_launch(ctypes.byref(args), ws_ptr, need, ctypes.c_void_p(stream)),
                         "gdn_prefill_launch")
+    if norm_output is not None:
+        norm_output()
     return output, new_state
 
 

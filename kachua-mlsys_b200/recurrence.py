@@ -1,0 +1,292 @@
+"""The per-channel gated linear recurrence: packed scan, backward pass, decode step.
+
+    h_t = g_t h_{t-1} + sigmoid(b_t) x_t,   y_t = h_t
+    g_t = exp(-exp(A_log) softplus(a_t + dt_bias))
+
+per channel, with the gates of the delta-rule entry points (``decode`` and
+``prefill``) and, like them, destination-passing: ``launch_scan`` over packed
+sequences (``cu_seqlens`` as ``prefill.launch_gdn``), ``launch_step`` for one
+or a few tokens per sequence (as ``decode.launch_gdn``), and
+``launch_scan_backward`` for training.  ``gated_scan`` is the differentiable
+form.
+
+``x``, ``a`` and ``b`` are ``[T, C]`` bf16, fp16 or fp32, all of one type,
+channels contiguous; the token stride is free, so column blocks of one
+projection's output need no copy.  ``A_log`` and ``dt_bias`` are fp32 ``[C]``,
+states fp32 ``[N, C]``.  The state, the gates and every sum are fp32; outputs
+are rounded once.  Everything runs on the current torch stream of the tensors'
+device, asynchronously.  Errors in arguments raise ``ValueError`` before
+anything launches; bad ``cu_seqlens`` values are reported through
+``prefill.device_status``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _capi
+
+DTYPES = {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16, torch.float32: _capi.DTYPE_F32}
+
+
+def _need(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
+    """Checks a ``[rows, width]`` tensor with contiguous rows; returns its row stride."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.shape != (rows, width):
+        raise ValueError(f"{name} must have shape {(rows, width)}, got {tuple(t.shape)}")
+    stride, inner = t.stride()
+    if width > 1 and inner != 1:
+        raise ValueError(f"{name} must have contiguous rows, got strides {t.stride()}")
+    if rows > 1 and stride < width:
+        raise ValueError(f"{name} must not have overlapping rows, got strides {t.stride()}")
+    return stride if rows > 1 else width
+
+
+def _dense(t, name: str, dtype, shape, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _call(fn, what: str, device, *args) -> None:
+    """``fn(*args, current stream of device)`` with that device current."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _capi.check(rc, what)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
+    """Checks what every entry point takes; returns (rows, channels, x, a and b strides)."""
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x must be a [T, C] tensor")
+    T, C = x.shape
+    dev = x.device
+    _need(dev.type == "cuda" or not require_cuda, "x must be a CUDA tensor (there is no CPU path)")
+    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    _need(C >= 1, "x must have at least one channel")
+    strides = _rows(x, "x", x.dtype, T, C, dev), _rows(a, "a", x.dtype, T, C, dev), _rows(b, "b", x.dtype, T, C, dev)
+    _dense(A_log, "A_log", torch.float32, (C,), dev)
+    _dense(dt_bias, "dt_bias", torch.float32, (C,), dev)
+    return T, C, strides
+
+
+def _seqlens(cu_seqlens, T: int, device, check: bool) -> int:
+    _need(isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1,
+          "cu_seqlens must be a 1-D tensor of N+1 offsets")
+    _need(cu_seqlens.dtype in (torch.int32, torch.int64), "cu_seqlens must be int32 or int64")
+    _need(cu_seqlens.device == device, f"cu_seqlens must be on {device}")
+    _need(cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous")
+    if check:
+        cu = cu_seqlens.to("cpu", torch.int64)
+        _need(int(cu[0]) >= 0, "cu_seqlens[0] must be >= 0")
+        _need(bool((cu[1:] >= cu[:-1]).all()), "cu_seqlens must be non-decreasing")
+        _need(int(cu[-1]) <= T, f"cu_seqlens[-1]={int(cu[-1])} exceeds total tokens {T}")
+    return cu_seqlens.numel() - 1
+
+
+def validate(x, A_log, a, dt_bias, b, cu_seqlens, state, output, new_state, checkpoints=None,
+             check_seqlens: bool = False, require_cuda: bool = True) -> tuple[int, int, int]:
+    """Checks every argument of ``launch_scan``; returns ``(T, N, C)``.
+
+    With ``check_seqlens`` the cu_seqlens values are copied to the host and
+    checked (a device sync).  ``require_cuda=False`` checks only
+    shapes/dtypes/layout (host-side tests).
+    """
+    T, C, _ = _inputs(x, A_log, a, dt_bias, b, require_cuda)
+    dev = x.device
+    N = _seqlens(cu_seqlens, T, dev, check_seqlens)
+    _rows(output, "output", x.dtype, T, C, dev)
+    _dense(new_state, "new_state", torch.float32, (N, C), dev)
+    if state is not None:
+        _dense(state, "state", torch.float32, (N, C), dev)
+        _need(N == 0 or state.data_ptr() != new_state.data_ptr(), "state must not alias new_state")
+    if checkpoints is not None:
+        _dense(checkpoints, "checkpoints", torch.float32, (_checkpoint_rows(T), C), dev)
+    _need(T == 0 or output.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr()),
+          "output must not overlap an input")
+    return T, N, C
+
+
+def _checkpoint_rows(T: int) -> int:
+    return int(_capi.load().gdn_scan_checkpoint_rows(T))
+
+
+def empty_checkpoints(x) -> torch.Tensor:
+    """The buffer that ``launch_scan`` fills for ``launch_scan_backward`` (one
+    fp32 row of channels per 128 packed tokens)."""
+    return torch.empty((_checkpoint_rows(x.shape[0]), x.shape[1]), dtype=torch.float32, device=x.device)
+
+
+def _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, seqs, output, new_state, checkpoints):
+    cu64 = cu_seqlens is not None and cu_seqlens.dtype == torch.int64
+    rows = x.shape[0]
+    return _capi.GdnScanArgs(
+        _ptr(x), _ptr(a), _ptr(b), *strides, _ptr(A_log), _ptr(dt_bias), _ptr(state), _ptr(cu_seqlens),
+        _capi.GDN_SEQLENS_INT64 if cu64 else _capi.GDN_SEQLENS_INT32, DTYPES[x.dtype], rows, seqs, x.shape[1],
+        _ptr(output), 0 if output is None else output.stride(0) if rows > 1 else x.shape[1], _ptr(new_state),
+        _ptr(checkpoints))
+
+
+def launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None, output=None, new_state=None, checkpoints=None,
+                check_seqlens: bool = False):
+    """The recurrence over packed sequences; returns ``(output, new_state)``.
+
+    ``state`` is ``[N, C]`` fp32 (``None``: zero) and must not be
+    ``new_state``; an empty sequence's ``new_state`` row is its ``state`` row.
+    Output rows of tokens that belong to no sequence are zeros.
+    ``checkpoints`` (``empty_checkpoints(x)``) is filled for the backward pass.
+    ``output`` may be row-strided (a column block of a wider buffer) and must
+    not overlap an input.
+    """
+    T, C, strides = _inputs(x, A_log, a, dt_bias, b, True)
+    if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device != x.device:
+        cu_seqlens = cu_seqlens.to(x.device)
+    N = _seqlens(cu_seqlens, T, x.device, check_seqlens)
+    if output is None:
+        output = torch.empty((T, C), dtype=x.dtype, device=x.device)
+    else:
+        _rows(output, "output", x.dtype, T, C, x.device)
+        _need(T == 0 or output.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr()),
+              "output must not overlap an input")
+    if new_state is None:
+        new_state = torch.empty((N, C), dtype=torch.float32, device=x.device)
+    else:
+        _dense(new_state, "new_state", torch.float32, (N, C), x.device)
+    if state is not None:
+        _dense(state, "state", torch.float32, (N, C), x.device)
+        _need(N == 0 or state.data_ptr() != new_state.data_ptr(), "state must not alias new_state")
+    if checkpoints is not None:
+        _dense(checkpoints, "checkpoints", torch.float32, (_checkpoint_rows(T), C), x.device)
+    args = _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, N, output, new_state, checkpoints)
+    _call(_capi.load().gdn_scan_launch, "gdn_scan_launch", x.device, ctypes.byref(args))
+    return output, new_state
+
+
+def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, checkpoints, d_new_state=None, dx=None,
+                         da=None, db=None):
+    """Gradients of ``launch_scan``: ``(dx, da, db, dA_log, d_dt_bias, d_state)``.
+
+    The arguments are those of the forward call and the ``checkpoints`` that it
+    filled; ``d_output`` is ``[T, C]`` of ``x``'s type, ``d_new_state`` fp32
+    ``[N, C]`` (``None``: zero).  ``dx``, ``da``, ``db`` may be given
+    (row-strided, e.g. column blocks of the projection's gradient); ``dA_log``
+    and ``d_dt_bias`` are fp32 ``[C]``, ``d_state`` fp32 ``[N, C]`` (``None``
+    when ``state`` is).  Sums are taken in a fixed order: the same call gives
+    the same bits.
+    """
+    T, C, strides = _inputs(x, A_log, a, dt_bias, b, True)
+    dev = x.device
+    if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device != dev:
+        cu_seqlens = cu_seqlens.to(dev)
+    N = _seqlens(cu_seqlens, T, dev, False)
+    dy_stride = _rows(d_output, "d_output", x.dtype, T, C, dev)
+    _dense(checkpoints, "checkpoints", torch.float32, (_checkpoint_rows(T), C), dev)
+    if state is not None:
+        _dense(state, "state", torch.float32, (N, C), dev)
+    if d_new_state is not None:
+        _dense(d_new_state, "d_new_state", torch.float32, (N, C), dev)
+    grads, grad_strides = [], []
+    for t, name in ((dx, "dx"), (da, "da"), (db, "db")):
+        if t is None:
+            t = torch.empty((T, C), dtype=x.dtype, device=dev)
+        grad_strides.append(_rows(t, name, x.dtype, T, C, dev))
+        _need(T == 0 or t.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr(), d_output.data_ptr()),
+              f"{name} must not overlap an input")
+        grads.append(t)
+    dA_log, d_dt_bias = torch.empty(C, dtype=torch.float32, device=dev), torch.empty(C, dtype=torch.float32, device=dev)
+    d_state = None if state is None else torch.empty((N, C), dtype=torch.float32, device=dev)
+    lib = _capi.load()
+    need = int(lib.gdn_scan_backward_workspace_size(T, N, C))
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    args = _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, N, None, None, checkpoints)
+    g = _capi.GdnScanGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_state), *(_ptr(t) for t in grads), *grad_strides,
+                              _ptr(dA_log), _ptr(d_dt_bias), _ptr(d_state))
+    _call(lib.gdn_scan_backward_launch, "gdn_scan_backward_launch", dev, ctypes.byref(args), ctypes.byref(g),
+          _ptr(workspace), need)
+    return (*grads, dA_log, d_dt_bias, d_state)
+
+
+def launch_step(x, A_log, a, dt_bias, b, state, output=None, new_state=None):
+    """One decode step; returns ``(output, new_state)``.
+
+    ``x``, ``a``, ``b`` are ``[B, C]``, or ``[B, T, C]`` for T tokens per
+    sequence applied in order; ``state`` is ``[B, C]`` fp32 and may be
+    ``new_state`` (in-place update).
+    """
+    _need(isinstance(x, torch.Tensor) and x.dim() in (2, 3), "x must be a [B, C] or [B, T, C] tensor")
+    shape, tokens = x.shape, 1
+    if x.dim() == 3:
+        tokens = shape[1]
+        _need(tokens >= 1, "x must have at least one token per sequence")
+        flat = []
+        for t, name in ((x, "x"), (a, "a"), (b, "b")):
+            _need(isinstance(t, torch.Tensor) and t.shape == shape, f"{name} must have shape {tuple(shape)}")
+            _need(shape[0] <= 1 or tokens <= 1 or t.stride(0) == tokens * t.stride(1),
+                  f"{name} must have evenly spaced tokens, got strides {t.stride()}")
+            flat.append(t.flatten(0, 1))
+        x, a, b = flat
+    rows, C, strides = _inputs(x, A_log, a, dt_bias, b, True)
+    dev, B = x.device, shape[0]
+    _dense(state, "state", torch.float32, (B, C), dev)
+    if output is None:
+        output = torch.empty(shape, dtype=x.dtype, device=dev)
+    else:
+        _dense(output, "output", x.dtype, shape, dev)
+    if new_state is None:
+        new_state = torch.empty_like(state)
+    elif new_state is not state:
+        _dense(new_state, "new_state", torch.float32, (B, C), dev)
+    args = _capi.GdnScanArgs(_ptr(x), _ptr(a), _ptr(b), *strides, _ptr(A_log), _ptr(dt_bias), _ptr(state), None, 0,
+                             DTYPES[x.dtype], rows, B, C, _ptr(output), C, _ptr(new_state), None)
+    _call(_capi.load().gdn_scan_step_launch, "gdn_scan_step_launch", dev, ctypes.byref(args), tokens)
+    return output, new_state
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, A_log, a, dt_bias, b, cu_seqlens, state):
+        checkpoints = empty_checkpoints(x)
+        output, new_state = launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state, checkpoints=checkpoints)
+        ctx.save_for_backward(x, A_log, a, dt_bias, b, cu_seqlens, state, checkpoints)
+        return output, new_state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_output, d_new_state):
+        x, A_log, a, dt_bias, b, cu_seqlens, state, checkpoints = ctx.saved_tensors
+        dx, da, db, dA_log, d_dt_bias, d_state = launch_scan_backward(
+            d_output.contiguous(), x, A_log, a, dt_bias, b, cu_seqlens, state, checkpoints, d_new_state.contiguous())
+        return dx, dA_log, da, d_dt_bias, db, None, d_state
+
+
+def gated_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None):
+    """Differentiable ``launch_scan``: ``(output, new_state)`` with gradients
+    for ``x``, ``A_log``, ``a``, ``dt_bias``, ``b`` and ``state``."""
+    if isinstance(cu_seqlens, torch.Tensor) and isinstance(x, torch.Tensor) and cu_seqlens.device != x.device:
+        cu_seqlens = cu_seqlens.to(x.device)
+    return _GatedScan.apply(x, A_log, a, dt_bias, b, cu_seqlens, state)

@@ -1,0 +1,525 @@
+"""The per-channel gated recurrence against its definition in 64 bits."""
+import ctypes
+
+import pytest
+import torch
+
+from tests import _layer_ref as ref
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+gpu = pytest.mark.gpu
+
+
+def make(lens, C, dtype, device="cpu", state=True, seed=0, tail=0, head=0, memory="mixed", fused=False):
+    """Inputs of packed sequences; ``head`` and ``tail`` tokens belong to none."""
+    gen = torch.Generator().manual_seed(seed)
+    T, N = sum(lens) + head + tail, len(lens)
+    n = lambda *s, scale=1.0: torch.randn(s, generator=gen) * scale  # noqa: E731
+    if fused:
+        p = n(T, 3 * C).to(device, dtype)
+        x, a, b = p[:, :C], p[:, C:2 * C], p[:, 2 * C:]
+    else:
+        x, a, b = (n(T, C).to(device, dtype) for _ in range(3))
+    A_log = torch.log(torch.rand(C, generator=gen) * 15 + 1)
+    lo, hi = {"mixed": (1e-3, 1e-1), "short": (0.5, 4.0)}[memory]
+    step = lo * (hi / lo) ** torch.rand(C, generator=gen)
+    dt_bias = step + torch.log(-torch.expm1(-step))
+    cu = torch.tensor([0] + lens).cumsum(0) + head
+    return dict(x=x, A_log=A_log.to(device), a=a, dt_bias=dt_bias.to(device), b=b, lens=lens, first=head,
+                cu=cu.to(device), state=n(N, C, scale=0.5).to(device) if state else None,
+                dy=n(T, C).to(device, dtype), dns=n(N, C).to(device))
+
+
+def gates(i):
+    return i["x"], i["A_log"], i["a"], i["dt_bias"], i["b"]
+
+
+def values(i, **kw):
+    return ref.scan(*gates(i), i["lens"], i["state"], first=i["first"], **kw)
+
+
+def check_forward(pkg, i, **kw):
+    y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"], **kw)
+    want = values(i)
+    ref.close(y, *want["y"], "y")
+    ref.close(ns, *want["new_state"], "new_state")
+    return y, ns
+
+
+def backward(pkg, i, dns=True, **kw):
+    rec = pkg.recurrence
+    ck = rec.empty_checkpoints(i["x"])
+    rec.launch_scan(*gates(i), i["cu"], i["state"], checkpoints=ck)
+    return rec.launch_scan_backward(i["dy"], *gates(i), i["cu"], i["state"], ck, i["dns"] if dns else None, **kw)
+
+
+def check_backward(pkg, i, dns=True):
+    got = backward(pkg, i, dns)
+    want = values(i, dy=i["dy"], dns=i["dns"] if dns else None)
+    for g, name in zip(got, ("dx", "da", "db", "dA_log", "d_dt_bias", "d_state")):
+        if name == "d_state" and i["state"] is None:
+            assert g is None
+        else:
+            ref.close(g, *want[name], name)
+    return got
+
+
+# lengths that meet the edges of a block of 128 tokens, and the sequences of nothing
+LENS = [[1], [0], [2, 0, 0, 1], [127], [128], [129], [5, 123, 128, 1, 255], [700], [64, 3, 0, 300, 1, 1, 1, 90], [1] * 200]
+
+
+@gpu
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: "x".join(map(str, v))[:24])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_scan_forward_and_backward(pkg, cuda_dev, lens, dtype):
+    i = make(lens, 72, dtype, cuda_dev)
+    check_forward(pkg, i)
+    check_backward(pkg, i)
+
+
+@gpu
+@pytest.mark.parametrize("C", [1, 2, 7, 8, 63, 64, 65, 128, 200, 1001])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_scan_channel_counts(pkg, cuda_dev, C, dtype):
+    i = make([40, 0, 133, 90], C, dtype, cuda_dev, seed=C)
+    check_forward(pkg, i)
+    check_backward(pkg, i)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[9000], [3000, 1, 0, 5200], [2500] * 3], ids=["one", "ragged", "even"])
+@pytest.mark.parametrize("C", [64, 130])
+def test_scan_long(pkg, cuda_dev, lens, C):
+    i = make(lens, C, torch.bfloat16, cuda_dev, seed=3)
+    check_forward(pkg, i)
+    check_backward(pkg, i)
+
+
+@gpu
+def test_scan_many_short_sequences(pkg, cuda_dev):
+    """More sequences than a block could hold offsets for."""
+    lens = [k % 4 for k in range(5000)]
+    i = make(lens, 66, torch.bfloat16, cuda_dev, seed=4)
+    check_forward(pkg, i)
+    check_backward(pkg, i)
+
+
+@gpu
+@pytest.mark.parametrize("state", [True, False])
+@pytest.mark.parametrize("dns", [True, False])
+def test_scan_without_states(pkg, cuda_dev, state, dns):
+    i = make([30, 200], 64, torch.bfloat16, cuda_dev, state=state)
+    check_forward(pkg, i)
+    check_backward(pkg, i, dns)
+
+
+@gpu
+@pytest.mark.parametrize("cu_dtype", [torch.int32, torch.int64])
+def test_scan_seqlens_types_and_cpu_seqlens(pkg, cuda_dev, cu_dtype):
+    i = make([30, 200], 64, torch.bfloat16, cuda_dev)
+    want = check_forward(pkg, i)
+    i["cu"] = i["cu"].to(cu_dtype)
+    for cu in (i["cu"], i["cu"].cpu()):
+        i["cu"] = cu
+        got = check_forward(pkg, i)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("head,tail", [(0, 5), (3, 0), (130, 260), (0, 1000)])
+def test_scan_tokens_of_no_sequence(pkg, cuda_dev, head, tail):
+    """Their rows and gradients are zeros, whatever they hold, and they reach nobody."""
+    i = make([30, 0, 150], 64, torch.bfloat16, cuda_dev, head=head, tail=tail)
+    for k in ("x", "a", "b", "dy"):
+        i[k][:head] = float("nan")
+        i[k][head + 180:] = float("inf")
+    out = torch.full_like(i["x"], 7.0)
+    y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"], output=out)
+    clean = make([30, 0, 150], 64, torch.bfloat16, cuda_dev, head=head, tail=tail)
+    want = values(clean)
+    sl = slice(head, head + 180)
+    ref.close(y[sl], want["y"][0][sl], want["y"][1][sl], "y")
+    ref.close(ns, *want["new_state"], "new_state")
+    assert not y[:head].any() and not y[head + 180:].any()
+    got = backward(pkg, i)
+    wantg = values(clean, dy=clean["dy"], dns=clean["dns"])
+    for g, name in zip(got, ("dx", "da", "db")):
+        assert not g[:head].any() and not g[head + 180:].any(), name
+        ref.close(g[sl], wantg[name][0][sl], wantg[name][1][sl], name)
+    for g, name in zip(got[3:], ("dA_log", "d_dt_bias", "d_state")):
+        assert bool(g.isfinite().all()), name
+
+
+@gpu
+def test_scan_sequences_do_not_leak(pkg, cuda_dev):
+    """NaN and infinity in one sequence leave its neighbours alone, forward and backward."""
+    lens = [40, 100, 3, 200]
+    i = make(lens, 64, torch.bfloat16, cuda_dev)
+    good = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    good_grads = backward(pkg, i)
+    for bad in (float("nan"), float("inf")):
+        j = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in i.items()}
+        j["x"][60] = bad
+        j["state"][1] = bad
+        j["dy"][70] = bad
+        j["dns"][1] = bad
+        y, ns = pkg.recurrence.launch_scan(*gates(j), j["cu"], j["state"])
+        keep = torch.ones(343, dtype=torch.bool, device=cuda_dev)
+        keep[40:140] = False
+        assert torch.equal(y[keep], good[0][keep]) and not y[60].isfinite().any()
+        assert torch.equal(ns[[0, 2, 3]], good[1][[0, 2, 3]])
+        grads = backward(pkg, j)
+        for g, w in zip(grads[:3], good_grads[:3]):
+            assert torch.equal(g[keep], w[keep])
+        assert torch.equal(grads[5][[0, 2, 3]], good_grads[5][[0, 2, 3]])
+
+
+@gpu
+def test_scan_extreme_gates(pkg, cuda_dev):
+    """Gates that open or close entirely; infinite pre-activations are limits."""
+    i = make([300], 64, torch.float32, cuda_dev, memory="short")
+    i["a"][10:20] = 300.0     # g = 0
+    i["a"][50:60] = -300.0    # g = 1
+    i["a"][100] = float("inf")
+    i["a"][101] = -float("inf")
+    i["b"][30:40] = 200.0
+    i["b"][70:80] = -200.0
+    i["b"][110] = float("inf")
+    i["b"][111] = -float("inf")
+    y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    fin = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in i.items()}
+    for k in ("a", "b"):
+        fin[k] = fin[k].clamp(-1e4, 1e4)
+    want = values(fin)
+    ref.close(y, *want["y"], "y")
+    ref.close(ns, *want["new_state"], "new_state")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("C", [64, 72, 65])
+def test_scan_strided_inputs_and_outputs(pkg, cuda_dev, dtype, C):
+    """Column blocks of one projection in, column blocks of a wider buffer out; nothing beside them is touched."""
+    i = make([40, 133], C, dtype, cuda_dev, fused=True)
+    wide = torch.full((173, C + 24), 7.0, dtype=dtype, device=cuda_dev)
+    check_forward(pkg, i, output=wide[:, 16:16 + C])
+    assert bool((wide[:, :16] == 7).all()) and bool((wide[:, 16 + C:] == 7).all())
+    g = torch.full((173, 3 * C + 1), 7.0, dtype=dtype, device=cuda_dev)
+    got = backward(pkg, i, dx=g[:, :C], da=g[:, C:2 * C], db=g[:, 2 * C:3 * C])
+    dense = backward(pkg, i)
+    for a, b in zip(got, dense):
+        assert torch.equal(a, b)
+    assert bool((g[:, 3 * C:] == 7).all())
+
+
+@gpu
+def test_scan_unaligned_base(pkg, cuda_dev):
+    i = make([40, 133], 64, torch.bfloat16, cuda_dev)
+    want = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    for k in ("x", "a", "b"):
+        buf = torch.empty(173 * 64 + 3, dtype=torch.bfloat16, device=cuda_dev)
+        buf[3:] = i[k].flatten()
+        i[k] = buf[3:].view(173, 64)
+    got = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+def test_scan_offsets_past_32_bits(pkg, cuda_dev):
+    C, T, wide = 64, 40000, 65536
+    big = torch.empty((T, wide), dtype=torch.bfloat16, device=cuda_dev)  # 2.6e9 elements
+    i = make([T - 100, 100], C, torch.bfloat16, cuda_dev)
+    want = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    big[:, -C:] = i["x"]
+    i["x"] = big[:, -C:]
+    got = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+def test_scan_chains_like_one_call(pkg, cuda_dev):
+    """A prefix, its state, the rest, then steps: the values of the whole sequence."""
+    i = make([400], 64, torch.float32, cuda_dev)
+    rec, want = pkg.recurrence, values(i)
+    x, A, a, d, b = gates(i)
+    cu = lambda n: torch.tensor([0, n], device=cuda_dev)  # noqa: E731
+    y0, s = rec.launch_scan(x[:150], A, a[:150], d, b[:150], cu(150), i["state"])
+    y1, s = rec.launch_scan(x[150:390], A, a[150:390], d, b[150:390], cu(240), s)
+    ys = []
+    for t in range(390, 397):
+        y, s = rec.launch_step(x[t:t + 1], A, a[t:t + 1], d, b[t:t + 1], s, new_state=s)
+        ys.append(y)
+    y3, s = rec.launch_step(x[None, 397:], A, a[None, 397:], d, b[None, 397:], s)
+    y = torch.cat([y0, y1, *ys, y3[0]])
+    # a split adds one association; the bound leaves a factor of two for that
+    ref.close(y, *want["y"], "y")
+    ref.close(s, *want["new_state"], "new_state")
+
+
+@gpu
+@pytest.mark.parametrize("B", [1, 3, 256])
+@pytest.mark.parametrize("C", [1, 65, 128, 1000, 4096])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_step(pkg, cuda_dev, B, C, dtype):
+    i = make([1] * B, C, dtype, cuda_dev, seed=B)
+    want = values(i)
+    y, ns = pkg.recurrence.launch_step(*gates(i), i["state"])
+    ref.close(y, *want["y"], "y")
+    ref.close(ns, *want["new_state"], "new_state")
+    inplace = i["state"].clone()
+    y2, ns2 = pkg.recurrence.launch_step(*gates(i), inplace, new_state=inplace)
+    assert ns2 is inplace and torch.equal(inplace, ns) and torch.equal(y2, y)
+
+
+@gpu
+def test_step_tokens_and_strides(pkg, cuda_dev):
+    i = make([5] * 7, 96, torch.bfloat16, cuda_dev, fused=True)
+    want = values(i)
+    x, A, a, d, b = gates(i)
+    v = lambda t: t.unflatten(0, (7, 5))  # noqa: E731
+    y, ns = pkg.recurrence.launch_step(v(x), A, v(a), d, v(b), i["state"])
+    assert y.shape == (7, 5, 96)
+    ref.close(y.flatten(0, 1), *want["y"], "y")
+    ref.close(ns, *want["new_state"], "new_state")
+
+
+@gpu
+def test_empty_calls(pkg, cuda_dev):
+    rec = pkg.recurrence
+    z = torch.zeros(0, 64, dtype=torch.bfloat16, device=cuda_dev)
+    v = torch.zeros(64, device=cuda_dev)
+    s = torch.randn(3, 64, device=cuda_dev)
+    cu = torch.zeros(4, dtype=torch.int64, device=cuda_dev)
+    y, ns = rec.launch_scan(z, v, z, v, z, cu, s)
+    assert y.shape == (0, 64) and torch.equal(ns, s)
+    assert not rec.launch_scan(z, v, z, v, z, cu)[1].any()
+    g = rec.launch_scan_backward(z, z, v, z, v, z, cu, s, rec.empty_checkpoints(z), d_new_state=s)
+    assert torch.equal(g[5], s) and not g[3].any() and not g[4].any()
+    x = torch.ones(5, 64, dtype=torch.bfloat16, device=cuda_dev)
+    y, ns = rec.launch_scan(x, v, x, v, x, cu[:1])
+    assert not y.any() and ns.shape == (0, 64)
+    g = rec.launch_scan_backward(x, x, v, x, v, x, cu[:1], None, rec.empty_checkpoints(x))
+    assert not any(t.any() for t in g[:5])
+    y, ns = rec.launch_step(z, v, z, v, z, torch.zeros(0, 64, device=cuda_dev))
+    assert y.shape == (0, 64)
+
+
+@gpu
+def test_scan_is_reproducible_and_uses_the_current_stream(pkg, cuda_dev):
+    i = make([3000, 17, 2000], 256, torch.bfloat16, cuda_dev)
+    y0, n0 = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    g0 = backward(pkg, i)
+    side = torch.cuda.Stream(cuda_dev)
+    side.wait_stream(torch.cuda.current_stream(cuda_dev))
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        j = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in i.items()}
+        for _ in range(4):
+            y, n = pkg.recurrence.launch_scan(*gates(j), j["cu"], j["state"])
+            g = backward(pkg, j)
+    side.synchronize()
+    assert torch.equal(y, y0) and torch.equal(n, n0)
+    for a, b in zip(g, g0):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_two_calls_at_once(pkg, cuda_dev):
+    i, j = (make([2000, 900], 512, torch.bfloat16, cuda_dev, seed=s) for s in (1, 2))
+    want = [backward(pkg, k) for k in (i, j)]
+    streams = [torch.cuda.Stream(cuda_dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(3):
+        for k, (s, inp) in enumerate(zip(streams, (i, j))):
+            with torch.cuda.stream(s):
+                got[k] = backward(pkg, inp)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for a, b in zip(g, w):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_scan_in_two_graphs(pkg, cuda_dev):
+    """Two captured training passes with buffers of their own, replayed in turn on new data."""
+    rec = pkg.recurrence
+    pair = [make([300, 50], 64, torch.bfloat16, cuda_dev, seed=s) for s in (1, 2)]
+    outs, graphs = [], []
+    for i in pair:
+        backward(pkg, i)  # warm up
+    torch.cuda.synchronize()
+    for i in pair:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append((rec.launch_scan(*gates(i), i["cu"], i["state"]), backward(pkg, i)))
+        graphs.append(g)
+    for i in pair:
+        i["x"].neg_()
+        i["dy"].mul_(2)
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for i, ((y, ns), grads) in zip(pair, outs):
+        want = values(i, dy=i["dy"], dns=i["dns"])
+        ref.close(y, *want["y"], "y")
+        ref.close(ns, *want["new_state"], "new_state")
+        for g, name in zip(grads, ("dx", "da", "db", "dA_log", "d_dt_bias", "d_state")):
+            ref.close(g, *want[name], name)
+
+
+@gpu
+def test_gated_scan_gradients(pkg, cuda_dev):
+    """The differentiable form gives the launch functions' gradients, and those follow differences."""
+    i = make([20, 150], 8, torch.float32, cuda_dev, memory="short")
+    leaves = [i[k].clone().requires_grad_() for k in ("x", "A_log", "a", "dt_bias", "b")]
+    s = i["state"].clone().requires_grad_()
+    y, ns = pkg.recurrence.gated_scan(*leaves, i["cu"], s)
+    ((y * i["dy"]).sum() + (ns * i["dns"]).sum()).backward()
+    dx, da, db, dA, ddt, ds = backward(pkg, i)
+    for leaf, want in zip(leaves + [s], (dx, dA, da, ddt, db, ds)):
+        assert torch.equal(leaf.grad, want)
+
+    def loss(**kw):
+        j = {**i, **kw}
+        w = ref.scan(*gates(j), j["lens"], j["state"])
+        return float((w["y"][0] * i["dy"].double()).sum() + (w["new_state"][0] * i["dns"].double()).sum())
+
+    gen = torch.Generator().manual_seed(5)
+    for name, grad in (("x", dx), ("a", da), ("b", db), ("A_log", dA), ("dt_bias", ddt), ("state", ds)):
+        v = torch.randn(grad.shape, generator=gen, dtype=torch.float64).to(cuda_dev)
+        h = 1e-5  # central differences of a 64-bit loss: h^2 of the third derivative, 1e-16 / h of rounding
+        slope = (loss(**{name: i[name].double() + h * v}) - loss(**{name: i[name].double() - h * v})) / (2 * h)
+        scale = float(grad.double().norm() * v.norm()) / grad.numel() ** 0.5
+        assert abs(slope - float((grad.double() * v).sum())) <= 1e-4 * scale, name
+
+
+@gpu
+def test_gated_scan_partial_gradients(pkg, cuda_dev):
+    """Only the state's output is used; an expanded gradient; no state."""
+    i = make([20, 150], 64, torch.bfloat16, cuda_dev, state=False)
+    x = i["x"].clone().requires_grad_()
+    y, ns = pkg.recurrence.gated_scan(x, *gates(i)[1:], i["cu"])
+    ns.sum().backward()
+    j = {**i, "dy": torch.zeros_like(i["dy"]), "dns": torch.ones_like(i["dns"])}
+    assert torch.equal(x.grad, backward(pkg, j)[0])
+    x.grad = None
+    y, ns = pkg.recurrence.gated_scan(x, *gates(i)[1:], i["cu"])
+    y.float().sum().backward()
+    j = {**i, "dy": torch.ones_like(i["dy"])}
+    assert torch.equal(x.grad, backward(pkg, j, dns=False)[0])
+
+
+@gpu
+@pytest.mark.parametrize("cu", [[0, 50, 40], [-5, 50, 90], [0, 50, 91], [0, 1000, 90]], ids=str)
+def test_bad_seqlens_are_reported(pkg, cuda_dev, cu):
+    i = make([50, 40], 64, torch.bfloat16, cuda_dev)
+    i["cu"] = torch.tensor(cu, device=cuda_dev)
+    assert pkg.prefill.device_status(cuda_dev) == 0
+    pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    assert pkg.prefill.device_status(cuda_dev) == pkg._capi.GDN_ERR_DEVICE_BAD_SEQLENS
+    backward(pkg, i)
+    assert pkg.prefill.device_status(cuda_dev) == pkg._capi.GDN_ERR_DEVICE_BAD_SEQLENS
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"], check_seqlens=True)
+    i["cu"] = torch.tensor([0, 50, 90], device=cuda_dev)
+    check_forward(pkg, i)
+    assert pkg.prefill.device_status(cuda_dev) == 0
+
+
+# ---------------------------------------------------------------- refusals --
+def _refuse(pkg, match, i, **kw):
+    args = dict(output=torch.empty_like(i["x"]), new_state=torch.empty(2, 16), require_cuda=False)
+    args.update(kw)
+    with pytest.raises(ValueError, match=match):
+        pkg.recurrence.validate(*gates(i), i["cu"], i["state"], **args)
+
+
+def test_scan_refusals(pkg):
+    i = make([4, 6], 16, torch.bfloat16)
+    ok = dict(output=torch.empty_like(i["x"]), new_state=torch.empty(2, 16), require_cuda=False)
+    assert pkg.recurrence.validate(*gates(i), i["cu"], i["state"], **ok, check_seqlens=True) == (10, 2, 16)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        pkg.recurrence.launch_step(*gates(i), i["state"])
+    _refuse(pkg, "x must be a", {**i, "x": i["x"][0]})
+    _refuse(pkg, "bfloat16, float16 or float32", {**i, "x": i["x"].double()})
+    _refuse(pkg, "a must be torch.bfloat16", {**i, "a": i["a"].float()})
+    _refuse(pkg, "b must have shape", {**i, "b": i["b"][:5]})
+    _refuse(pkg, "contiguous rows", {**i, "a": i["a"].t().contiguous().t()})
+    _refuse(pkg, "overlapping rows", {**i, "a": i["a"][:1].expand(10, 16)})
+    _refuse(pkg, "A_log must be torch.float32", {**i, "A_log": i["A_log"].double()})
+    _refuse(pkg, "dt_bias must have shape", {**i, "dt_bias": i["dt_bias"][:3]})
+    _refuse(pkg, "int32 or int64", {**i, "cu": i["cu"].float()})
+    _refuse(pkg, "N\\+1 offsets", {**i, "cu": i["cu"][:0]})
+    _refuse(pkg, "state must have shape", {**i, "state": i["state"][:1]})
+    _refuse(pkg, "state must be torch.float32", {**i, "state": i["state"].bfloat16()})
+    _refuse(pkg, "must not alias", i, new_state=i["state"])
+    _refuse(pkg, "must not overlap", i, output=i["x"])
+    _refuse(pkg, "checkpoints must have shape", i, checkpoints=torch.empty(3, 16))
+    _refuse(pkg, "exceeds total tokens", {**i, "cu": torch.tensor([0, 4, 11])}, check_seqlens=True)
+    _refuse(pkg, "non-decreasing", {**i, "cu": torch.tensor([0, 6, 4])}, check_seqlens=True)
+
+
+def test_scan_capi_refusals(pkg):
+    """Host-side checks come before any device call, so they answer without a GPU."""
+    lib, C = pkg._capi.load(), pkg._capi
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+
+    def args(**kw):
+        a = C.GdnScanArgs(p, p, p, 16, 16, 16, p, p, None, p, C.GDN_SEQLENS_INT64, C.DTYPE_BF16, 4, 2, 16, p, 16, p + 256, p)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return ctypes.byref(a)
+
+    def grads(**kw):
+        g = C.GdnScanGradArgs(p, 16, None, p, p, p, 16, 16, 16, p, p, None)
+        for k, v in kw.items():
+            setattr(g, k, v)
+        return ctypes.byref(g)
+
+    NULL, SIZE, ALIGN, WS, DTYPE = 1, 2, 3, 4, 6
+    for want, kw in [(NULL, dict(x=None)), (NULL, dict(A_log=None)), (NULL, dict(cu_seqlens=None)), (NULL, dict(output=None)),
+                     (NULL, dict(new_state=None)), (SIZE, dict(total_tokens=-1)), (SIZE, dict(num_seqs=-1)),
+                     (SIZE, dict(channels=0)), (SIZE, dict(channels=1 << 21)), (SIZE, dict(x_stride=15)),
+                     (SIZE, dict(output_stride=15)), (SIZE, dict(state=p + 256)), (ALIGN, dict(x=p + 1)),
+                     (ALIGN, dict(cu_seqlens=p + 4)), (ALIGN, dict(new_state=p + 2)), (DTYPE, dict(dtype=3)),
+                     (DTYPE, dict(cu_seqlens_dtype=2))]:
+        assert lib.gdn_scan_launch(args(**kw), None) == want, kw
+    assert lib.gdn_scan_launch(None, None) == NULL
+    need = lib.gdn_scan_backward_workspace_size(4, 2, 16)
+    assert need > 0 and lib.gdn_scan_backward_workspace_size(-1, 2, 16) == 0
+    for want, kw in [(NULL, dict(dx=None)), (NULL, dict(d_output=None)), (NULL, dict(dA_log=None)), (SIZE, dict(da_stride=3)),
+                     (ALIGN, dict(db=p + 1)), (ALIGN, dict(d_state=p + 2))]:
+        assert lib.gdn_scan_backward_launch(args(), grads(**kw), p, need, None) == want, kw
+    assert lib.gdn_scan_backward_launch(args(), None, p, need, None) == NULL
+    assert lib.gdn_scan_backward_launch(args(checkpoints=None), grads(), p, need, None) == NULL
+    assert lib.gdn_scan_backward_launch(args(), grads(), p, need - 1, None) == WS
+    assert lib.gdn_scan_backward_launch(args(), grads(), None, need, None) == WS
+    step = dict(total_tokens=2, state=p)
+    assert lib.gdn_scan_step_launch(args(**step), 0, None) == SIZE
+    assert lib.gdn_scan_step_launch(args(**step), 2, None) == SIZE
+    assert lib.gdn_scan_step_launch(args(**{**step, "state": None}), 1, None) == NULL
+    assert lib.gdn_scan_checkpoint_rows(0) == 0 and lib.gdn_scan_checkpoint_rows(129) == 2
+
+
+def test_bounds_follow_fp32(pkg):
+    """The oracle's bounds hold for a plain fp32 evaluation, and notice a wrong gate."""
+    i = make([60, 0, 41], 12, torch.float32)
+    want = values(i, dy=i["dy"], dns=i["dns"])
+    x, A_log, a, dt, b = gates(i)
+    sp = torch.nn.functional.softplus(a + dt, threshold=1000.0)
+    g, beta = torch.exp(-A_log.exp() * sp), torch.sigmoid(b)
+    h, ys = i["state"].clone(), []
+    for n, (t0, t1) in enumerate(((0, 60), (60, 60), (60, 101))):
+        for t in range(t0, t1):
+            h[n] = g[t] * h[n] + beta[t] * x[t]
+            ys.append(h[n].clone())
+    y = torch.stack(ys)
+    ref.close(y, *want["y"], "y")
+    ref.close(h, *want["new_state"], "new_state")
+    with pytest.raises(AssertionError):
+        ref.close(y * (1 + 1e-4), *want["y"], "y")
