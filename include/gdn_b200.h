@@ -323,13 +323,10 @@ typedef struct GdnScanGradArgs {
 int gdn_scan_launch(const GdnScanArgs* args, void* stream);
 
 /* The backward pass of gdn_scan_launch: the same args (output and new_state
- * unused) with the checkpoints that the forward call wrote.  The workspace
- * (16-byte aligned) is free again when the call's kernels have run; calls
- * that overlap need one each. */
+ * unused) with the checkpoints that the forward call wrote.  Sums are taken
+ * in a fixed order: the same call gives the same bits. */
 int64_t gdn_scan_checkpoint_rows(int64_t total_tokens);
-size_t gdn_scan_backward_workspace_size(int64_t total_tokens, int64_t num_seqs, int64_t channels);
-int gdn_scan_backward_launch(const GdnScanArgs* args, const GdnScanGradArgs* grads, void* workspace,
-                             size_t workspace_bytes, void* stream);
+int gdn_scan_backward_launch(const GdnScanArgs* args, const GdnScanGradArgs* grads, void* stream);
 
 /* Decode: `tokens` >= 1 tokens for each of num_seqs sequences, total_tokens =
  * num_seqs * tokens rows in sequence order; cu_seqlens and checkpoints are not

@@ -40,7 +40,6 @@ EXPORTED_SYMBOLS = (
     "gdn_prefill_cp_launch",
     "gdn_scan_launch",
     "gdn_scan_checkpoint_rows",
-    "gdn_scan_backward_workspace_size",
     "gdn_scan_backward_launch",
     "gdn_scan_step_launch",
     "gdn_add_norm_launch",
@@ -253,8 +252,7 @@ def load(build_if_needed: bool = True) -> ctypes.CDLL:
         for name, restype, argtypes in (
                 ("gdn_scan_launch", ctypes.c_int, [scan, P]),
                 ("gdn_scan_checkpoint_rows", i64, [i64]),
-                ("gdn_scan_backward_workspace_size", size, [i64, i64, i64]),
-                ("gdn_scan_backward_launch", ctypes.c_int, [scan, scan_grad, P, size, P]),
+                ("gdn_scan_backward_launch", ctypes.c_int, [scan, scan_grad, P]),
                 ("gdn_scan_step_launch", ctypes.c_int, [scan, i64, P]),
                 ("gdn_add_norm_launch", ctypes.c_int, [norm, P]),
                 ("gdn_add_norm_backward_workspace_size", size, [i64, i64]),

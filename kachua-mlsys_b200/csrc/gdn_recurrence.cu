@@ -12,8 +12,10 @@
 // State, gates, sums and gradients are held in fp32; y and dx, da, db are
 // rounded once, when they are stored.
 #include <cuda_fp16.h>
+#include <string.h>
 
 #include "gdn_common.cuh"
+#include "tc05.cuh"
 
 namespace gdn {
 
@@ -35,15 +37,173 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// ------------------------------------------------ two channels at a time --
+// A thread owns two neighbouring channels; sm_100 multiplies and adds such a
+// pair in one instruction (fma.rn.f32x2).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 splat2(float a) { return pack2(a, a); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_keep_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// z -> log2 g = rate softplus(z) of N pairs side by side (a polynomial's
+// constants are then in registers once for all of them), with
+// softplus(z) = max(z, 0) + log1p(u), u = exp(-|z|) in [0, 1].
+// log1p(u) / u is a polynomial, fitted by weighted least squares iterated to
+// the smallest maximal relative error (Lawson): 1.9e-7.  lg2.approx is not
+// usable here: its error near 1 is absolute (2^-22), and softplus of a
+// strongly negative argument is a tiny number whose relative error the
+// recurrence multiplies by its memory.  ex2.approx serves for 2^t: measured,
+// within 1.2 units in the last place for t in [-20, 0], and off by 0.05 to 0.1
+// on average for t in [-0.01, 0], where a decay's memory is long.
+template <int N>
+__device__ __forceinline__ void log2_decays(F2 (&z)[N], F2 (&u)[N], F2 rate) {
+    constexpr float kLog1p[8] = {0.9999998211860657f, -0.4999740421772003f, 0.33275479078292847f, -0.24495463073253632f, 0.17745240032672882f, -0.10768169909715652f, 0.04408962279558182f, -0.008539206348359585f};
+    F2 r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float2 e = unpack2(mul2(z[i], splat2(kLog2e))), v = unpack2(z[i]);
+        u[i] = pack2(ex2_approx(-fabsf(e.x)), ex2_approx(-fabsf(e.y)));
+        z[i] = pack2(max_keep_nan(v.x, 0.0f), max_keep_nan(v.y, 0.0f));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = fma2(splat2(kLog1p[7]), u[i], splat2(kLog1p[6]));
+#pragma unroll
+    for (int d = 5; d >= 0; --d)
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = fma2(r[i], u[i], splat2(kLog1p[d]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = mul2(rate, fma2(u[i], r[i], z[i]));
+}
+__device__ __forceinline__ F2 exp2_2(F2 t) {
+    const float2 v = unpack2(t);
+    return pack2(ex2_approx(v.x), ex2_approx(v.y));
+}
+template <int N>
+__device__ __forceinline__ void decays(F2 (&z)[N], F2 rate) {
+    F2 u[N];
+    log2_decays(z, u, rate);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = exp2_2(z[i]);
+}
+__device__ __forceinline__ F2 sigmoid2(F2 b) {
+    const float2 e = unpack2(mul2(b, splat2(-kLog2e)));
+    const float2 d = unpack2(add2(pack2(ex2_approx(e.x), ex2_approx(e.y)), splat2(1.0f)));
+    return pack2(rcp_approx(d.x), rcp_approx(d.y));
+}
+
+template <typename T>
+__device__ __forceinline__ F2 load_pair(const void* p);  // two neighbouring elements in shared memory
+template <>
+__device__ __forceinline__ F2 load_pair<float>(const void* p) { return *static_cast<const F2*>(p); }
+template <>
+__device__ __forceinline__ F2 load_pair<__half>(const void* p) {
+    const float2 v = __half22float2(*static_cast<const __half2*>(p));
+    return pack2(v.x, v.y);
+}
+template <>
+__device__ __forceinline__ F2 load_pair<__nv_bfloat16>(const void* p) {
+    const uint32_t u = *static_cast<const uint32_t*>(p);
+    return pack2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// Two neighbouring elements of a row; `pairs`: the row starts on a pair's boundary.
+template <typename T>
+__device__ __forceinline__ void store_pair(T* p, F2 v, bool pairs, bool ok0, bool ok1) {
+    const float2 f = unpack2(v);
+    if (pairs && ok1) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float2*>(p) = f;
+        } else {
+            T e[2] = {from_f32<T>(f.x), from_f32<T>(f.y)};
+            *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(e);
+        }
+    } else {
+        if (ok0) p[0] = from_f32<T>(f.x);
+        if (ok1) p[1] = from_f32<T>(f.y);
+    }
+}
+
+// ---------------------------------------------------------------- cluster --
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// 16 bytes into the same shared address of CTA `rank` of the cluster, counted
+// by that CTA's mbarrier at the address of `bar`: neither side needs a fence.
+__device__ __forceinline__ void st_cluster_f4(uint32_t a, uint32_t bar, uint32_t rank, float4 v) {
+    uint32_t ra, rb;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rb) : "r"(bar), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(ra),
+                 "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(rb)
+                 : "memory");
+}
+// The scans' CTA: 16 map warps and a chain warp, 64 channels wide.
+constexpr int kScanCh = 64, kScanWarps = 16, kScanThreads = 32 * (kScanWarps + 1);
+// Tokens per map warp and tile: a thread's inputs of the next tile wait in
+// registers (forward) and what its gates gave in shared memory (backward).
+template <typename T>
+constexpr int kScanPiece = sizeof(T) == 4 ? 4 : 8;
+constexpr int kGradPiece = 4, kGradTile = kScanWarps * kGradPiece;
+constexpr int kScanMaxCluster = 16;
+
 // The carry into every kScanCkpt-th packed token is kept for the backward
-// pass, which recomputes the states between two of them.
-constexpr int kScanCkpt = 128;
+// pass, which recomputes the states of a tile from it.
+constexpr int kScanCkpt = kGradTile;
 
 struct ScanParams {
     const void* x;
     const void* a;
     const void* b;
-    int64_t x_stride, a_stride, b_stride, out_stride;  // elements between tokens
+    uint32_t x_stride, a_stride, b_stride, out_stride;  // BYTES between tokens
     const float* A_log;
     const float* dt_bias;
     const float* state;  // NULL: zero
@@ -54,21 +214,27 @@ struct ScanParams {
     void* out;
     float* new_state;
     float* ckpt;  // NULL: not wanted
+    bool x_pairs, a_pairs, b_pairs, out_pairs;  // rows start on a pair of elements' boundary
 };
 
 struct ScanGradParams {
     const void* dy;
-    int64_t dy_stride, dx_stride, da_stride, db_stride;
+    uint32_t dy_stride, dx_stride, da_stride, db_stride;  // BYTES between tokens
     const float* d_new_state;  // NULL: zero
     void* dx;
     void* da;
     void* db;
     float* d_state;  // NULL: not wanted
-    float* dA_part;  // per-sequence partial sums [seqs, channels], then dA_log, ddt_bias
-    float* dt_part;
     float* dA_log;
     float* ddt_bias;
+    bool dy_pairs, grad_pairs;  // rows start on a pair of elements' boundary (dx, da and db together)
 };
+
+// Row t of a tensor with `stride` bytes between rows (one wide multiply-add).
+template <typename T>
+__device__ __forceinline__ T* row_at(const void* base, int64_t t, uint32_t stride) {
+    return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + static_cast<uint64_t>(static_cast<uint32_t>(t)) * stride);
+}
 
 __device__ __forceinline__ int64_t scan_cu(const ScanParams& p, int64_t n) {
     return p.cu_is_int64 ? static_cast<const int64_t*>(p.cu)[n] : static_cast<const int32_t*>(p.cu)[n];
@@ -97,101 +263,714 @@ __device__ __forceinline__ Gates scan_gates(float rate, float dt_bias, float a, 
     return r;
 }
 
-// Simple form: one thread per (sequence, channel), token by token.
-template <typename T>
-__global__ void __launch_bounds__(128) gdn_scan_kernel(const ScanParams p) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= p.channels) return;
-    const float rate = expf(p.A_log[c]), dtb = p.dt_bias[c];
-    for (int64_t n = blockIdx.y; n < p.seqs; n += gridDim.y) {
-        int64_t t0, t1;
-        scan_bounds(p, n, t0, t1);
-        float h = p.state ? p.state[n * p.channels + c] : 0.0f;
-        for (int64_t t = t0; t < t1; ++t) {
-            if (p.ckpt && t % kScanCkpt == 0) p.ckpt[t / kScanCkpt * p.channels + c] = h;
-            const Gates q = scan_gates(rate, dtb, to_f32(static_cast<const T*>(p.a)[t * p.a_stride + c]),
-                                       to_f32(static_cast<const T*>(p.b)[t * p.b_stride + c]));
-            h = q.g * h + q.beta * to_f32(static_cast<const T*>(p.x)[t * p.x_stride + c]);
-            static_cast<T*>(p.out)[t * p.out_stride + c] = from_f32<T>(h);
+// A piece of the recurrence is an affine map of the state before it,
+// h -> A h + H, as (A0, A1, H0, H1) for a thread's two channels.  A piece in
+// which a sequence starts does not depend on the state before it: A = -0
+// says so (decays are >= +0, and a product keeps the sign).  The fast forms
+// multiply all the same, which drops a finite state; an infinity or a NaN
+// would cross into the next sequence as a NaN, so a chain that ends in one is
+// done again with the forms that select.
+__device__ __forceinline__ bool is_start(float a) { return __float_as_uint(a) == 0x80000000u; }
+__device__ __forceinline__ F2 apply_map(float4 m, F2 h) { return fma2(pack2(m.x, m.y), h, pack2(m.z, m.w)); }
+__device__ __forceinline__ F2 apply_map_select(float4 m, F2 h) {
+    const float2 r = unpack2(apply_map(m, h));
+    return pack2(is_start(m.x) ? m.z : r.x, is_start(m.y) ? m.w : r.y);
+}
+struct Map2 {
+    F2 A, H;
+};
+__device__ __forceinline__ bool has_nan(F2 v) {
+    const float2 f = unpack2(v);
+    return !(f.x == f.x) || !(f.y == f.y);
+}
+__device__ __forceinline__ bool all_finite(F2 v) {
+    const float2 f = unpack2(v);
+    return fabsf(f.x) <= 3.402823466e38f && fabsf(f.y) <= 3.402823466e38f;
+}
+// The product of maps[0], maps[step], ... of n pieces, and to before[32 i] the
+// product of those ahead of piece i (out of line: the slow form).
+__device__ __noinline__ Map2 chain_select(const float4* maps, int n, int step, float4* before) {
+    Map2 r = {splat2(1.0f), splat2(0.0f)};
+    for (int i = 0; i < n; ++i) {
+        const float4 m = maps[i * step];
+        const float2 a = unpack2(r.A), h = unpack2(r.H);
+        before[i * 32] = make_float4(a.x, a.y, h.x, h.y);
+        r.H = apply_map_select(m, r.H);
+        r.A = pack2(is_start(m.x) ? m.x : a.x * m.x, is_start(m.y) ? m.y : a.y * m.y);
+    }
+    return r;
+}
+// The state behind n pieces
+__device__ __noinline__ F2 fold_select(const float4* maps, int n, int step, F2 h) {
+    for (int i = 0; i < n; ++i) h = apply_map_select(maps[i * step], h);
+    return h;
+}
+
+__device__ __forceinline__ int64_t cu_at(const void* cu, bool is64, int64_t n) {
+    return is64 ? static_cast<const int64_t*>(cu)[n] : static_cast<const int32_t*>(cu)[n];
+}
+
+// First sequence that ends behind packed token t (seqs if none), by the whole
+// warp.  Out of line, like everything that only tiles with a sequence's start
+// or end need: the loop over whole tiles has to fit the instruction cache.
+__device__ __noinline__ int seq_of_token(const void* cu, bool is64, int seqs, int64_t t) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = seqs;
+    while (hi - lo > 32) {
+        const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step - 1;
+        const int n = __popc(__ballot_sync(0xffffffffu, i < hi && cu_at(cu, is64, i + 1) <= t));
+        lo += n * step;
+        hi = min(hi, lo + step);
+    }
+    const int i = lo + lane;
+    return lo + __popc(__ballot_sync(0xffffffffu, i < hi && cu_at(cu, is64, i + 1) <= t));
+}
+
+// Which of W (up to 32) tokens from t on start a sequence, end one,
+// belong to one; and the sequence [lo, hi) around the last of them, so that
+// tiles inside it need no look at the offsets.
+struct Spans {
+    uint32_t start, end, covered;
+    int lo, hi;
+};
+template <int W>
+constexpr uint32_t kAllTokens = 0xffffffffu >> (32 - W);
+__device__ __noinline__ Spans find_spans(const void* cu, bool is64, int seqs, int64_t tokens, int64_t t, int width) {
+    const int lane = threadIdx.x & 31;
+    Spans s = {0, 0, 0, 0, 0};
+    const int64_t stop = t + width < tokens ? t + width : tokens;
+    if (t >= stop) return s;
+    for (int n = seq_of_token(cu, is64, seqs, t); n < seqs; n += 32) {
+        int64_t b = stop, e = stop;
+        if (n + lane < seqs) b = cu_at(cu, is64, n + lane), e = cu_at(cu, is64, n + lane + 1);
+        uint32_t st = 0, en = 0, cov = 0;
+        int lo = 0, hi = 0;
+        if (e > b && b < stop && e > t) {
+            if (b >= t) st = 1u << (b - t);
+            if (e <= stop) en = 1u << (e - 1 - t);
+            const int from = b > t ? static_cast<int>(b - t) : 0, to = static_cast<int>((e < stop ? e : stop) - t);
+            cov = (0xffffffffu >> (32 - to)) & (0xffffffffu << from);  // 0 <= from < to <= 32
+            if (e > stop) lo = static_cast<int>(b > 0 ? b : 0), hi = static_cast<int>(e < tokens ? e : tokens);
         }
-        p.new_state[n * p.channels + c] = h;
+        s.start |= __reduce_or_sync(0xffffffffu, st);
+        s.end |= __reduce_or_sync(0xffffffffu, en);
+        s.covered |= __reduce_or_sync(0xffffffffu, cov);
+        s.lo = max(s.lo, __reduce_max_sync(0xffffffffu, lo));
+        s.hi = max(s.hi, __reduce_max_sync(0xffffffffu, hi));
+        if (__shfl_sync(0xffffffffu, b, 31) >= stop) break;
+    }
+    return s;
+}
+// The same, with `s` of an earlier tile: tiles inside one sequence cost two comparisons.
+template <int W>
+__device__ __forceinline__ void token_spans(const ScanParams& p, int64_t t, Spans& s) {
+    if (t > s.lo && t + W < s.hi) {
+        s.start = s.end = 0;
+        s.covered = kAllTokens<W>;
+    } else {
+        s = find_spans(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.tokens, t, W);
     }
 }
 
+// Channels c and c + 1 of a state's row for packed token t's sequence (zeros without a state).
+__device__ __noinline__ F2 state_of_token(const void* cu, bool is64, int seqs, const float* state, int channels, int64_t t,
+                                          int c) {
+    const int n = seq_of_token(cu, is64, seqs, t);
+    if (state == nullptr || n >= seqs) return splat2(0.0f);
+    const float* row = state + static_cast<int64_t>(n) * channels;
+    return pack2(c < channels ? row[c] : 0.0f, c + 1 < channels ? row[c + 1] : 0.0f);
+}
+__device__ __noinline__ void store_state_of_token(const void* cu, bool is64, int seqs, float* state, int channels, int64_t t,
+                                                  int c, F2 h) {
+    const int n = seq_of_token(cu, is64, seqs, t);
+    if (state == nullptr || n >= seqs) return;
+    const float2 v = unpack2(h);
+    float* row = state + static_cast<int64_t>(n) * channels;
+    if (c < channels) row[c] = v.x;
+    if (c + 1 < channels) row[c + 1] = v.y;
+}
+
+// Two neighbouring elements as they are stored, read past the L1 cache.
 template <typename T>
-__global__ void __launch_bounds__(128) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= p.channels) return;
-    const float rate = expf(p.A_log[c]), dtb = p.dt_bias[c];
-    for (int64_t n = blockIdx.y; n < p.seqs; n += gridDim.y) {
+struct RawPair {
+    uint32_t bits;
+};
+template <>
+struct RawPair<float> {
+    uint2 bits;
+};
+template <typename T>
+__device__ __forceinline__ RawPair<T> load_raw(const T* p) {
+    RawPair<T> r;
+    if constexpr (sizeof(T) == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.bits.x), "=r"(r.bits.y) : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.bits) : "l"(p));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ RawPair<T> load_raw_part(const T* p, bool ok0, bool ok1) {
+    RawPair<T> r;
+    T e[2] = {from_f32<T>(0.0f), from_f32<T>(0.0f)};
+    if (ok0) e[0] = p[0];
+    if (ok1) e[1] = p[1];
+    memcpy(&r, e, sizeof(e));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ F2 raw_to_f2(RawPair<T> r) { return load_pair<T>(&r); }
+
+// Sequences without a token pass their state on; bad offsets are reported.
+__device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const float* from, float* to, int c0, int first,
+                                                     int step) {
+    const int c1 = min(p.channels, c0 + kScanCh);
+    for (int64_t n = first; n < p.seqs; n += step) {
         int64_t t0, t1;
         scan_bounds(p, n, t0, t1);
-        float e = d.d_new_state ? d.d_new_state[n * p.channels + c] : 0.0f;
-        float sA = 0.0f, sdt = 0.0f;
-        float before[kScanCkpt];
-        int64_t end = t1;
-        while (end > t0) {
-            int64_t begin = (end - 1) / kScanCkpt * kScanCkpt;
-            float h;
-            if (begin <= t0) {
-                begin = t0;
-                h = p.state ? p.state[n * p.channels + c] : 0.0f;
+        if (t0 == t1 && to)
+            for (int c = c0; c < c1; ++c) to[n * p.channels + c] = from ? from[n * p.channels + c] : 0.0f;
+    }
+}
+
+// The packed scan in one pass over the data.  A cluster of R CTAs takes 64
+// channels and walks the packed tokens, whatever sequences they belong to, R
+// tiles at a time: ragged batches and one long sequence load the GPU alike.
+// A lane owns two channels.
+//   map warp    g and u = beta x of its piece of the tile's tokens, chained
+//               into the maps from the piece's start, to shared memory (its
+//               own words: no other warp reads them but the piece's last);
+//               then the states and outputs of its piece of the tile before.
+//               The next tile's inputs are on their way meanwhile.
+//   chain warp  the tile's W maps chained, their product sent to every CTA of
+//               the cluster (distributed shared memory, counted by an mbarrier
+//               there: no fence, no cluster-wide barrier), and behind all R of
+//               them the state at the tile's start, always chained in the same
+//               order (the same bits on every run).
+// So the gates' arithmetic, which is what the kernel is made of, has a whole
+// tile's time to hide the cluster's exchange behind.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanParams p) {
+    constexpr int W = kScanWarps, kPiece = kScanPiece<T>, kTile = W * kPiece;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ F2 s_in[2][32];  // the state at the tile's start
+    __shared__ __align__(8) uint64_t s_bar[6];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int R = cluster_size(), rank = cluster_rank();
+    float4* maps = reinterpret_cast<float4*>(smem) + lane;  // [2][kTile][32]: of each token, from its piece's start
+    float4* befores = maps + 2 * kTile * 32;                // [2][W][32]: of each piece, from the tile's start
+    float4* ranks = befores + 2 * W * 32;                   // [2][R][32]: the cluster's tiles
+    const int c0 = blockIdx.y * kScanCh, c = c0 + 2 * lane;
+    const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
+    const uint32_t full = tc05::smem_u32(s_bar), ready = full + 16, arrived = full + 32;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            tc05::mbar_init(full + 8 * i, W);
+            tc05::mbar_init(ready + 8 * i, 1);
+            tc05::mbar_init(arrived + 8 * i, 1);
+            tc05::mbar_expect_tx(arrived + 8 * i, R * 512);
+        }
+        tc05::fence_mbar_init();
+    }
+    cluster_arrive();
+    const int tokens = static_cast<int>(p.tokens);
+    const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
+    scan_empty_sequences(p, p.state, p.new_state, c0, rank * blockDim.x + threadIdx.x, R * blockDim.x);
+    cluster_wait();  // every CTA of the cluster runs and has its barriers
+
+    if (warp == W) {
+        F2 carry = splat2(0.0f);
+        for (int k = 0; k < steps; ++k) {
+            const int buf = k & 1, phase = k >> 1 & 1;
+            if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            const float4* last = maps + (buf * kTile + kPiece - 1) * 32;  // a piece's whole map is its last token's
+            float4* before = befores + buf * W * 32;
+            F2 A = splat2(1.0f), H = splat2(0.0f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float4 m = last[w * kPiece * 32];
+                const float2 va = unpack2(A), vh = unpack2(H);
+                before[w * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                H = apply_map(m, H);
+                A = mul2(A, pack2(m.x, m.y));
+            }
+            if (__any_sync(0xffffffffu, has_nan(A) || has_nan(H))) {
+                const Map2 all = chain_select(last, W, kPiece * 32, before);
+                A = all.A, H = all.H;
+            }
+            const float2 va = unpack2(A), vh = unpack2(H);
+            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32);
+            // A slot is written again two tiles on: by then this CTA has every
+            // CTA's map of tile k + 1, sent after that CTA had read tile k's.
+            for (int r = 0; r < R; ++r)
+                st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
+            if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
+            const float4* all = ranks + buf * R * 32;
+            F2 in = carry;
+#pragma unroll 4
+            for (int r = 0; r < rank; ++r) in = apply_map(all[r * 32], in);
+            F2 next = in;
+#pragma unroll 4
+            for (int r = rank; r < R; ++r) next = apply_map(all[r * 32], next);
+            if (__any_sync(0xffffffffu, has_nan(next))) {
+                in = fold_select(all, rank, 32, carry);
+                next = fold_select(all + rank * 32, R - rank, 32, in);
+            }
+            s_in[buf][lane] = in;
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(ready + 8 * buf);
+            carry = next;
+            if (p.ckpt) {
+#pragma unroll
+                for (int i = 0; i < kTile; i += kScanCkpt) {
+                    const int t = (k * R + rank) * kTile + i;
+                    const float2 v = unpack2(i ? apply_map_select(before[i / kPiece * 32], in) : in);
+                    float* ck = p.ckpt + static_cast<int64_t>(t / kScanCkpt) * p.channels;
+                    if (t < tokens && ok0) ck[c] = v.x;
+                    if (t < tokens && ok1) ck[c + 1] = v.y;
+                }
+            }
+        }
+        return;
+    }
+
+    const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
+    const F2 rate = pack2(ok0 ? -kLog2e * expf(p.A_log[c]) : 0.0f, ok1 ? -kLog2e * expf(p.A_log[c + 1]) : 0.0f);
+    const T* x0 = static_cast<const T*>(p.x) + c;
+    const T* a0 = static_cast<const T*>(p.a) + c;
+    const T* b0 = static_cast<const T*>(p.b) + c;
+    T* out0 = static_cast<T*>(p.out) + c;
+    const bool all_channels = c0 + kScanCh <= p.channels;
+    const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && all_channels;
+    constexpr int kBatch = 4;
+    RawPair<T> x[kPiece], a[kPiece], b[kPiece];
+    auto fetch = [&](int k, int from) {  // kBatch tokens of tile k
+        const int t0 = (k * R + rank) * kTile + warp * kPiece;
+        if (whole && k < steps && t0 + kPiece <= tokens) {
+#pragma unroll
+            for (int j = from; j < from + kBatch; ++j) {
+                x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
+                a[j] = load_raw(row_at<const T>(a0, t0 + j, p.a_stride));
+                b[j] = load_raw(row_at<const T>(b0, t0 + j, p.b_stride));
+            }
+        } else {
+#pragma unroll
+            for (int j = from; j < from + kBatch; ++j) {
+                const bool live = k < steps && t0 + j < tokens;
+                x[j] = load_raw_part(row_at<const T>(x0, t0 + j, p.x_stride), live && ok0, live && ok1);
+                a[j] = load_raw_part(row_at<const T>(a0, t0 + j, p.a_stride), live && ok0, live && ok1);
+                b[j] = load_raw_part(row_at<const T>(b0, t0 + j, p.b_stride), live && ok0, live && ok1);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kPiece; i += kBatch) fetch(0, i);
+    Spans span = {0, 0, 0, 0, 0};
+    uint32_t ends = 0;  // of the tile before
+    for (int k = 0; k <= steps; ++k) {
+        if (k < steps) {
+            const int t0 = (k * R + rank) * kTile + warp * kPiece, buf = k & 1;
+            token_spans<kPiece>(p, t0, span);
+            const uint32_t special = span.start | (~span.covered & kAllTokens<kPiece>);
+            float4* m = maps + (buf * kTile + warp * kPiece) * 32;
+            F2 A = splat2(1.0f), H = splat2(0.0f);  // the map up to each token
+#pragma unroll
+            for (int i = 0; i < kPiece; i += kBatch) {
+                F2 z[kBatch], u[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    z[j] = add2(raw_to_f2<T>(a[i + j]), dtb);
+                    u[j] = mul2(sigmoid2(raw_to_f2<T>(b[i + j])), raw_to_f2<T>(x[i + j]));
+                }
+                fetch(k + 1, i);
+                decays(z, rate);
+                auto put = [&](int j) {
+                    const float2 va = unpack2(A), vh = unpack2(H);
+                    m[(i + j) * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                };
+                if (special == 0) {
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        A = mul2(A, z[j]);
+                        H = fma2(z[j], H, u[j]);
+                        put(j);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        F2 before = H;
+                        if (special >> (i + j) & 1) {
+                            A = splat2(-0.0f);
+                            before = state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.state, p.channels,
+                                                    t0 + i + j, c);
+                        } else {
+                            A = mul2(A, z[j]);
+                        }
+                        H = span.covered >> (i + j) & 1 ? fma2(z[j], before, u[j]) : splat2(0.0f);
+                        put(j);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
+        }
+        if (k > 0) {
+            const int buf = (k - 1) & 1, t0 = ((k - 1) * R + rank) * kTile + warp * kPiece;
+            if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            const float4* m = maps + (buf * kTile + warp * kPiece) * 32;
+            const float4 before = befores[(buf * W + warp) * 32];
+            const F2 tile_in = s_in[buf][lane];
+            F2 in = apply_map(before, tile_in), h[kPiece];
+            const bool finite = !__any_sync(0xffffffffu, !all_finite(tile_in) || !all_finite(in));
+            if (finite) {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) h[j] = apply_map(m[j * 32], in);
             } else {
-                h = p.ckpt[begin / kScanCkpt * p.channels + c];
+                in = apply_map_select(before, tile_in);
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
             }
-            for (int64_t t = begin; t < end; ++t) {
-                before[t - begin] = h;
-                const Gates q = scan_gates(rate, dtb, to_f32(static_cast<const T*>(p.a)[t * p.a_stride + c]),
-                                           to_f32(static_cast<const T*>(p.b)[t * p.b_stride + c]));
-                h = q.g * h + q.beta * to_f32(static_cast<const T*>(p.x)[t * p.x_stride + c]);
+            T* out = row_at<T>(out0, t0, p.out_stride);
+            if (ends == 0 && t0 + kPiece <= tokens && p.out_pairs && all_channels) {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) store_pair(row_at<T>(out, j, p.out_stride), h[j], true, true, true);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) {
+                    if (t0 + j < tokens) store_pair(row_at<T>(out, j, p.out_stride), h[j], p.out_pairs, ok0, ok1);
+                    if (ends >> j & 1)
+                        store_state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.new_state, p.channels, t0 + j, c,
+                                             h[j]);
+                }
             }
-            for (int64_t t = end - 1; t >= begin; --t) {
-                const Gates q = scan_gates(rate, dtb, to_f32(static_cast<const T*>(p.a)[t * p.a_stride + c]),
-                                           to_f32(static_cast<const T*>(p.b)[t * p.b_stride + c]));
-                const float x = to_f32(static_cast<const T*>(p.x)[t * p.x_stride + c]);
-                const float G = to_f32(static_cast<const T*>(d.dy)[t * d.dy_stride + c]) + e;
-                e = q.g * G;
-                const float dl = e * before[t - begin];
-                const float da = -dl * rate / (1.0f + expf(-q.z));
-                sA += dl * q.l;
-                sdt += da;
-                static_cast<T*>(d.dx)[t * d.dx_stride + c] = from_f32<T>(G * q.beta);
-                static_cast<T*>(d.da)[t * d.da_stride + c] = from_f32<T>(da);
-                static_cast<T*>(d.db)[t * d.db_stride + c] = from_f32<T>(G * x * q.beta * (1.0f - q.beta));
-            }
-            end = begin;
         }
-        if (d.d_state) d.d_state[n * p.channels + c] = e;
-        d.dA_part[n * p.channels + c] = sA;
-        d.dt_part[n * p.channels + c] = sdt;
+        ends = span.end;
     }
 }
 
-// Rows that belong to no sequence: out rows (and gradients) are zeros.
+// What the gates of a backward tile gave, per token and lane: log2 g, beta,
+// sigmoid(z) and the two inputs that are needed again, x and dy.  A thread
+// reads only what it wrote.
 template <typename T>
-__global__ void gdn_scan_zero_uncovered_kernel(const ScanParams p, T* o0, int64_t s0, T* o1, int64_t s1, T* o2,
-                                               int64_t s2) {
-    int64_t lo = p.seqs > 0 ? scan_cu(p, 0) : 0, hi = p.seqs > 0 ? scan_cu(p, p.seqs) : 0;
-    for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-        if (t >= lo && t < hi) continue;
-        for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
-            o0[t * s0 + c] = from_f32<T>(0.0f);
-            if (o1) o1[t * s1 + c] = from_f32<T>(0.0f);
-            if (o2) o2[t * s2 + c] = from_f32<T>(0.0f);
+struct GradTile {  // 16-bit inputs: 32 bytes
+    static constexpr size_t kBytes = 2 * kGradTile * 32 * 32;
+    float4* base;
+    __device__ GradTile(unsigned char* smem, int lane) : base(reinterpret_cast<float4*>(smem) + lane) {}
+    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<T> x, RawPair<T> dy) {
+        const float2 a = unpack2(t), b = unpack2(beta), c = unpack2(sig);
+        base[2 * i * 32] = make_float4(a.x, a.y, b.x, b.y);
+        base[(2 * i + 1) * 32] = make_float4(c.x, c.y, __uint_as_float(x.bits), __uint_as_float(dy.bits));
+    }
+    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& sig, F2& x, F2& dy) const {
+        const float4 a = base[2 * i * 32], b = base[(2 * i + 1) * 32];
+        t = pack2(a.x, a.y);
+        beta = pack2(a.z, a.w);
+        sig = pack2(b.x, b.y);
+        x = raw_to_f2<T>({__float_as_uint(b.z)});
+        dy = raw_to_f2<T>({__float_as_uint(b.w)});
+    }
+};
+template <>
+struct GradTile<float> {  // 40 bytes
+    static constexpr size_t kBytes = 2 * kGradTile * 32 * 40;
+    float4* base;
+    float2* sigs;
+    __device__ GradTile(unsigned char* smem, int lane)
+        : base(reinterpret_cast<float4*>(smem) + lane),
+          sigs(reinterpret_cast<float2*>(smem + 2 * kGradTile * 32 * 32) + lane) {}
+    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<float> x, RawPair<float> dy) {
+        const float2 a = unpack2(t), b = unpack2(beta);
+        base[2 * i * 32] = make_float4(a.x, a.y, b.x, b.y);
+        base[(2 * i + 1) * 32] = make_float4(__uint_as_float(x.bits.x), __uint_as_float(x.bits.y),
+                                             __uint_as_float(dy.bits.x), __uint_as_float(dy.bits.y));
+        sigs[i * 32] = unpack2(sig);
+    }
+    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& sig, F2& x, F2& dy) const {
+        const float4 a = base[2 * i * 32], b = base[(2 * i + 1) * 32];
+        const float2 c = sigs[i * 32];
+        t = pack2(a.x, a.y);
+        beta = pack2(a.z, a.w);
+        sig = pack2(c.x, c.y);
+        x = pack2(b.x, b.y);
+        dy = pack2(b.z, b.w);
+    }
+};
+
+// The backward pass, built like the forward one, from the last tile to the
+// first.  The gradient that reaches a piece from behind obeys a recurrence of
+// its own, e -> g (dy + e), so a piece has two maps: of the state before it
+// (the tile's own comes from the forward pass's checkpoint) and of the
+// gradient behind it (exchanged over the cluster).  A map warp computes the
+// gates once, keeps what the gradients need of them in shared memory, and
+// writes its piece's gradients a tile later, when both ends are known.  The
+// sums over tokens stay in registers to the end, and are added over the CTA's
+// warps and the cluster's CTAs in order.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
+    constexpr int W = kScanWarps, kPiece = kGradPiece, kTile = kGradTile;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float4 s_ends[2][32];  // the state before the tile, the gradient behind it
+    __shared__ __align__(8) uint64_t s_bar[7];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int R = cluster_size(), rank = cluster_rank();
+    GradTile<T> vals(smem, lane);
+    float4* state_maps = reinterpret_cast<float4*>(smem + GradTile<T>::kBytes) + lane;  // [2][W][32], and then what precedes
+    float4* grad_maps = state_maps + 2 * W * 32;                                        // [2][W][32], and then what follows
+    float4* ranks = grad_maps + 2 * W * 32;                                             // [2][R][32]
+    float4* cta_sums = ranks + 2 * R * 32;  // [R][32], the first CTA's: others write while it still works
+    const int c0 = blockIdx.y * kScanCh, c = c0 + 2 * lane;
+    const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
+    const uint32_t full = tc05::smem_u32(s_bar), ready = full + 16, arrived = full + 32, summed = full + 48;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            tc05::mbar_init(full + 8 * i, W);
+            tc05::mbar_init(ready + 8 * i, 1);
+            tc05::mbar_init(arrived + 8 * i, 1);
+            tc05::mbar_expect_tx(arrived + 8 * i, R * 512);
+        }
+        tc05::mbar_init(summed, 1);
+        tc05::mbar_expect_tx(summed, R * 512);
+        tc05::fence_mbar_init();
+    }
+    cluster_arrive();
+    const int tokens = static_cast<int>(p.tokens), seqs = static_cast<int>(p.seqs);
+    const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
+    scan_empty_sequences(p, d.d_new_state, d.d_state, c0, rank * blockDim.x + threadIdx.x, R * blockDim.x);
+    cluster_wait();  // every CTA of the cluster runs and has its barriers
+    // first token of the CTA's tile of step k; before the first token when there is none left
+    auto tile_start = [&](int k) { return (tiles - 1 - (k * R + rank)) * kTile; };
+
+    F2 sum_A = splat2(0.0f), sum_dt = splat2(0.0f);
+    if (warp == W) {
+        F2 carry = splat2(0.0f);
+        auto checkpoint = [&](int k) {
+            const int t = tile_start(k);
+            if (k >= steps || t < 0) return splat2(0.0f);
+            const float* ck = p.ckpt + static_cast<int64_t>(t / kScanCkpt) * p.channels;
+            return pack2(ok0 ? ck[c] : 0.0f, ok1 ? ck[c + 1] : 0.0f);
+        };
+        F2 state = checkpoint(0);
+        for (int k = 0; k < steps; ++k) {
+            const int buf = k & 1, phase = k >> 1 & 1;
+            const F2 state_in = state;
+            state = checkpoint(k + 1);
+            if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            auto chain = [&](float4* m, bool back) {  // in place: a piece's map makes way for what comes before it
+                Map2 all = {splat2(1.0f), splat2(0.0f)};
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int w = back ? W - 1 - i : i;
+                    const float4 e = m[w * 32];
+                    const float2 va = unpack2(all.A), vh = unpack2(all.H);
+                    m[w * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                    const F2 A = pack2(e.x, e.y);
+                    const float2 r = unpack2(fma2(A, all.H, pack2(e.z, e.w))), a = unpack2(mul2(all.A, A));
+                    all.H = pack2(is_start(e.x) ? e.z : r.x, is_start(e.y) ? e.w : r.y);
+                    all.A = pack2(is_start(e.x) ? e.x : a.x, is_start(e.y) ? e.y : a.y);
+                }
+                return all;
+            };
+            const Map2 all_grad = chain(grad_maps + buf * W * 32, true);
+            const float2 va = unpack2(all_grad.A), vh = unpack2(all_grad.H);
+            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32);
+            // A slot is written again two tiles on: by then this CTA has every
+            // CTA's map of the tile between, sent after that CTA had read this one's.
+            for (int r = 0; r < R; ++r)
+                st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
+            chain(state_maps + buf * W * 32, false);
+            if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
+            const float4* every = ranks + buf * R * 32;
+            F2 in = carry;
+#pragma unroll 4
+            for (int r = 0; r < rank; ++r) in = apply_map(every[r * 32], in);
+            F2 next = in;
+#pragma unroll 4
+            for (int r = rank; r < R; ++r) next = apply_map(every[r * 32], next);
+            if (__any_sync(0xffffffffu, has_nan(next))) {
+                in = fold_select(every, rank, 32, carry);
+                next = fold_select(every + rank * 32, R - rank, 32, in);
+            }
+            const float2 h = unpack2(state_in), e = unpack2(in);
+            s_ends[buf][lane] = make_float4(h.x, h.y, e.x, e.y);
+            __syncwarp();
+            if (lane == 0) tc05::mbar_arrive(ready + 8 * buf);
+            carry = next;
+        }
+    } else {
+        const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
+        const float2 decay = make_float2(ok0 ? expf(p.A_log[c]) : 0.0f, ok1 ? expf(p.A_log[c + 1]) : 0.0f);
+        const F2 rate = pack2(-kLog2e * decay.x, -kLog2e * decay.y), minus_decay = pack2(-decay.x, -decay.y);
+        const bool all_channels = c0 + kScanCh <= p.channels;
+        const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && d.dy_pairs && all_channels;
+        RawPair<T> x[kPiece], a[kPiece], b[kPiece], dy[kPiece];
+        auto fetch = [&](int k) {
+            const int t0 = k < steps ? tile_start(k) + warp * kPiece : -kTile;
+            const T* x0 = static_cast<const T*>(p.x) + c;
+            const T* a0 = static_cast<const T*>(p.a) + c;
+            const T* b0 = static_cast<const T*>(p.b) + c;
+            const T* dy0 = static_cast<const T*>(d.dy) + c;
+            if (whole && t0 >= 0 && t0 + kPiece <= tokens) {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) {
+                    x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
+                    a[j] = load_raw(row_at<const T>(a0, t0 + j, p.a_stride));
+                    b[j] = load_raw(row_at<const T>(b0, t0 + j, p.b_stride));
+                    dy[j] = load_raw(row_at<const T>(dy0, t0 + j, d.dy_stride));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) {
+                    const bool live = t0 >= 0 && t0 + j < tokens;
+                    x[j] = load_raw_part(row_at<const T>(x0, t0 + j, p.x_stride), live && ok0, live && ok1);
+                    a[j] = load_raw_part(row_at<const T>(a0, t0 + j, p.a_stride), live && ok0, live && ok1);
+                    b[j] = load_raw_part(row_at<const T>(b0, t0 + j, p.b_stride), live && ok0, live && ok1);
+                    dy[j] = load_raw_part(row_at<const T>(dy0, t0 + j, d.dy_stride), live && ok0, live && ok1);
+                }
+            }
+        };
+        fetch(0);
+        Spans span = {0, 0, 0, 0, 0}, done = span;
+        for (int k = 0; k <= steps; ++k) {
+            if (k < steps) {
+                const int t0 = tile_start(k) + warp * kPiece, buf = k & 1;
+                if (t0 >= 0)
+                    token_spans<kPiece>(p, t0, span);
+                else
+                    span = {0, 0, 0, 0, 0};
+                const bool special = (span.start | span.end | (~span.covered & kAllTokens<kPiece>)) != 0;
+                F2 z[kPiece], e[kPiece], u[kPiece], in[kPiece];
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) z[j] = add2(raw_to_f2<T>(a[j]), dtb);
+                F2 sig[kPiece];
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) sig[j] = z[j];
+                log2_decays(z, e, rate);
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) {
+                    // sigmoid(z) = 1 / (1 + e) or e / (1 + e), e = exp(-|z|)
+                    const float2 v = unpack2(sig[j]), w = unpack2(e[j]);
+                    const float2 q = make_float2(rcp_approx(1.0f + w.x), rcp_approx(1.0f + w.y));
+                    sig[j] = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
+                    const F2 beta = sigmoid2(raw_to_f2<T>(b[j]));
+                    vals.put(buf * kTile + warp * kPiece + j, z[j], beta, sig[j], x[j], dy[j]);
+                    z[j] = exp2_2(z[j]);
+                    u[j] = mul2(beta, raw_to_f2<T>(x[j]));
+                    in[j] = raw_to_f2<T>(dy[j]);
+                }
+                fetch(k + 1);
+                F2 A = splat2(1.0f), H = splat2(0.0f), B = splat2(1.0f), E = splat2(0.0f);
+                if (!special) {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) {
+                        A = mul2(A, z[j]);
+                        H = fma2(z[j], H, u[j]);
+                    }
+                    B = A;
+#pragma unroll
+                    for (int j = kPiece - 1; j >= 0; --j) E = mul2(z[j], add2(in[j], E));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) {
+                        const bool covered = span.covered >> j & 1, start = span.start >> j & 1;
+                        if (start) H = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
+                        A = start || !covered ? splat2(-0.0f) : mul2(A, z[j]);
+                        H = covered ? fma2(z[j], H, u[j]) : splat2(0.0f);
+                    }
+#pragma unroll
+                    for (int j = kPiece - 1; j >= 0; --j) {
+                        const bool covered = span.covered >> j & 1, end = span.end >> j & 1;
+                        if (end) E = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
+                        B = end || !covered ? splat2(-0.0f) : mul2(B, z[j]);
+                        E = covered ? mul2(z[j], add2(in[j], E)) : splat2(0.0f);
+                    }
+                }
+                const float2 va = unpack2(A), vh = unpack2(H), vb = unpack2(B), ve = unpack2(E);
+                state_maps[(buf * W + warp) * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                grad_maps[(buf * W + warp) * 32] = make_float4(vb.x, vb.y, ve.x, ve.y);
+                __syncwarp();
+                if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
+            }
+            if (k > 0 && tile_start(k - 1) >= 0) {
+                const int buf = (k - 1) & 1, t0 = tile_start(k - 1) + warp * kPiece;
+                if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+                const float4 ends = s_ends[buf][lane];
+                const F2 tile_h = pack2(ends.x, ends.y), tile_e = pack2(ends.z, ends.w);
+                const float4 hm = state_maps[(buf * W + warp) * 32], em = grad_maps[(buf * W + warp) * 32];
+                F2 h = apply_map(hm, tile_h), e = apply_map(em, tile_e);
+                if (__any_sync(0xffffffffu, !all_finite(tile_h) || !all_finite(tile_e))) {
+                    h = apply_map_select(hm, tile_h);
+                    e = apply_map_select(em, tile_e);
+                }
+                const bool special = (done.start | done.end | (~done.covered & kAllTokens<kPiece>)) != 0;
+                F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) {
+                    vals.get(buf * kTile + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
+                    g[j] = exp2_2(t[j]);
+                    if (special && (done.start >> j & 1))
+                        h = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
+                    before[j] = h;
+                    h = fma2(g[j], h, mul2(beta[j], xs[j]));
+                    if (special && !(done.covered >> j & 1)) h = splat2(0.0f);
+                }
+                T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
+                T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
+                T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
+                const bool plain = all_channels && d.grad_pairs && t0 + kPiece <= tokens;
+#pragma unroll
+                for (int j = kPiece - 1; j >= 0; --j) {
+                    if (special && (done.end >> j & 1))
+                        e = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
+                    const F2 G = add2(dys[j], e);
+                    e = mul2(g[j], G);
+                    const F2 dl = mul2(e, before[j]);
+                    F2 vx = mul2(G, beta[j]), va = mul2(mul2(dl, minus_decay), sig[j]);
+                    F2 vb = mul2(mul2(vx, xs[j]), fma2(beta[j], splat2(-1.0f), splat2(1.0f)));
+                    if (special && !(done.covered >> j & 1)) {
+                        vx = va = vb = e = splat2(0.0f);
+                    } else {
+                        sum_A = fma2(dl, t[j], sum_A);
+                        sum_dt = add2(sum_dt, va);
+                    }
+                    if (special && (done.start >> j & 1))
+                        store_state_of_token(p.cu, p.cu_is_int64, seqs, d.d_state, p.channels, t0 + j, c, e);
+                    if (plain) {
+                        store_pair(row_at<T>(dx, j, d.dx_stride), vx, true, true, true);
+                        store_pair(row_at<T>(da, j, d.da_stride), va, true, true, true);
+                        store_pair(row_at<T>(db, j, d.db_stride), vb, true, true, true);
+                    } else if (t0 + j < tokens) {
+                        store_pair(row_at<T>(dx, j, d.dx_stride), vx, d.grad_pairs, ok0, ok1);
+                        store_pair(row_at<T>(da, j, d.da_stride), va, d.grad_pairs, ok0, ok1);
+                        store_pair(row_at<T>(db, j, d.db_stride), vb, d.grad_pairs, ok0, ok1);
+                    }
+                }
+            }
+            done = span;
         }
     }
-}
-
-__global__ void gdn_scan_sum_parts_kernel(const float* a, const float* b, float* oa, float* ob, int64_t n, int channels) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= channels) return;
-    float sa = 0.0f, sb = 0.0f;
-    for (int64_t i = 0; i < n; ++i) {
-        sa += a[i * channels + c];
-        sb += b[i * channels + c];
-    }
-    oa[c] = sa;
-    ob[c] = sb;
+    // sums over the CTA's warps, in order, then over the cluster's CTAs
+    __syncthreads();
+    const float2 va = unpack2(sum_A), vd = unpack2(sum_dt);
+    float4* sums = state_maps;  // nobody reads the maps any more
+    if (warp < W) sums[warp * 32] = make_float4(va.x, va.y, vd.x, vd.y);
+    __syncthreads();
+    if (warp != 0) return;
+    auto add_up = [](const float4* v, int n) {
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < n; ++i) {
+            const float4 e = v[i * 32];
+            s.x += e.x, s.y += e.y, s.z += e.z, s.w += e.w;
+        }
+        return s;
+    };
+    st_cluster_f4(tc05::smem_u32(cta_sums + rank * 32), summed, 0, add_up(sums, W));
+    if (rank != 0) return;
+    if (!tc05::mbar_wait(summed, 0)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+    const float4 s = add_up(cta_sums, R);
+    constexpr float kLn2 = 0.6931471805599453f;  // l = ln 2 log2 g
+    if (ok0) d.dA_log[c] = s.x * kLn2, d.ddt_bias[c] = s.z;
+    if (ok1) d.dA_log[c + 1] = s.y * kLn2, d.ddt_bias[c + 1] = s.w;
 }
 
 // One or a few tokens per sequence: element (sequence, channel) per thread.
@@ -205,10 +984,10 @@ __global__ void __launch_bounds__(128) gdn_scan_step_kernel(const ScanParams p, 
     for (int64_t n = blockIdx.y; n < p.seqs; n += gridDim.y) {
         float h = p.state[n * p.channels + c];
         for (int64_t t = n * steps; t < (n + 1) * steps; ++t) {
-            const Gates q = scan_gates(rate, dtb, to_f32(static_cast<const T*>(p.a)[t * p.a_stride + c]),
-                                       to_f32(static_cast<const T*>(p.b)[t * p.b_stride + c]));
-            h = q.g * h + q.beta * to_f32(static_cast<const T*>(p.x)[t * p.x_stride + c]);
-            static_cast<T*>(p.out)[t * p.out_stride + c] = from_f32<T>(h);
+            const Gates q = scan_gates(rate, dtb, to_f32(row_at<const T>(p.a, t, p.a_stride)[c]),
+                                       to_f32(row_at<const T>(p.b, t, p.b_stride)[c]));
+            h = q.g * h + q.beta * to_f32(row_at<const T>(p.x, t, p.x_stride)[c]);
+            row_at<T>(p.out, t, p.out_stride)[c] = from_f32<T>(h);
         }
         p.new_state[n * p.channels + c] = h;
     }
@@ -219,27 +998,90 @@ static size_t scan_backward_workspace_bytes(int64_t tokens, int64_t seqs, int64_
     return static_cast<size_t>(2 * (seqs > 0 ? seqs : 1) * channels) * sizeof(float);
 }
 
+// `kernel` with gridDim = (cluster, groups of kScanCh channels); `attr` outlives the launch.
+static cudaLaunchConfig_t scan_config(int cluster, int channels, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster, (channels + kScanCh - 1) / kScanCh);
+    cfg.blockDim = dim3(kScanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+template <typename Kernel>
+static cudaError_t allow_cluster(Kernel kernel, size_t smem) {
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))
+        return e;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+// Clusters of `n` CTAs of `kernel` that run at once, asked once per device and size.
+template <typename Kernel>
+static int active_clusters(Kernel kernel, int n, size_t smem, int (*cache)[kScanMaxCluster + 1]) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (cache[dev][n] == 0) {
+        cudaLaunchAttribute attr[1];
+        const cudaLaunchConfig_t cfg = scan_config(n, kScanCh, smem, nullptr, attr);
+        int got = 0;
+        const bool ok = allow_cluster(kernel, smem) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0;
+        if (!ok) (void)cudaGetLastError();
+        cache[dev][n] = ok ? got : -1;
+    }
+    return cache[dev][n];
+}
+template <typename... Params, typename... Args>
+static cudaError_t launch_scan_cluster(void (*kernel)(Params...), int cluster, int channels, size_t smem, cudaStream_t s,
+                                       Args... args) {
+    if (cudaError_t e = allow_cluster(kernel, smem)) return e;
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = scan_config(cluster, channels, smem, s, attr);
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+// CTAs per cluster.  A cluster's CTAs sit in one GPC, so how many clusters run
+// at once depends on their size in steps (of 16 tiles' CTAs on a B200: 33
+// clusters of 4, 22 of 6, 15 of 8 or 9); the size taken is the one with the
+// fewest tiles in a row, waves x tiles / size.  `active` gives the clusters
+// that run at once.
+template <typename Active>
+static int scan_cluster(int64_t tiles, int channels, Active active) {
+    const int64_t groups = (channels + kScanCh - 1) / kScanCh;
+    int best = 1;
+    int64_t best_steps = INT64_MAX;
+    for (int r = 1; r <= kScanMaxCluster && (r == 1 || r <= tiles); ++r) {
+        const int64_t n = active(r);
+        if (n < 1) continue;
+        const int64_t steps = (groups + n - 1) / n * ((tiles + r - 1) / r);
+        if (steps < best_steps) best = r, best_steps = steps;
+    }
+    return best;
+}
+
 template <typename T>
 static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
-    const dim3 grid((p.channels + 127) / 128, static_cast<unsigned>(p.seqs < 65535 ? (p.seqs > 0 ? p.seqs : 1) : 65535));
-    gdn_scan_kernel<T><<<grid, 128, 0, s>>>(p);
-    if (p.tokens > 0)
-        gdn_scan_zero_uncovered_kernel<T><<<static_cast<unsigned>(p.tokens < 1024 ? p.tokens : 1024), 128, 0, s>>>(
-            p, static_cast<T*>(p.out), p.out_stride, nullptr, 0, nullptr, 0);
-    return cudaGetLastError();
+    constexpr int kTile = kScanWarps * kScanPiece<T>;
+    const auto smem = [](int r) { return (2 * kTile + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
+    const int r = scan_cluster((p.tokens + kTile - 1) / kTile, p.channels, [&](int n) {
+        static int cache[64][kScanMaxCluster + 1];
+        return active_clusters(gdn_scan_kernel<T>, n, smem(n), cache);
+    });
+    return launch_scan_cluster(gdn_scan_kernel<T>, r, p.channels, smem(r), s, p);
 }
 
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
-    const unsigned gx = (p.channels + 127) / 128;
-    const dim3 grid(gx, static_cast<unsigned>(p.seqs < 65535 ? (p.seqs > 0 ? p.seqs : 1) : 65535));
-    gdn_scan_backward_kernel<T><<<grid, 128, 0, s>>>(p, d);
-    gdn_scan_sum_parts_kernel<<<gx, 128, 0, s>>>(d.dA_part, d.dt_part, d.dA_log, d.ddt_bias, p.seqs, p.channels);
-    if (p.tokens > 0)
-        gdn_scan_zero_uncovered_kernel<T><<<static_cast<unsigned>(p.tokens < 1024 ? p.tokens : 1024), 128, 0, s>>>(
-            p, static_cast<T*>(d.dx), d.dx_stride, static_cast<T*>(d.da), d.da_stride, static_cast<T*>(d.db),
-            d.db_stride);
-    return cudaGetLastError();
+    const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kScanWarps + 3 * r) * 32 * sizeof(float4); };
+    const int r = scan_cluster((p.tokens + kGradTile - 1) / kGradTile, p.channels, [&](int n) {
+        static int cache[64][kScanMaxCluster + 1];
+        return active_clusters(gdn_scan_backward_kernel<T>, n, smem(n), cache);
+    });
+    return launch_scan_cluster(gdn_scan_backward_kernel<T>, r, p.channels, smem(r), s, p, d);
 }
 
 template <typename T>
@@ -251,6 +1093,12 @@ static cudaError_t launch_scan_step(const ScanParams& p, int64_t steps, cudaStre
 
 static bool dtype_ok(int dtype) { return dtype >= GDN_DTYPE_BF16 && dtype <= GDN_DTYPE_F32; }
 static uintptr_t dtype_bytes(int dtype) { return dtype == GDN_DTYPE_F32 ? 4 : 2; }
+
+// Elements between tokens: the kernels hold the bytes in 32 bits.
+static bool stride_ok(int64_t stride) { return stride >= 0 && stride <= (1 << 29); }
+
+// Every row starts on a boundary of two elements, so a pair is one access.
+static bool rows_in_pairs(const void* q, int64_t stride, uintptr_t es) { return aligned(q, 2 * es) && stride % 2 == 0; }
 
 // Argument checks shared by the three entry points, then the kernel parameters.
 static int scan_setup(const GdnScanArgs* a, ScanParams& p, bool step) {
@@ -265,6 +1113,8 @@ static int scan_setup(const GdnScanArgs* a, ScanParams& p, bool step) {
     if (a->total_tokens > 0 && (!a->x || !a->a || !a->b)) return GDN_ERR_NULL_POINTER;
     if (a->total_tokens > 1 && (a->x_stride < a->channels || a->a_stride < a->channels || a->b_stride < a->channels))
         return GDN_ERR_BAD_SIZE;
+    if (!stride_ok(a->x_stride) || !stride_ok(a->a_stride) || !stride_ok(a->b_stride) || !stride_ok(a->output_stride))
+        return GDN_ERR_BAD_SIZE;
     const uintptr_t es = dtype_bytes(a->dtype);
     if (!aligned(a->x, es) || !aligned(a->a, es) || !aligned(a->b, es) || !aligned(a->output, es) ||
         !aligned(a->A_log, 4) || !aligned(a->dt_bias, 4) || !aligned(a->state, 4) || !aligned(a->new_state, 4) ||
@@ -274,10 +1124,10 @@ static int scan_setup(const GdnScanArgs* a, ScanParams& p, bool step) {
     p.x = a->x;
     p.a = a->a;
     p.b = a->b;
-    p.x_stride = a->x_stride;
-    p.a_stride = a->a_stride;
-    p.b_stride = a->b_stride;
-    p.out_stride = a->output_stride;
+    p.x_stride = static_cast<uint32_t>(a->x_stride * es);
+    p.a_stride = static_cast<uint32_t>(a->a_stride * es);
+    p.b_stride = static_cast<uint32_t>(a->b_stride * es);
+    p.out_stride = static_cast<uint32_t>(a->output_stride * es);
     p.A_log = a->A_log;
     p.dt_bias = a->dt_bias;
     p.state = a->state;
@@ -289,6 +1139,10 @@ static int scan_setup(const GdnScanArgs* a, ScanParams& p, bool step) {
     p.out = a->output;
     p.new_state = a->new_state;
     p.ckpt = a->checkpoints;
+    p.x_pairs = rows_in_pairs(a->x, a->x_stride, es);
+    p.a_pairs = rows_in_pairs(a->a, a->a_stride, es);
+    p.b_pairs = rows_in_pairs(a->b, a->b_stride, es);
+    p.out_pairs = rows_in_pairs(a->output, a->output_stride, es);
     return GDN_OK;
 }
 }  // namespace gdn
@@ -313,19 +1167,15 @@ extern "C" int64_t gdn_scan_checkpoint_rows(int64_t total_tokens) {
     return total_tokens < 0 ? 0 : (total_tokens + kScanCkpt - 1) / kScanCkpt;
 }
 
-extern "C" size_t gdn_scan_backward_workspace_size(int64_t total_tokens, int64_t num_seqs, int64_t channels) {
-    if (total_tokens < 0 || num_seqs < 0 || channels < 1) return 0;
-    return scan_backward_workspace_bytes(total_tokens, num_seqs, channels);
-}
-
-extern "C" int gdn_scan_backward_launch(const GdnScanArgs* a, const GdnScanGradArgs* g, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
+extern "C" int gdn_scan_backward_launch(const GdnScanArgs* a, const GdnScanGradArgs* g, void* stream) {
     if (g == nullptr) return GDN_ERR_NULL_POINTER;
     ScanParams p;
     if (int rc = scan_setup(a, p, false)) return rc;
     if (a->total_tokens > 0 && (!g->d_output || !g->dx || !g->da || !g->db || !a->checkpoints))
         return GDN_ERR_NULL_POINTER;
     if (!g->dA_log || !g->d_dt_bias) return GDN_ERR_NULL_POINTER;
+    if (!stride_ok(g->d_output_stride) || !stride_ok(g->dx_stride) || !stride_ok(g->da_stride) || !stride_ok(g->db_stride))
+        return GDN_ERR_BAD_SIZE;
     if (a->total_tokens > 1 && (g->d_output_stride < a->channels || g->dx_stride < a->channels ||
                                 g->da_stride < a->channels || g->db_stride < a->channels))
         return GDN_ERR_BAD_SIZE;
@@ -333,24 +1183,23 @@ extern "C" int gdn_scan_backward_launch(const GdnScanArgs* a, const GdnScanGradA
     if (!aligned(g->d_output, es) || !aligned(g->dx, es) || !aligned(g->da, es) || !aligned(g->db, es) ||
         !aligned(g->d_new_state, 4) || !aligned(g->d_state, 4) || !aligned(g->dA_log, 4) || !aligned(g->d_dt_bias, 4))
         return GDN_ERR_MISALIGNED;
-    const size_t need = scan_backward_workspace_bytes(a->total_tokens, a->num_seqs, a->channels);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)) return GDN_ERR_WORKSPACE;
     if (int rc = check_device()) return rc;
     ScanGradParams d;
     d.dy = g->d_output;
-    d.dy_stride = g->d_output_stride;
-    d.dx_stride = g->dx_stride;
-    d.da_stride = g->da_stride;
-    d.db_stride = g->db_stride;
+    d.dy_stride = static_cast<uint32_t>(g->d_output_stride * es);
+    d.dx_stride = static_cast<uint32_t>(g->dx_stride * es);
+    d.da_stride = static_cast<uint32_t>(g->da_stride * es);
+    d.db_stride = static_cast<uint32_t>(g->db_stride * es);
     d.d_new_state = g->d_new_state;
     d.dx = g->dx;
     d.da = g->da;
     d.db = g->db;
     d.d_state = g->d_state;
-    d.dA_part = static_cast<float*>(workspace);
-    d.dt_part = d.dA_part + (a->num_seqs > 0 ? a->num_seqs : 1) * a->channels;
     d.dA_log = g->dA_log;
     d.ddt_bias = g->d_dt_bias;
+    d.dy_pairs = rows_in_pairs(g->d_output, g->d_output_stride, es);
+    d.grad_pairs = rows_in_pairs(g->dx, g->dx_stride, es) && rows_in_pairs(g->da, g->da_stride, es) &&
+                   rows_in_pairs(g->db, g->db_stride, es);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = a->dtype == GDN_DTYPE_F32   ? launch_scan_backward<float>(p, d, s)
                           : a->dtype == GDN_DTYPE_F16 ? launch_scan_backward<__half>(p, d, s)

@@ -83,8 +83,9 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 // kWaitMaxPolls polls, whichever comes first, and returns false; callers
 // record GDN_ERR_DEVICE_TIMEOUT and unwind instead of hanging the GPU.  Every
 // wait in this library is on an mbarrier of the waiting CTA, completed by
-// that CTA's own copies or MMAs (never by another CTA or GPU), which take
-// microseconds; 10 ms is far above any legitimate wait.
+// that CTA's own copies or MMAs or by the CTAs of its cluster, which run at
+// the same time (never by another cluster or GPU); these take microseconds,
+// and 10 ms is far above any legitimate wait.
 constexpr uint64_t kWaitLimitNs = 10ull * 1000 * 1000;
 constexpr uint32_t kWaitMaxPolls = 1u << 26;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {

@@ -138,7 +138,7 @@ def _checkpoint_rows(T: int) -> int:
 
 def empty_checkpoints(x) -> torch.Tensor:
     """The buffer that ``launch_scan`` fills for ``launch_scan_backward`` (one
-    fp32 row of channels per 128 packed tokens)."""
+    fp32 row of channels per 64 packed tokens)."""
     return torch.empty((_checkpoint_rows(x.shape[0]), x.shape[1]), dtype=torch.float32, device=x.device)
 
 
@@ -220,14 +220,10 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
         grads.append(t)
     dA_log, d_dt_bias = torch.empty(C, dtype=torch.float32, device=dev), torch.empty(C, dtype=torch.float32, device=dev)
     d_state = None if state is None else torch.empty((N, C), dtype=torch.float32, device=dev)
-    lib = _capi.load()
-    need = int(lib.gdn_scan_backward_workspace_size(T, N, C))
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     args = _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, N, None, None, checkpoints)
     g = _capi.GdnScanGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_state), *(_ptr(t) for t in grads), *grad_strides,
                               _ptr(dA_log), _ptr(d_dt_bias), _ptr(d_state))
-    _call(lib.gdn_scan_backward_launch, "gdn_scan_backward_launch", dev, ctypes.byref(args), ctypes.byref(g),
-          _ptr(workspace), need)
+    _call(_capi.load().gdn_scan_backward_launch, "gdn_scan_backward_launch", dev, ctypes.byref(args), ctypes.byref(g))
     return (*grads, dA_log, d_dt_bias, d_state)
 
 

@@ -481,7 +481,7 @@ def test_scan_capi_refusals(pkg):
             setattr(g, k, v)
         return ctypes.byref(g)
 
-    NULL, SIZE, ALIGN, WS, DTYPE = 1, 2, 3, 4, 6
+    NULL, SIZE, ALIGN, DTYPE = 1, 2, 3, 6
     for want, kw in [(NULL, dict(x=None)), (NULL, dict(A_log=None)), (NULL, dict(cu_seqlens=None)), (NULL, dict(output=None)),
                      (NULL, dict(new_state=None)), (SIZE, dict(total_tokens=-1)), (SIZE, dict(num_seqs=-1)),
                      (SIZE, dict(channels=0)), (SIZE, dict(channels=1 << 21)), (SIZE, dict(x_stride=15)),
@@ -490,20 +490,16 @@ def test_scan_capi_refusals(pkg):
                      (DTYPE, dict(cu_seqlens_dtype=2))]:
         assert lib.gdn_scan_launch(args(**kw), None) == want, kw
     assert lib.gdn_scan_launch(None, None) == NULL
-    need = lib.gdn_scan_backward_workspace_size(4, 2, 16)
-    assert need > 0 and lib.gdn_scan_backward_workspace_size(-1, 2, 16) == 0
     for want, kw in [(NULL, dict(dx=None)), (NULL, dict(d_output=None)), (NULL, dict(dA_log=None)), (SIZE, dict(da_stride=3)),
                      (ALIGN, dict(db=p + 1)), (ALIGN, dict(d_state=p + 2))]:
-        assert lib.gdn_scan_backward_launch(args(), grads(**kw), p, need, None) == want, kw
-    assert lib.gdn_scan_backward_launch(args(), None, p, need, None) == NULL
-    assert lib.gdn_scan_backward_launch(args(checkpoints=None), grads(), p, need, None) == NULL
-    assert lib.gdn_scan_backward_launch(args(), grads(), p, need - 1, None) == WS
-    assert lib.gdn_scan_backward_launch(args(), grads(), None, need, None) == WS
+        assert lib.gdn_scan_backward_launch(args(), grads(**kw), None) == want, kw
+    assert lib.gdn_scan_backward_launch(args(), None, None) == NULL
+    assert lib.gdn_scan_backward_launch(args(checkpoints=None), grads(), None) == NULL
     step = dict(total_tokens=2, state=p)
     assert lib.gdn_scan_step_launch(args(**step), 0, None) == SIZE
     assert lib.gdn_scan_step_launch(args(**step), 2, None) == SIZE
     assert lib.gdn_scan_step_launch(args(**{**step, "state": None}), 1, None) == NULL
-    assert lib.gdn_scan_checkpoint_rows(0) == 0 and lib.gdn_scan_checkpoint_rows(129) == 2
+    assert lib.gdn_scan_checkpoint_rows(0) == 0 and lib.gdn_scan_checkpoint_rows(129) == 3
 
 
 def test_bounds_follow_fp32(pkg):
