@@ -186,8 +186,9 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t a, uint32_t bar, uint32_t
                  "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(rb)
                  : "memory");
 }
-// The scans' CTA: 16 map warps and a chain warp, 64 channels wide.
-constexpr int kScanCh = 64, kScanWarps = 16, kScanThreads = 32 * (kScanWarps + 1);
+// The scans' CTA: 15 map warps and a chain warp (four warps to a scheduler,
+// so 128 registers a thread), 64 channels wide.
+constexpr int kScanCh = 64, kScanWarps = 15, kScanThreads = 32 * (kScanWarps + 1);
 // Tokens per map warp and tile: a thread's inputs of the next tile wait in
 // registers (forward) and what its gates gave in shared memory (backward).
 template <typename T>
@@ -524,7 +525,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
 #pragma unroll
                 for (int i = 0; i < kTile; i += kScanCkpt) {
                     const int t = (k * R + rank) * kTile + i;
-                    const float2 v = unpack2(i ? apply_map_select(before[i / kPiece * 32], in) : in);
+                    F2 at = in;
+                    if (i) {  // the token before it: its piece's start, and on from there
+                        at = apply_map_select(before[(i - 1) / kPiece * 32], at);
+                        at = apply_map_select(maps[(buf * kTile + i - 1) * 32], at);
+                    }
+                    const float2 v = unpack2(at);
                     float* ck = p.ckpt + static_cast<int64_t>(t / kScanCkpt) * p.channels;
                     if (t < tokens && ok0) ck[c] = v.x;
                     if (t < tokens && ok1) ck[c + 1] = v.y;

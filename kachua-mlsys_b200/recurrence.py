@@ -138,7 +138,7 @@ def _checkpoint_rows(T: int) -> int:
 
 def empty_checkpoints(x) -> torch.Tensor:
     """The buffer that ``launch_scan`` fills for ``launch_scan_backward`` (one
-    fp32 row of channels per 64 packed tokens)."""
+    fp32 row of channels per 60 packed tokens)."""
     return torch.empty((_checkpoint_rows(x.shape[0]), x.shape[1]), dtype=torch.float32, device=x.device)
 
 

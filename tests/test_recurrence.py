@@ -64,8 +64,8 @@ def check_backward(pkg, i, dns=True):
     return got
 
 
-# lengths that meet the edges of a block of 128 tokens, and the sequences of nothing
-LENS = [[1], [0], [2, 0, 0, 1], [127], [128], [129], [5, 123, 128, 1, 255], [700], [64, 3, 0, 300, 1, 1, 1, 90], [1] * 200]
+# lengths that meet the edges of the kernels' tiles (60 and 120 tokens), and sequences of nothing
+LENS = [[1], [0], [2, 0, 0, 1], [59], [60], [61], [120], [121], [127], [128], [129], [5, 123, 128, 1, 255], [700], [64, 3, 0, 300, 1, 1, 1, 90], [1] * 200]
 
 
 @gpu
