@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "gdn_common.cuh"
 #include "tc05.cuh"
 
@@ -908,49 +910,54 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                     h = apply_map_select(hm, tile_h);
                     e = apply_map_select(em, tile_e);
                 }
-                const bool special = (done.start | done.end | (~done.covered & kAllTokens<kPiece>)) != 0;
-                F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
+                // whole pieces inside one sequence go without a branch
+                auto finish = [&](auto inside) {
+                    constexpr bool kInside = decltype(inside)::value;
+                    F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
 #pragma unroll
-                for (int j = 0; j < kPiece; ++j) {
-                    vals.get(buf * kTile + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
-                    g[j] = exp2_2(t[j]);
-                    if (special && (done.start >> j & 1))
-                        h = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
-                    before[j] = h;
-                    h = fma2(g[j], h, mul2(beta[j], xs[j]));
-                    if (special && !(done.covered >> j & 1)) h = splat2(0.0f);
-                }
-                T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
-                T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
-                T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
-                const bool plain = all_channels && d.grad_pairs && t0 + kPiece <= tokens;
+                    for (int j = 0; j < kPiece; ++j) {
+                        vals.get(buf * kTile + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
+                        g[j] = exp2_2(t[j]);
+                    }
 #pragma unroll
-                for (int j = kPiece - 1; j >= 0; --j) {
-                    if (special && (done.end >> j & 1))
-                        e = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
-                    const F2 G = add2(dys[j], e);
-                    e = mul2(g[j], G);
-                    const F2 dl = mul2(e, before[j]);
-                    F2 vx = mul2(G, beta[j]), va = mul2(mul2(dl, minus_decay), sig[j]);
-                    F2 vb = mul2(mul2(vx, xs[j]), fma2(beta[j], splat2(-1.0f), splat2(1.0f)));
-                    if (special && !(done.covered >> j & 1)) {
-                        vx = va = vb = e = splat2(0.0f);
-                    } else {
-                        sum_A = fma2(dl, t[j], sum_A);
-                        sum_dt = add2(sum_dt, va);
+                    for (int j = 0; j < kPiece; ++j) {
+                        if (!kInside && (done.start >> j & 1))
+                            h = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
+                        before[j] = h;
+                        h = fma2(g[j], h, mul2(beta[j], xs[j]));
+                        if (!kInside && !(done.covered >> j & 1)) h = splat2(0.0f);
                     }
-                    if (special && (done.start >> j & 1))
-                        store_state_of_token(p.cu, p.cu_is_int64, seqs, d.d_state, p.channels, t0 + j, c, e);
-                    if (plain) {
-                        store_pair(row_at<T>(dx, j, d.dx_stride), vx, true, true, true);
-                        store_pair(row_at<T>(da, j, d.da_stride), va, true, true, true);
-                        store_pair(row_at<T>(db, j, d.db_stride), vb, true, true, true);
-                    } else if (t0 + j < tokens) {
-                        store_pair(row_at<T>(dx, j, d.dx_stride), vx, d.grad_pairs, ok0, ok1);
-                        store_pair(row_at<T>(da, j, d.da_stride), va, d.grad_pairs, ok0, ok1);
-                        store_pair(row_at<T>(db, j, d.db_stride), vb, d.grad_pairs, ok0, ok1);
+                    T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
+                    T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
+                    T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
+#pragma unroll
+                    for (int j = kPiece - 1; j >= 0; --j) {
+                        if (!kInside && (done.end >> j & 1))
+                            e = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
+                        const F2 G = add2(dys[j], e);
+                        e = mul2(g[j], G);
+                        const F2 dl = mul2(e, before[j]);
+                        F2 vx = mul2(G, beta[j]), va = mul2(mul2(dl, minus_decay), sig[j]);
+                        F2 vb = mul2(mul2(vx, xs[j]), fma2(beta[j], splat2(-1.0f), splat2(1.0f)));
+                        if (!kInside && !(done.covered >> j & 1)) {
+                            vx = va = vb = e = splat2(0.0f);
+                        } else {
+                            sum_A = fma2(dl, t[j], sum_A);
+                            sum_dt = add2(sum_dt, va);
+                        }
+                        if (!kInside && (done.start >> j & 1))
+                            store_state_of_token(p.cu, p.cu_is_int64, seqs, d.d_state, p.channels, t0 + j, c, e);
+                        if (kInside || t0 + j < tokens) {
+                            store_pair(row_at<T>(dx, j, d.dx_stride), vx, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
+                            store_pair(row_at<T>(da, j, d.da_stride), va, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
+                            store_pair(row_at<T>(db, j, d.db_stride), vb, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
+                        }
                     }
-                }
+                };
+                if ((done.start | done.end) == 0 && done.covered == kAllTokens<kPiece> && all_channels && d.grad_pairs)
+                    finish(std::true_type{});
+                else
+                    finish(std::false_type{});
             }
             done = span;
         }
