@@ -201,6 +201,8 @@ _lock = threading.Lock()
 def load(build_if_needed: bool = True) -> ctypes.CDLL:
     """Load (building first if needed) the C-ABI library and declare its signatures."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -1026,35 +1026,25 @@ static cudaLaunchConfig_t scan_config(int cluster, int channels, size_t smem, cu
     cfg.numAttrs = 1;
     return cfg;
 }
+// Clusters of `n` CTAs of `kernel` that run at once (-1: none), asked once per
+// device and size; the kernel's attributes are set with it, for `most` bytes of
+// shared memory.
 template <typename Kernel>
-static cudaError_t allow_cluster(Kernel kernel, size_t smem) {
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)))
-        return e;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-}
-// Clusters of `n` CTAs of `kernel` that run at once, asked once per device and size.
-template <typename Kernel>
-static int active_clusters(Kernel kernel, int n, size_t smem, int (*cache)[kScanMaxCluster + 1]) {
+static int active_clusters(Kernel kernel, int n, size_t smem, size_t most, int (*cache)[kScanMaxCluster + 1]) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
     if (cache[dev][n] == 0) {
         cudaLaunchAttribute attr[1];
         const cudaLaunchConfig_t cfg = scan_config(n, kScanCh, smem, nullptr, attr);
         int got = 0;
-        const bool ok = allow_cluster(kernel, smem) == cudaSuccess &&
-                        cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0;
+        const bool ok =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) == cudaSuccess &&
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+            cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0;
         if (!ok) (void)cudaGetLastError();
         cache[dev][n] = ok ? got : -1;
     }
     return cache[dev][n];
-}
-template <typename... Params, typename... Args>
-static cudaError_t launch_scan_cluster(void (*kernel)(Params...), int cluster, int channels, size_t smem, cudaStream_t s,
-                                       Args... args) {
-    if (cudaError_t e = allow_cluster(kernel, smem)) return e;
-    cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = scan_config(cluster, channels, smem, s, attr);
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
 // CTAs per cluster.  A cluster's CTAs sit in one GPC, so how many clusters run
@@ -1065,7 +1055,7 @@ static cudaError_t launch_scan_cluster(void (*kernel)(Params...), int cluster, i
 template <typename Active>
 static int scan_cluster(int64_t tiles, int channels, Active active) {
     const int64_t groups = (channels + kScanCh - 1) / kScanCh;
-    int best = 1;
+    int best = 0;
     int64_t best_steps = INT64_MAX;
     for (int r = 1; r <= kScanMaxCluster && (r == 1 || r <= tiles); ++r) {
         const int64_t n = active(r);
@@ -1076,25 +1066,33 @@ static int scan_cluster(int64_t tiles, int channels, Active active) {
     return best;
 }
 
+// Launches `kernel` in clusters of the best size; smem(r) bytes for size r.
+template <typename Smem, typename... Params, typename... Args>
+static cudaError_t launch_scan_clusters(void (*kernel)(Params...), int (*cache)[kScanMaxCluster + 1], int64_t tiles,
+                                        int channels, Smem smem, cudaStream_t s, Args... args) {
+    const int r = scan_cluster(tiles, channels, [&](int n) {
+        return active_clusters(kernel, n, smem(n), smem(kScanMaxCluster), cache);
+    });
+    if (r == 0) return cudaErrorInvalidConfiguration;
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = scan_config(r, channels, smem(r), s, attr);
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 template <typename T>
 static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
     constexpr int kTile = kScanWarps * kScanPiece<T>;
+    static int cache[64][kScanMaxCluster + 1];
     const auto smem = [](int r) { return (2 * kTile + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
-    const int r = scan_cluster((p.tokens + kTile - 1) / kTile, p.channels, [&](int n) {
-        static int cache[64][kScanMaxCluster + 1];
-        return active_clusters(gdn_scan_kernel<T>, n, smem(n), cache);
-    });
-    return launch_scan_cluster(gdn_scan_kernel<T>, r, p.channels, smem(r), s, p);
+    return launch_scan_clusters(gdn_scan_kernel<T>, cache, (p.tokens + kTile - 1) / kTile, p.channels, smem, s, p);
 }
 
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
+    static int cache[64][kScanMaxCluster + 1];
     const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kScanWarps + 3 * r) * 32 * sizeof(float4); };
-    const int r = scan_cluster((p.tokens + kGradTile - 1) / kGradTile, p.channels, [&](int n) {
-        static int cache[64][kScanMaxCluster + 1];
-        return active_clusters(gdn_scan_backward_kernel<T>, n, smem(n), cache);
-    });
-    return launch_scan_cluster(gdn_scan_backward_kernel<T>, r, p.channels, smem(r), s, p, d);
+    return launch_scan_clusters(gdn_scan_backward_kernel<T>, cache, (p.tokens + kGradTile - 1) / kGradTile, p.channels, smem,
+                                s, p, d);
 }
 
 template <typename T>

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _capi
-from .recurrence import DTYPES, _call, _dense, _need, _ptr, _rows
+from .recurrence import DTYPES, _call, _dense, _fault, _need, _ptr, _rows
 
 QUANT = {None: _capi.QUANT_NONE, "row": _capi.QUANT_ROW, "group": _capi.QUANT_GROUP}
 GROUP = 128
@@ -30,19 +30,24 @@ HEAD_DIMS = (64, 128, 256)
 
 
 def _weight(weight, width: int, dtype, device) -> int:
-    _need(isinstance(weight, torch.Tensor), "weight must be a torch.Tensor")
-    _need(weight.dtype in (torch.float32, dtype), f"weight must be float32 or {dtype}, got {weight.dtype}")
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in (torch.float32, dtype):
+        raise ValueError(f"weight must be float32 or {dtype}, got {getattr(weight, 'dtype', type(weight))}")
     _dense(weight, "weight", weight.dtype, (width,), device)
     return DTYPES[weight.dtype]
 
 
 def _row_inputs(x, weight, eps) -> tuple[int, int, int]:
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x must be a [rows, width] tensor")
-    _need(x.device.type == "cuda", "x must be a CUDA tensor (there is no CPU path)")
-    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a [rows, width] tensor")
+    if x.device.type != "cuda":
+        raise ValueError("x must be a CUDA tensor (there is no CPU path)")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
     rows, width = x.shape
-    _need(1 <= width <= MAX_WIDTH, f"rows must have 1 to {MAX_WIDTH} elements, got {width}")
-    _need(eps >= 0, "eps must be >= 0")
+    if not 1 <= width <= MAX_WIDTH:
+        raise ValueError(f"rows must have 1 to {MAX_WIDTH} elements, got {width}")
+    if not eps >= 0:
+        raise ValueError("eps must be >= 0")
     return rows, width, _weight(weight, width, x.dtype, x.device)
 
 
@@ -59,8 +64,10 @@ def launch_add_norm(x, residual, weight, eps=1e-6, output=None, new_residual=Non
     """
     rows, width, wdt = _row_inputs(x, weight, eps)
     dev = x.device
-    _need(quant in QUANT, f"quant must be None, 'row' or 'group', got {quant!r}")
-    _need(quant != "group" or width % GROUP == 0, f"group scales need a width that is a multiple of {GROUP}, got {width}")
+    if quant not in QUANT:
+        raise ValueError(f"quant must be None, 'row' or 'group', got {quant!r}")
+    if quant == "group" and width % GROUP:
+        raise ValueError(f"group scales need a width that is a multiple of {GROUP}, got {width}")
     x_stride = _rows(x, "x", x.dtype, rows, width, dev)
     res_stride = 0
     if residual is not None:
@@ -122,33 +129,43 @@ def launch_add_norm_backward(d_output, new_residual, weight, eps=1e-6, d_new_res
 
 def _heads(t, name: str, dtype, shape, device) -> int:
     """Checks a [tokens, heads, dim] tensor whose tokens are contiguous; returns the token stride."""
-    _need(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
-    _need(t.shape == shape, f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+        _fault(t, name, dtype, shape, device)
     tokens, heads, dim = shape
-    s = t.stride()
-    _need(s[2] == 1 and (heads == 1 or s[1] == dim), f"{name} must have contiguous heads, got strides {s}")
-    _need(tokens <= 1 or s[0] >= heads * dim, f"{name} must not have overlapping tokens, got strides {s}")
-    return s[0] if tokens > 1 else heads * dim
+    step, head, inner = t.stride()
+    if inner != 1 or (head != dim and heads > 1):
+        raise ValueError(f"{name} must have contiguous heads, got strides {t.stride()}")
+    if tokens <= 1:
+        return heads * dim
+    if step < heads * dim:
+        raise ValueError(f"{name} must not have overlapping tokens, got strides {t.stride()}")
+    return step
 
 
 def _gated_inputs(x, z, weight, eps):
     """x and z as [tokens, heads, dim] with their token strides, and the weight's type."""
-    _need(isinstance(x, torch.Tensor) and x.dim() >= 3, "x must be a [tokens, heads, dim] tensor")
-    _need(x.device.type == "cuda", "x must be a CUDA tensor (there is no CPU path)")
-    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    _need(isinstance(z, torch.Tensor) and z.shape == x.shape, f"z must have the shape of x, {tuple(x.shape)}")
+    if not isinstance(x, torch.Tensor) or x.dim() < 3:
+        raise ValueError("x must be a [tokens, heads, dim] tensor")
+    if x.device.type != "cuda":
+        raise ValueError("x must be a CUDA tensor (there is no CPU path)")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if not isinstance(z, torch.Tensor) or z.shape != x.shape:
+        raise ValueError(f"z must have the shape of x, {tuple(x.shape)}")
     heads, dim = x.shape[-2:]
-    _need(dim in HEAD_DIMS, f"the head dim must be one of {HEAD_DIMS}, got {dim}")
-    _need(1 <= heads <= 4096, f"x must have 1 to 4096 heads, got {heads}")
-    _need(eps >= 0, "eps must be >= 0")
+    if dim not in HEAD_DIMS:
+        raise ValueError(f"the head dim must be one of {HEAD_DIMS}, got {dim}")
+    if not 1 <= heads <= 4096:
+        raise ValueError(f"x must have 1 to 4096 heads, got {heads}")
+    if not eps >= 0:
+        raise ValueError("eps must be >= 0")
     if x.dim() > 3:  # [batch, tokens, heads, dim]
         _need(x.is_contiguous() and z.is_contiguous(), "x and z must be contiguous with more than three dimensions")
         x, z = x.view(-1, heads, dim), z.view(-1, heads, dim)
-    _need(x.shape[0] * heads <= 0x7FFF0000, "too many heads in one call")
-    xs, zs = _heads(x, "x", x.dtype, x.shape, x.device), _heads(z, "z", x.dtype, x.shape, x.device)
-    return x, z, xs, zs, _weight(weight, dim, x.dtype, x.device)
+    shape, dev = x.shape, x.device
+    if shape[0] * heads > 0x7FFF0000:
+        raise ValueError("too many heads in one call")
+    return x, z, _heads(x, "x", x.dtype, shape, dev), _heads(z, "z", x.dtype, shape, dev), _weight(weight, dim, x.dtype, dev)
 
 
 def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):

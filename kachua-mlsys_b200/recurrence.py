@@ -35,44 +35,49 @@ def _need(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
+def _fault(t, name: str, dtype, shape, device) -> None:
+    """Says what keeps ``t`` from being a tensor of that type, device and shape."""
+    _need(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
+    _need(t.shape == shape, f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+# The checks below run on every call, a decode step's among them: messages are
+# made only when there is something to say.
 def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
     """Checks a ``[rows, width]`` tensor with contiguous rows; returns its row stride."""
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.shape != (rows, width):
-        raise ValueError(f"{name} must have shape {(rows, width)}, got {tuple(t.shape)}")
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != (rows, width):
+        _fault(t, name, dtype, (rows, width), device)
     stride, inner = t.stride()
-    if width > 1 and inner != 1:
+    if inner != 1 and width > 1:
         raise ValueError(f"{name} must have contiguous rows, got strides {t.stride()}")
-    if rows > 1 and stride < width:
+    if rows <= 1:
+        return width
+    if stride < width:
         raise ValueError(f"{name} must not have overlapping rows, got strides {t.stride()}")
-    return stride if rows > 1 else width
+    return stride
 
 
 def _dense(t, name: str, dtype, shape, device) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+        _fault(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn, what: str, device, *args) -> None:
     """``fn(*args, current stream of device)`` with that device current."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _capi.check(rc, what)
 
@@ -83,13 +88,17 @@ def _ptr(t):
 
 def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
     """Checks what every entry point takes; returns (rows, channels, x, a and b strides)."""
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x must be a [T, C] tensor")
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a [T, C] tensor")
+    dtype, dev = x.dtype, x.device
     T, C = x.shape
-    dev = x.device
-    _need(dev.type == "cuda" or not require_cuda, "x must be a CUDA tensor (there is no CPU path)")
-    _need(x.dtype in DTYPES, f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    _need(C >= 1, "x must have at least one channel")
-    strides = _rows(x, "x", x.dtype, T, C, dev), _rows(a, "a", x.dtype, T, C, dev), _rows(b, "b", x.dtype, T, C, dev)
+    if require_cuda and dev.type != "cuda":
+        raise ValueError("x must be a CUDA tensor (there is no CPU path)")
+    if dtype not in DTYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
+    if C < 1:
+        raise ValueError("x must have at least one channel")
+    strides = _rows(x, "x", dtype, T, C, dev), _rows(a, "a", dtype, T, C, dev), _rows(b, "b", dtype, T, C, dev)
     _dense(A_log, "A_log", torch.float32, (C,), dev)
     _dense(dt_bias, "dt_bias", torch.float32, (C,), dev)
     return T, C, strides
@@ -234,20 +243,22 @@ def launch_step(x, A_log, a, dt_bias, b, state, output=None, new_state=None):
     sequence applied in order; ``state`` is ``[B, C]`` fp32 and may be
     ``new_state`` (in-place update).
     """
-    _need(isinstance(x, torch.Tensor) and x.dim() in (2, 3), "x must be a [B, C] or [B, T, C] tensor")
+    if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3):
+        raise ValueError("x must be a [B, C] or [B, T, C] tensor")
     shape, tokens = x.shape, 1
+    B = shape[0]
     if x.dim() == 3:
         tokens = shape[1]
         _need(tokens >= 1, "x must have at least one token per sequence")
         flat = []
         for t, name in ((x, "x"), (a, "a"), (b, "b")):
             _need(isinstance(t, torch.Tensor) and t.shape == shape, f"{name} must have shape {tuple(shape)}")
-            _need(shape[0] <= 1 or tokens <= 1 or t.stride(0) == tokens * t.stride(1),
+            _need(B <= 1 or tokens <= 1 or t.stride(0) == tokens * t.stride(1),
                   f"{name} must have evenly spaced tokens, got strides {t.stride()}")
             flat.append(t.flatten(0, 1))
         x, a, b = flat
     rows, C, strides = _inputs(x, A_log, a, dt_bias, b, True)
-    dev, B = x.device, shape[0]
+    dev = x.device
     _dense(state, "state", torch.float32, (B, C), dev)
     if output is None:
         output = torch.empty(shape, dtype=x.dtype, device=dev)
@@ -257,8 +268,9 @@ def launch_step(x, A_log, a, dt_bias, b, state, output=None, new_state=None):
         new_state = torch.empty_like(state)
     elif new_state is not state:
         _dense(new_state, "new_state", torch.float32, (B, C), dev)
-    args = _capi.GdnScanArgs(_ptr(x), _ptr(a), _ptr(b), *strides, _ptr(A_log), _ptr(dt_bias), _ptr(state), None, 0,
-                             DTYPES[x.dtype], rows, B, C, _ptr(output), C, _ptr(new_state), None)
+    args = _capi.GdnScanArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), *strides, A_log.data_ptr(), dt_bias.data_ptr(),
+                             state.data_ptr(), None, 0, DTYPES[x.dtype], rows, B, C, output.data_ptr(), C,
+                             new_state.data_ptr(), None)
     _call(_capi.load().gdn_scan_step_launch, "gdn_scan_step_launch", dev, ctypes.byref(args), tokens)
     return output, new_state
 
