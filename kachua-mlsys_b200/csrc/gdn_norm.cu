@@ -15,6 +15,8 @@
 // (one 16-byte vector of a 16-bit type).
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 namespace gdn {
 
 constexpr float kFp8Max = 448.0f;
@@ -68,53 +70,66 @@ struct GatedNormGradParams {
     float* part;
 };
 
-// 8 consecutive elements as floats; `left` elements are inside the row.
+// 8 consecutive elements as they are stored.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int left, float (&f)[8]) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const T* e = reinterpret_cast<const T*>(&u);
+struct Raw8 {
+    uint4 v[sizeof(T) / 2];
+};
+// VEC: the row is whole vectors on 16-byte boundaries, so `left` (the elements
+// from p to the row's end) is a multiple of 8.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int left) {
+    Raw8<T> r = {};
+    if constexpr (VEC) {
+        if (left > 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
-        } else {
-            const float4 u = reinterpret_cast<const float4*>(p)[0], v = reinterpret_cast<const float4*>(p)[1];
-            f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
         }
     } else {
+        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < left ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            if (i < left) e[i] = p[i];
     }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, F2 (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = load_pair<T>(reinterpret_cast<const T*>(&r) + 2 * i);
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, bool vec, int left, const float (&f)[8]) {
-    if (vec && left >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            uint4 u;
-            T* e = reinterpret_cast<T*>(&u);
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int left, const F2 (&f)[4]) {
+    Raw8<T> r;
+    T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
-            *reinterpret_cast<uint4*>(p) = u;
-        } else {
-            reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(f[i]);
+        e[2 * i] = from_f32<T>(v.x);
+        e[2 * i + 1] = from_f32<T>(v.y);
+    }
+    if constexpr (VEC) {
+        if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = from_f32<T>(f[i]);
+            if (i < left) p[i] = e[i];
     }
 }
 
-__device__ __forceinline__ void store8_e4m3(uint8_t* p, bool vec, int left, const float (&f)[8], float inv) {
+template <bool VEC>
+__device__ __forceinline__ void store8_e4m3(uint8_t* p, int left, const F2 (&f)[4], float inv) {
     uint2 u;
     uint16_t* h = reinterpret_cast<uint16_t*>(&u);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    if (vec && left >= 8) {
-        *reinterpret_cast<uint2*>(p) = u;
+        h[i] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[i], splat2(inv))), __NV_SATFINITE, __NV_E4M3);
+    if constexpr (VEC) {
+        if (left > 0) *reinterpret_cast<uint2*>(p) = u;
     } else {
         const uint8_t* e = reinterpret_cast<const uint8_t*>(&u);
 #pragma unroll
@@ -123,17 +138,15 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* p, bool vec, int left, cons
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_weight8(const void* w, bool f32, int col, bool vec, int left, float (&f)[8]) {
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weight8(const void* w, bool f32, int col, int left, F2 (&f)[4]) {
     if (f32)
-        load8(static_cast<const float*>(w) + col, vec, left, f);
+        unpack8(load8<float, VEC>(static_cast<const float*>(w) + col, left), f);
     else
-        load8(static_cast<const T*>(w) + col, vec, left, f);
+        unpack8(load8<T, VEC>(static_cast<const T*>(w) + col, left), f);
 }
 
-// A maximum that keeps a NaN (fmaxf drops it): a row that holds one gets a NaN scale.
-__device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
-
+// Maxima keep a NaN (fmaxf drops it): a row that holds one gets a NaN scale.
 template <int W>
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
@@ -143,15 +156,20 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <int W>
 __device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = W / 2; o > 0; o >>= 1) v = max_keep_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-
-__device__ __forceinline__ float abs_max8(const float (&y)[8]) {
-    float m = fabsf(y[0]);
+__device__ __forceinline__ float abs_max8(const F2 (&y)[4], float m) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(y[i]));
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(y[i]);
+        m = max_keep_nan(m, max_keep_nan(fabsf(v.x), fabsf(v.y)));
+    }
     return m;
+}
+__device__ __forceinline__ float sum2(F2 v) {
+    const float2 f = unpack2(v);
+    return f.x + f.y;
 }
 
 // Sum (or maximum) over a row's blockDim.x threads, in the same order on every
@@ -166,115 +184,119 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
     v = r[0];
-    for (int w = 1; w < warps; ++w) v = MAX ? max_nan(v, r[w]) : v + r[w];
+    for (int w = 1; w < warps; ++w) v = MAX ? max_keep_nan(v, r[w]) : v + r[w];
     return v;
 }
 
 // blockDim = (threads per row, rows per CTA); thread i holds the row's
 // vectors i, i + blockDim.x, ...
-template <typename T, int VPT>
+template <typename T, int VPT, bool VEC>
 __global__ void __launch_bounds__(1024) gdn_add_norm_kernel(const NormParams p) {
     __shared__ float red_sum[32], red_max[32];
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const bool live = row < p.rows;
+    const int width = row < p.rows ? p.width : 0;
     const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    const T* res = static_cast<const T*>(p.residual) + row * p.residual_stride;
-    float r[VPT][8];
-    float ss = 0.0f;
+    const T* res = static_cast<const T*>(p.residual) + (p.residual ? row * p.residual_stride : 0);
+    const int64_t out = row * p.width;
+    Raw8<T> rx[VPT], rr[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int col = (threadIdx.x + j * blockDim.x) * 8;
-        const int left = live ? p.width - col : 0;
-        load8(x + col, p.vec, left, r[j]);
+        rx[j] = load8<T, VEC>(x + col, width - col);
+        rr[j] = load8<T, VEC>(res + col, p.residual ? width - col : 0);
     }
-    if (p.residual) {
+    F2 r[VPT][4], ss = splat2(0.0f);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (threadIdx.x + j * blockDim.x) * 8;
-            const int left = live ? p.width - col : 0;
-            float f[8];
-            load8(res + col, p.vec, left, f);
+    for (int j = 0; j < VPT; ++j) {
+        const int col = (threadIdx.x + j * blockDim.x) * 8;
+        F2 f[4];
+        unpack8(rx[j], r[j]);
+        unpack8(rr[j], f);
+        if (p.residual) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[j][i] += f[i];
-            store8(static_cast<T*>(p.new_residual) + row * p.width + col, p.vec, left, r[j]);
+            for (int i = 0; i < 4; ++i) r[j][i] = add2(r[j][i], f[i]);
+            store8<T, VEC>(static_cast<T*>(p.new_residual) + out + col, width - col, r[j]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss = fma2(r[j][i], r[j][i], ss);
     }
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(r[j][i], r[j][i], ss);
-    ss = row_reduce<false>(ss, red_sum);
-    const float rstd = rsqrtf(ss / static_cast<float>(p.width) + p.eps);
+    const float rstd = rsqrtf(row_reduce<false>(sum2(ss), red_sum) / static_cast<float>(p.width) + p.eps);
     float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8;
-        const int left = live ? p.width - col : 0;
-        float w[8];
-        load_weight8<T>(p.weight, p.weight_f32, col, p.vec, left, w);
+        const int col = (threadIdx.x + j * blockDim.x) * 8, left = width - col;
+        F2 w[4];
+        load_weight8<T, VEC>(p.weight, p.weight_f32, col, left, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[j][i] *= rstd * w[i];
+        for (int i = 0; i < 4; ++i) r[j][i] = mul2(mul2(r[j][i], splat2(rstd)), w[i]);
         if (p.quant == 0) {
-            store8(static_cast<T*>(p.out) + row * p.width + col, p.vec, left, r[j]);
+            store8<T, VEC>(static_cast<T*>(p.out) + out + col, left, r[j]);
         } else if (p.quant == 2) {  // 16 threads hold a group's 128 channels
-            const float amax = max_nan(lanes_max<16>(left > 0 ? abs_max8(r[j]) : 0.0f), kAmaxMin);
-            if (left > 0) {
-                store8_e4m3(static_cast<uint8_t*>(p.out) + row * p.width + col, p.vec, left, r[j], kFp8Max / amax);
-                if ((threadIdx.x & 15) == 0) p.scale[row * (p.width / kQuantGroup) + col / kQuantGroup] = amax / kFp8Max;
-            }
+            const float amax = lanes_max<16>(left > 0 ? abs_max8(r[j], kAmaxMin) : kAmaxMin);
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out + col, left, r[j], kFp8Max / amax);
+            if (left > 0 && (threadIdx.x & 15) == 0)
+                p.scale[row * (p.width / kQuantGroup) + col / kQuantGroup] = amax / kFp8Max;
         } else if (left > 0) {
-            m = max_nan(m, abs_max8(r[j]));
+            m = abs_max8(r[j], m);
         }
     }
     if (p.quant == 1) {
-        const float amax = max_nan(row_reduce<true>(m, red_max), kAmaxMin);
+        const float amax = max_keep_nan(row_reduce<true>(m, red_max), kAmaxMin), inv = kFp8Max / amax;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int col = (threadIdx.x + j * blockDim.x) * 8;
-            const int left = live ? p.width - col : 0;
-            store8_e4m3(static_cast<uint8_t*>(p.out) + row * p.width + col, p.vec, left, r[j], kFp8Max / amax);
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out + col, width - col, r[j], inv);
         }
-        if (live && threadIdx.x == 0) p.scale[row] = amax / kFp8Max;
+        if (width > 0 && threadIdx.x == 0) p.scale[row] = amax / kFp8Max;
     }
 }
 
 // blockDim = (threads per row, 1); CTA k takes rows k, k + gridDim.x, ... and
-// keeps its share of dweight in registers.
-template <typename T, int VPT>
-__global__ void __launch_bounds__(1024) gdn_add_norm_backward_kernel(const NormParams p, const NormGradParams d) {
+// keeps its share of dweight in registers.  The next row is on its way while
+// one is worked on (up to two vectors a thread).
+template <typename T, int VPT, bool VEC>
+__global__ void __launch_bounds__(VPT == 4 ? 1024 : 512, VPT == 1 ? 2 : 1) gdn_add_norm_backward_kernel(const NormParams p, const NormGradParams d) {
     __shared__ float red[2][2][32];
-    float dw[VPT][8], w[VPT][8];
+    F2 dw[VPT][4], w[VPT][4];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int col = (threadIdx.x + j * blockDim.x) * 8;
-        load_weight8<T>(p.weight, p.weight_f32, col, p.vec, p.width - col, w[j]);
+        load_weight8<T, VEC>(p.weight, p.weight_f32, col, p.width - col, w[j]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) dw[j][i] = splat2(0.0f);
     }
     const float inv_width = 1.0f / static_cast<float>(p.width);
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-        const T* dy = static_cast<const T*>(d.dy) + row * d.dy_stride;
-        float r[VPT][8], g[VPT][8];
-        float ss = 0.0f, dot = 0.0f;
+    Raw8<T> rx[VPT], ry[VPT], rd[VPT];
+    auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int col = (threadIdx.x + j * blockDim.x) * 8;
-            load8(x + col, p.vec, p.width - col, r[j]);
-            load8(dy + col, p.vec, p.width - col, g[j]);
+            const int col = (threadIdx.x + j * blockDim.x) * 8, left = row < p.rows ? p.width - col : 0;
+            rx[j] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.x_stride + col, left);
+            ry[j] = load8<T, VEC>(static_cast<const T*>(d.dy) + row * d.dy_stride + col, left);
+            rd[j] = load8<T, VEC>(static_cast<const T*>(d.dr) + (d.dr ? row * d.dr_stride + col : 0), d.dr ? left : 0);
         }
+    };
+    constexpr bool kAhead = false;
+    if (kAhead) fetch(blockIdx.x);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        if (!kAhead) fetch(row);
+        F2 r[VPT][4], g[VPT][4], o[VPT][4], ss2 = splat2(0.0f), dot2 = splat2(0.0f);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j)
+        for (int j = 0; j < VPT; ++j) {
+            unpack8(rx[j], r[j]);
+            unpack8(ry[j], g[j]);
+            unpack8(rd[j], o[j]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                ss = fmaf(r[j][i], r[j][i], ss);
-                dot = fmaf(g[j][i] * w[j][i], r[j][i], dot);
+            for (int i = 0; i < 4; ++i) {
+                ss2 = fma2(r[j][i], r[j][i], ss2);
+                dot2 = fma2(mul2(g[j][i], w[j][i]), r[j][i], dot2);
             }
+        }
+        if (kAhead) fetch(row + gridDim.x);
         // both sums in one exchange; the buffers alternate, so a fast warp's
         // next row cannot overwrite what a slow warp still reads
-        ss = lanes_sum<32>(ss);
-        dot = lanes_sum<32>(dot);
+        float ss = lanes_sum<32>(sum2(ss2)), dot = lanes_sum<32>(sum2(dot2));
         const int warps = blockDim.x >> 5;
         if (warps > 1) {
             if ((threadIdx.x & 31) == 0) red[turn][0][threadIdx.x >> 5] = ss, red[turn][1][threadIdx.x >> 5] = dot;
@@ -283,32 +305,22 @@ __global__ void __launch_bounds__(1024) gdn_add_norm_backward_kernel(const NormP
             for (int k = 0; k < warps; ++k) ss += red[turn][0][k], dot += red[turn][1][k];
         }
         const float rstd = rsqrtf(ss * inv_width + p.eps);
-        const float back = dot * rstd * rstd * rstd * inv_width;
+        const F2 rstd2 = splat2(rstd), back = splat2(-dot * rstd * rstd * rstd * inv_width);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int col = (threadIdx.x + j * blockDim.x) * 8;
-            const int left = p.width - col;
-            float o[8];
-            if (d.dr) {
-                load8(static_cast<const T*>(d.dr) + row * d.dr_stride + col, p.vec, left, o);
-            } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                dw[j][i] = fma2(g[j][i], mul2(r[j][i], rstd2), dw[j][i]);
+                o[j][i] = add2(o[j][i], fma2(mul2(g[j][i], w[j][i]), rstd2, mul2(r[j][i], back)));
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                dw[j][i] = fmaf(g[j][i], r[j][i] * rstd, dw[j][i]);
-                o[i] += fmaf(g[j][i] * w[j][i], rstd, -r[j][i] * back);
-            }
-            store8(static_cast<T*>(d.dx) + row * p.width + col, p.vec, left, o);
+            store8<T, VEC>(static_cast<T*>(d.dx) + row * p.width + col, p.width - col, o[j]);
         }
     }
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int col = (threadIdx.x + j * blockDim.x) * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (col + i < p.width) d.part[static_cast<int64_t>(blockIdx.x) * p.width + col + i] = dw[j][i];
+        store8<float, VEC>(d.part + static_cast<int64_t>(blockIdx.x) * p.width + col, p.width - col, dw[j]);
     }
 }
 
@@ -325,78 +337,108 @@ __global__ void __launch_bounds__(1024) gdn_sum_columns_kernel(const float* part
     if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < width) out[blockIdx.x * 32 + threadIdx.y] = s;
 }
 
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.0f / (1.0f + __expf(-z)); }
-
-// LANES = head dim / 8 threads per head; item = (token, head).
-template <typename T, int LANES>
+// LANES = head dim / 8 threads per head; item = (token, head), kGatedItems of
+// them per thread.
+constexpr int kGatedItems = 2;
+template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormParams p) {
-    constexpr int kHeadDim = LANES * 8;
-    const unsigned item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    constexpr int kHeadDim = LANES * 8, kGroups = 256 / LANES;
     const int col = (threadIdx.x % LANES) * 8;
-    const int left = item < p.items ? 8 : 0;
-    const unsigned token = item / p.heads, head = item - token * p.heads;
-    const int64_t in = static_cast<int64_t>(head) * kHeadDim + col, o = static_cast<int64_t>(item) * kHeadDim + col;
-    float x[8], z[8], w[8];
-    load8(static_cast<const T*>(p.x) + token * p.x_stride + in, p.vec, left, x);
-    load8(static_cast<const T*>(p.z) + token * p.z_stride + in, p.vec, left, z);
-    load_weight8<T>(p.weight, p.weight_f32, col, p.vec, 8, w);
-    float ss = 0.0f;
+    Raw8<T> rx[kGatedItems], rz[kGatedItems];
+    unsigned items[kGatedItems];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-    const float rstd = rsqrtf(lanes_sum<LANES>(ss) * (1.0f / kHeadDim) + p.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * w[i] * (z[i] * sigmoid_f(z[i]));
-    if (!p.quant) {
-        store8(static_cast<T*>(p.out) + o, p.vec, left, x);
-        return;
+    for (int n = 0; n < kGatedItems; ++n) {
+        const unsigned item = (blockIdx.x * kGatedItems + n) * kGroups + threadIdx.x / LANES;
+        const unsigned token = item / p.heads, head = item - token * p.heads;
+        const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
+        items[n] = item;
+        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, item < p.items ? 8 : 0);
+        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, item < p.items ? 8 : 0);
     }
-    const float amax = max_nan(lanes_max<LANES>(abs_max8(x)), kAmaxMin);
-    store8_e4m3(static_cast<uint8_t*>(p.out) + o, p.vec, left, x, kFp8Max / amax);
-    if (col == 0 && left) p.scale[item] = amax / kFp8Max;
+    F2 w[4];
+    load_weight8<T, VEC>(p.weight, p.weight_f32, col, 8, w);
+#pragma unroll
+    for (int n = 0; n < kGatedItems; ++n) {
+        const unsigned item = items[n];
+        const int left = item < p.items ? 8 : 0;
+        const int64_t o = static_cast<int64_t>(item) * kHeadDim + col;
+        F2 x[4], z[4], ss = splat2(0.0f);
+        unpack8(rx[n], x);
+        unpack8(rz[n], z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss = fma2(x[i], x[i], ss);
+        const F2 rstd = splat2(rsqrtf(lanes_sum<LANES>(sum2(ss)) * (1.0f / kHeadDim) + p.eps));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(mul2(x[i], rstd), w[i]), mul2(z[i], sigmoid2(z[i])));
+        if (!p.quant) {
+            store8<T, VEC>(static_cast<T*>(p.out) + o, left, x);
+        } else {
+            const float amax = lanes_max<LANES>(abs_max8(x, kAmaxMin));
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + o, left, x, kFp8Max / amax);
+            if (col == 0 && left) p.scale[item] = amax / kFp8Max;
+        }
+    }
 }
 
 // Every thread keeps the same 8 columns for all its items: dweight stays in
-// registers, and the CTA's groups are added in order at the end.
-template <typename T, int LANES>
+// registers, and the CTA's groups are added in order at the end.  The next
+// item is on its way while one is worked on.
+template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const GatedNormParams p,
                                                                        const GatedNormGradParams d) {
     constexpr int kHeadDim = LANES * 8, kGroups = 256 / LANES;
     __shared__ float red[kGroups][kHeadDim];
     const int group = threadIdx.x / LANES, col = (threadIdx.x % LANES) * 8;
-    float w[8], dw[8] = {};
-    load_weight8<T>(p.weight, p.weight_f32, col, p.vec, 8, w);
-    for (unsigned first = blockIdx.x * kGroups; first < p.items; first += gridDim.x * kGroups) {
-        const unsigned item = first + group;
-        const int left = item < p.items ? 8 : 0;
+    F2 w[4], dw[4];
+    load_weight8<T, VEC>(p.weight, p.weight_f32, col, 8, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dw[i] = splat2(0.0f);
+    Raw8<T> rx, rz, ry;
+    auto fetch = [&](int64_t first) {
+        const int left = first + group < p.items ? 8 : 0;
+        const unsigned item = left ? static_cast<unsigned>(first + group) : 0;
         const unsigned token = item / p.heads, head = item - token * p.heads;
-        const int64_t in = static_cast<int64_t>(head) * kHeadDim + col, o = static_cast<int64_t>(item) * kHeadDim + col;
-        float x[8], z[8], dy[8];
-        load8(static_cast<const T*>(p.x) + token * p.x_stride + in, p.vec, left, x);
-        load8(static_cast<const T*>(p.z) + token * p.z_stride + in, p.vec, left, z);
-        load8(static_cast<const T*>(d.dy) + token * d.dy_stride + in, p.vec, left, dy);
-        float ss = 0.0f, dot = 0.0f;
+        const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
+        rx = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, left);
+        rz = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, left);
+        ry = load8<T, VEC>(static_cast<const T*>(d.dy) + token * d.dy_stride + in, left);
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+    int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups;
+    fetch(first);
+    for (; first < p.items; first += step) {
+        const int64_t item = first + group;
+        F2 x[4], z[4], dy[4], sig[4], ss2 = splat2(0.0f), dot2 = splat2(0.0f);
+        unpack8(rx, x);
+        unpack8(rz, z);
+        unpack8(ry, dy);
+        fetch(first + step);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            ss = fmaf(x[i], x[i], ss);
-            const float sig = sigmoid_f(z[i]);
-            dot = fmaf(dy[i] * w[i] * (z[i] * sig), x[i], dot);
+        for (int i = 0; i < 4; ++i) {
+            sig[i] = sigmoid2(z[i]);
+            ss2 = fma2(x[i], x[i], ss2);
+            dot2 = fma2(mul2(mul2(dy[i], w[i]), mul2(z[i], sig[i])), x[i], dot2);
         }
-        ss = lanes_sum<LANES>(ss);
-        dot = lanes_sum<LANES>(dot);
+        const float ss = lanes_sum<LANES>(sum2(ss2)), dot = lanes_sum<LANES>(sum2(dot2));
         const float rstd = rsqrtf(ss * (1.0f / kHeadDim) + p.eps);
-        const float back = dot * rstd * rstd * rstd * (1.0f / kHeadDim);
+        const F2 rstd2 = splat2(rstd), back = splat2(-dot * rstd * rstd * rstd * (1.0f / kHeadDim));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float sig = sigmoid_f(z[i]), gate = z[i] * sig, n = x[i] * rstd, dyn = dy[i] * n;
-            if (left) dw[i] = fmaf(dyn, gate, dw[i]);
-            x[i] = fmaf(dy[i] * w[i] * gate, rstd, -x[i] * back);
-            z[i] = dyn * w[i] * (sig + gate * (1.0f - sig));
+        for (int i = 0; i < 4; ++i) {
+            const F2 gate = mul2(z[i], sig[i]), dyn = mul2(dy[i], mul2(x[i], rstd2));
+            if (item < p.items) dw[i] = fma2(dyn, gate, dw[i]);
+            x[i] = fma2(mul2(mul2(dy[i], w[i]), gate), rstd2, mul2(x[i], back));
+            z[i] = mul2(mul2(dyn, w[i]), fma2(gate, fma2(sig[i], splat2(-1.0f), splat2(1.0f)), sig[i]));
         }
-        store8(static_cast<T*>(d.dx) + o, p.vec, left, x);
-        store8(static_cast<T*>(d.dz) + o, p.vec, left, z);
+        const int left = item < p.items ? 8 : 0;
+        store8<T, VEC>(static_cast<T*>(d.dx) + item * kHeadDim + col, left, x);
+        store8<T, VEC>(static_cast<T*>(d.dz) + item * kHeadDim + col, left, z);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[group][col + i] = dw[i];
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(dw[i]);
+        red[group][col + 2 * i] = v.x;
+        red[group][col + 2 * i + 1] = v.y;
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < kHeadDim; c += 256) {
         float s = 0.0f;
@@ -419,24 +461,40 @@ static RowShape row_shape(int width) {
 }
 constexpr int kNormMaxWidth = 1024 * 8 * 4;
 
+// Calls f with the vectors per thread and whether rows are whole vectors, as constants.
+template <int V>
+using Int = std::integral_constant<int, V>;
+template <typename F>
+static void with_row_shape(int vpt, bool vec, F f) {
+    const auto go = [&](auto n) { vec ? f(n, std::true_type{}) : f(n, std::false_type{}); };
+    vpt == 1 ? go(Int<1>{}) : vpt == 2 ? go(Int<2>{}) : go(Int<4>{});
+}
+template <typename F>
+static void with_head_shape(int head_dim, bool vec, F f) {
+    const auto go = [&](auto n) { vec ? f(n, std::true_type{}) : f(n, std::false_type{}); };
+    head_dim == 64 ? go(Int<8>{}) : head_dim == 128 ? go(Int<16>{}) : go(Int<32>{});
+}
+
 template <typename T>
 static cudaError_t launch_add_norm(const NormParams& p, cudaStream_t s) {
     const RowShape r = row_shape(p.width);
     const int per_cta = r.threads >= 256 ? 1 : 256 / r.threads;
     const dim3 block(r.threads, per_cta);
     const unsigned grid = static_cast<unsigned>((p.rows + per_cta - 1) / per_cta);
-    if (r.vpt == 1)
-        gdn_add_norm_kernel<T, 1><<<grid, block, 0, s>>>(p);
-    else if (r.vpt == 2)
-        gdn_add_norm_kernel<T, 2><<<grid, block, 0, s>>>(p);
-    else
-        gdn_add_norm_kernel<T, 4><<<grid, block, 0, s>>>(p);
+    with_row_shape(r.vpt, p.vec, [&](auto vpt, auto vec) { gdn_add_norm_kernel<T, vpt(), vec()><<<grid, block, 0, s>>>(p); });
     return cudaGetLastError();
 }
 
+// The backward pass holds the weight and its gradient's share too: fewer
+// vectors per thread, more threads.
+static RowShape row_shape_backward(int width) {
+    const int vecs = (width + 7) / 8, vpt = vecs <= 512 ? 1 : vecs <= 1024 ? 2 : 4;
+    return {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt};
+}
+
 static int norm_backward_ctas(int64_t rows, int width) {
-    const RowShape r = row_shape(width);
-    const int per_sm = 1024 / r.threads < 1 ? 1 : 1024 / r.threads > 8 ? 8 : 1024 / r.threads;
+    const RowShape r = row_shape_backward(width);
+    const int per_sm = r.vpt > 1 ? 1 : 1024 / r.threads > 8 ? 8 : 1024 / r.threads;
     const int64_t most = static_cast<int64_t>(kSmCount) * per_sm;
     return static_cast<int>(rows < most ? (rows > 0 ? rows : 1) : most);
 }
@@ -448,32 +506,26 @@ static cudaError_t launch_sum_columns(const float* part, int rows, int width, fl
 
 template <typename T>
 static cudaError_t launch_add_norm_backward(const NormParams& p, const NormGradParams& d, float* dweight, cudaStream_t s) {
-    const RowShape r = row_shape(p.width);
+    const RowShape r = row_shape_backward(p.width);
     const int grid = norm_backward_ctas(p.rows, p.width);
-    if (r.vpt == 1)
-        gdn_add_norm_backward_kernel<T, 1><<<grid, r.threads, 0, s>>>(p, d);
-    else if (r.vpt == 2)
-        gdn_add_norm_backward_kernel<T, 2><<<grid, r.threads, 0, s>>>(p, d);
-    else
-        gdn_add_norm_backward_kernel<T, 4><<<grid, r.threads, 0, s>>>(p, d);
+    with_row_shape(r.vpt, p.vec, [&](auto vpt, auto vec) {
+        gdn_add_norm_backward_kernel<T, vpt(), vec()><<<grid, r.threads, 0, s>>>(p, d);
+    });
     if (cudaError_t e = cudaGetLastError()) return e;
     return launch_sum_columns(d.part, grid, p.width, dweight, s);
 }
 
 template <typename T>
 static cudaError_t launch_gated_norm(const GatedNormParams& p, int head_dim, cudaStream_t s) {
-    const unsigned per_cta = 256 / (head_dim / 8), grid = (p.items + per_cta - 1) / per_cta;
-    if (head_dim == 64)
-        gdn_gated_norm_kernel<T, 8><<<grid, 256, 0, s>>>(p);
-    else if (head_dim == 128)
-        gdn_gated_norm_kernel<T, 16><<<grid, 256, 0, s>>>(p);
-    else
-        gdn_gated_norm_kernel<T, 32><<<grid, 256, 0, s>>>(p);
+    const unsigned per_cta = kGatedItems * 256 / (head_dim / 8), grid = (p.items + per_cta - 1) / per_cta;
+    with_head_shape(head_dim, p.vec, [&](auto lanes, auto vec) {
+        gdn_gated_norm_kernel<T, lanes(), vec()><<<grid, 256, 0, s>>>(p);
+    });
     return cudaGetLastError();
 }
 
 static int gated_norm_backward_ctas(int64_t items, int head_dim) {
-    const int64_t per_cta = 256 / (head_dim / 8), want = (items + per_cta - 1) / per_cta, most = kSmCount * 4;
+    const int64_t per_cta = 256 / (head_dim / 8), want = (items + per_cta - 1) / per_cta, most = kSmCount * 8;
     return static_cast<int>(want < most ? (want > 0 ? want : 1) : most);
 }
 
@@ -481,12 +533,9 @@ template <typename T>
 static cudaError_t launch_gated_norm_backward(const GatedNormParams& p, const GatedNormGradParams& d, int head_dim,
                                               float* dweight, cudaStream_t s) {
     const int grid = gated_norm_backward_ctas(p.items, head_dim);
-    if (head_dim == 64)
-        gdn_gated_norm_backward_kernel<T, 8><<<grid, 256, 0, s>>>(p, d);
-    else if (head_dim == 128)
-        gdn_gated_norm_backward_kernel<T, 16><<<grid, 256, 0, s>>>(p, d);
-    else
-        gdn_gated_norm_backward_kernel<T, 32><<<grid, 256, 0, s>>>(p, d);
+    with_head_shape(head_dim, p.vec, [&](auto lanes, auto vec) {
+        gdn_gated_norm_backward_kernel<T, lanes(), vec()><<<grid, 256, 0, s>>>(p, d);
+    });
     if (cudaError_t e = cudaGetLastError()) return e;
     return launch_sum_columns(d.part, grid, head_dim, dweight, s);
 }
