@@ -22,6 +22,8 @@ namespace gdn {
 constexpr float kFp8Max = 448.0f;
 constexpr float kAmaxMin = 1e-12f;  // an all-zero row keeps a finite scale
 constexpr int kQuantGroup = 128;    // channels per scale in group mode: 16 threads of 8
+constexpr int kNormStages = 3;
+constexpr int kNormThreads = 512, kNormWarps = 32;  // up to 1024 threads in the backward kernel's narrow form
 
 struct NormParams {
     const void* x;
@@ -37,6 +39,7 @@ struct NormParams {
     void* out;
     void* new_residual;
     float* scale;
+    int stages;  // backward: rows in flight in shared memory
 };
 
 struct NormGradParams {
@@ -75,21 +78,35 @@ template <typename T>
 struct Raw8 {
     uint4 v[sizeof(T) / 2];
 };
-// VEC: the row is whole vectors on 16-byte boundaries, so `left` (the elements
-// from p to the row's end) is a multiple of 8.
+// Which 8 elements of a row are a thread's j-th: neighbours where the row is
+// whole vectors on 16-byte boundaries (VEC), elsewhere `step` apart, so that a
+// warp's accesses touch neighbouring elements all the same.
+struct Cols {
+    int first, step, width;
+    __device__ __forceinline__ bool in(int i) const { return first + i * step < width; }
+};
+template <bool VEC>
+__device__ __forceinline__ Cols row_cols(int j, int width, bool groups) {
+    const int t = threadIdx.x, n = blockDim.x;
+    return VEC || groups ? Cols{(t + j * n) * 8, 1, width} : Cols{j * 8 * n + t, n, width};
+}
+
 template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T* p, int left) {
+__device__ __forceinline__ Raw8<T> load8(const T* row, Cols c) {
     Raw8<T> r = {};
     if constexpr (VEC) {
-        if (left > 0) {
+        if (c.in(0)) {
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(row + c.first)[i];
         }
     } else {
-        T* e = reinterpret_cast<T*>(&r);
+        // all loads first, from the row's start where the column is outside
+        T e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) e[i] = p[i];
+        for (int i = 0; i < 8; ++i) e[i] = row[c.in(i) ? c.first + i * c.step : 0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = c.in(i) ? e[i] : from_f32<T>(0.0f);
+        memcpy(&r, e, sizeof(r));
     }
     return r;
 }
@@ -100,7 +117,7 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& r, F2 (&f)[4]) {
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int left, const F2 (&f)[4]) {
+__device__ __forceinline__ void store8(T* row, Cols c, const F2 (&f)[4]) {
     Raw8<T> r;
     T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
@@ -110,40 +127,40 @@ __device__ __forceinline__ void store8(T* p, int left, const F2 (&f)[4]) {
         e[2 * i + 1] = from_f32<T>(v.y);
     }
     if constexpr (VEC) {
-        if (left > 0) {
+        if (c.in(0)) {
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + c.first)[i] = r.v[i];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = e[i];
+            if (c.in(i)) row[c.first + i * c.step] = e[i];
     }
 }
 
 template <bool VEC>
-__device__ __forceinline__ void store8_e4m3(uint8_t* p, int left, const F2 (&f)[4], float inv) {
+__device__ __forceinline__ void store8_e4m3(uint8_t* row, Cols c, const F2 (&f)[4], float inv) {
     uint2 u;
     uint16_t* h = reinterpret_cast<uint16_t*>(&u);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         h[i] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[i], splat2(inv))), __NV_SATFINITE, __NV_E4M3);
     if constexpr (VEC) {
-        if (left > 0) *reinterpret_cast<uint2*>(p) = u;
+        if (c.in(0)) *reinterpret_cast<uint2*>(row + c.first) = u;
     } else {
         const uint8_t* e = reinterpret_cast<const uint8_t*>(&u);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = e[i];
+            if (c.in(i)) row[c.first + i * c.step] = e[i];
     }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight8(const void* w, bool f32, int col, int left, F2 (&f)[4]) {
+__device__ __forceinline__ void load_weight8(const void* w, bool f32, Cols c, F2 (&f)[4]) {
     if (f32)
-        unpack8(load8<float, VEC>(static_cast<const float*>(w) + col, left), f);
+        unpack8(load8<float, VEC>(static_cast<const float*>(w), c), f);
     else
-        unpack8(load8<T, VEC>(static_cast<const T*>(w) + col, left), f);
+        unpack8(load8<T, VEC>(static_cast<const T*>(w), c), f);
 }
 
 // Maxima keep a NaN (fmaxf drops it): a row that holds one gets a NaN scale.
@@ -184,38 +201,47 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
     v = r[0];
+#pragma unroll 4
     for (int w = 1; w < warps; ++w) v = MAX ? max_keep_nan(v, r[w]) : v + r[w];
     return v;
 }
+// Sums of a and b over a warp, in five shuffles: the halves take one sum each.
+// Lanes 0 and 16 hold them.
+__device__ __forceinline__ float lanes_sum_pair(float a, float b) {
+    const bool upper = threadIdx.x & 16;
+    float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
-// blockDim = (threads per row, rows per CTA); thread i holds the row's
-// vectors i, i + blockDim.x, ...
+// blockDim = (threads per row, rows per CTA), 8 VPT elements of a row per thread.
 template <typename T, int VPT, bool VEC>
-__global__ void __launch_bounds__(1024) gdn_add_norm_kernel(const NormParams p) {
-    __shared__ float red_sum[32], red_max[32];
+__global__ void __launch_bounds__(kNormThreads) gdn_add_norm_kernel(const NormParams p) {
+    __shared__ float red_sum[kNormWarps], red_max[kNormWarps];
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const int width = row < p.rows ? p.width : 0;
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    const T* res = static_cast<const T*>(p.residual) + (p.residual ? row * p.residual_stride : 0);
+    const bool live = row < p.rows;
+    const int width = live ? p.width : 0;
+    const T* x = static_cast<const T*>(p.x) + (live ? row * p.x_stride : 0);
+    const T* res = static_cast<const T*>(p.residual) + (live && p.residual ? row * p.residual_stride : 0);
     const int64_t out = row * p.width;
+    const bool groups = p.quant == 2;
     Raw8<T> rx[VPT], rr[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8;
-        rx[j] = load8<T, VEC>(x + col, width - col);
-        rr[j] = load8<T, VEC>(res + col, p.residual ? width - col : 0);
+        rx[j] = load8<T, VEC>(x, row_cols<VEC>(j, width, groups));
+        if (p.residual) rr[j] = load8<T, VEC>(res, row_cols<VEC>(j, width, groups));
     }
     F2 r[VPT][4], ss = splat2(0.0f);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8;
-        F2 f[4];
         unpack8(rx[j], r[j]);
-        unpack8(rr[j], f);
         if (p.residual) {
+            F2 f[4];
+            unpack8(rr[j], f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[j][i] = add2(r[j][i], f[i]);
-            store8<T, VEC>(static_cast<T*>(p.new_residual) + out + col, width - col, r[j]);
+            store8<T, VEC>(static_cast<T*>(p.new_residual) + out, row_cols<VEC>(j, width, groups), r[j]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss = fma2(r[j][i], r[j][i], ss);
@@ -224,104 +250,127 @@ __global__ void __launch_bounds__(1024) gdn_add_norm_kernel(const NormParams p) 
     float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8, left = width - col;
+        const Cols c = row_cols<VEC>(j, width, groups);
         F2 w[4];
-        load_weight8<T, VEC>(p.weight, p.weight_f32, col, left, w);
+        load_weight8<T, VEC>(p.weight, p.weight_f32, c, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[j][i] = mul2(mul2(r[j][i], splat2(rstd)), w[i]);
         if (p.quant == 0) {
-            store8<T, VEC>(static_cast<T*>(p.out) + out + col, left, r[j]);
-        } else if (p.quant == 2) {  // 16 threads hold a group's 128 channels
-            const float amax = lanes_max<16>(left > 0 ? abs_max8(r[j], kAmaxMin) : kAmaxMin);
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out + col, left, r[j], kFp8Max / amax);
-            if (left > 0 && (threadIdx.x & 15) == 0)
-                p.scale[row * (p.width / kQuantGroup) + col / kQuantGroup] = amax / kFp8Max;
-        } else if (left > 0) {
+            store8<T, VEC>(static_cast<T*>(p.out) + out, c, r[j]);
+        } else if (groups) {  // 16 threads hold a group's 128 channels
+            const float amax = lanes_max<16>(c.in(0) ? abs_max8(r[j], kAmaxMin) : kAmaxMin);
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out, c, r[j], kFp8Max / amax);
+            if (c.in(0) && (threadIdx.x & 15) == 0)
+                p.scale[row * (p.width / kQuantGroup) + c.first / kQuantGroup] = amax / kFp8Max;
+        } else if (c.in(0)) {
             m = abs_max8(r[j], m);
         }
     }
     if (p.quant == 1) {
         const float amax = max_keep_nan(row_reduce<true>(m, red_max), kAmaxMin), inv = kFp8Max / amax;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (threadIdx.x + j * blockDim.x) * 8;
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out + col, width - col, r[j], inv);
-        }
+        for (int j = 0; j < VPT; ++j)
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out, row_cols<VEC>(j, width, false), r[j], inv);
         if (width > 0 && threadIdx.x == 0) p.scale[row] = amax / kFp8Max;
     }
 }
 
 // blockDim = (threads per row, 1); CTA k takes rows k, k + gridDim.x, ... and
-// keeps its share of dweight in registers.  The next row is on its way while
-// one is worked on (up to two vectors a thread).
+// keeps its share of dweight in registers.  With p.stages > 0 the rows of x, dy
+// and dr arrive in shared memory by bulk copies, p.stages rows ahead of use
+// (without them a row's loads would wait for the row before it).
 template <typename T, int VPT, bool VEC>
-__global__ void __launch_bounds__(VPT == 4 ? 1024 : 512, VPT == 1 ? 2 : 1) gdn_add_norm_backward_kernel(const NormParams p, const NormGradParams d) {
-    __shared__ float red[2][2][32];
+__global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_backward_kernel(const NormParams p, const NormGradParams d) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float red[2][2][kNormWarps];
+    __shared__ __align__(8) uint64_t s_bar[kNormStages];
     F2 dw[VPT][4], w[VPT][4];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8;
-        load_weight8<T, VEC>(p.weight, p.weight_f32, col, p.width - col, w[j]);
+        load_weight8<T, VEC>(p.weight, p.weight_f32, row_cols<VEC>(j, p.width, false), w[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dw[j][i] = splat2(0.0f);
     }
-    const float inv_width = 1.0f / static_cast<float>(p.width);
-    Raw8<T> rx[VPT], ry[VPT], rd[VPT];
-    auto fetch = [&](int64_t row) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (threadIdx.x + j * blockDim.x) * 8, left = row < p.rows ? p.width - col : 0;
-            rx[j] = load8<T, VEC>(static_cast<const T*>(p.x) + row * p.x_stride + col, left);
-            ry[j] = load8<T, VEC>(static_cast<const T*>(d.dy) + row * d.dy_stride + col, left);
-            rd[j] = load8<T, VEC>(static_cast<const T*>(d.dr) + (d.dr ? row * d.dr_stride + col : 0), d.dr ? left : 0);
-        }
+    const uint32_t row_bytes = p.width * sizeof(T), bar = tc05::smem_u32(s_bar);
+    auto fetch = [&](int64_t row, int stage) {  // by one thread
+        if (row >= p.rows) return;
+        const uint32_t to = tc05::smem_u32(smem) + stage * 3 * row_bytes;
+        tc05::mbar_expect_tx(bar + 8 * stage, row_bytes * (d.dr ? 3 : 2));
+        tc05::bulk_g2s(to, static_cast<const T*>(p.x) + row * p.x_stride, row_bytes, bar + 8 * stage);
+        tc05::bulk_g2s(to + row_bytes, static_cast<const T*>(d.dy) + row * d.dy_stride, row_bytes, bar + 8 * stage);
+        if (d.dr) tc05::bulk_g2s(to + 2 * row_bytes, static_cast<const T*>(d.dr) + row * d.dr_stride, row_bytes, bar + 8 * stage);
     };
-    constexpr bool kAhead = false;
-    if (kAhead) fetch(blockIdx.x);
-    int turn = 0;
+    if (p.stages > 0 && threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) tc05::mbar_init(bar + 8 * i, 1);
+        tc05::fence_mbar_init();
+        for (int i = 0; i < p.stages; ++i) fetch(blockIdx.x + static_cast<int64_t>(i) * gridDim.x, i);
+    }
+    if (p.stages > 0) __syncthreads();
+    const float inv_width = 1.0f / static_cast<float>(p.width);
+    int turn = 0, stage = 0, phase = 0;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        if (!kAhead) fetch(row);
+        const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+        const T* dy = static_cast<const T*>(d.dy) + row * d.dy_stride;
+        const T* dr = static_cast<const T*>(d.dr) + (d.dr ? row * d.dr_stride : 0);
+        if (VEC && p.stages > 0) {
+            if (!tc05::mbar_wait(bar + 8 * stage, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            x = reinterpret_cast<const T*>(smem + stage * 3 * row_bytes);
+            dy = x + p.width;
+            dr = dy + p.width;
+        }
         F2 r[VPT][4], g[VPT][4], o[VPT][4], ss2 = splat2(0.0f), dot2 = splat2(0.0f);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            unpack8(rx[j], r[j]);
-            unpack8(ry[j], g[j]);
-            unpack8(rd[j], o[j]);
+            const Cols c = row_cols<VEC>(j, p.width, false);
+            unpack8(load8<T, VEC>(x, c), r[j]);
+            unpack8(load8<T, VEC>(dy, c), g[j]);
+            if (d.dr) {
+                unpack8(load8<T, VEC>(dr, c), o[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[j][i] = splat2(0.0f);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 ss2 = fma2(r[j][i], r[j][i], ss2);
                 dot2 = fma2(mul2(g[j][i], w[j][i]), r[j][i], dot2);
             }
         }
-        if (kAhead) fetch(row + gridDim.x);
         // both sums in one exchange; the buffers alternate, so a fast warp's
         // next row cannot overwrite what a slow warp still reads
-        float ss = lanes_sum<32>(sum2(ss2)), dot = lanes_sum<32>(sum2(dot2));
+        const float both = lanes_sum_pair(sum2(ss2), sum2(dot2));
         const int warps = blockDim.x >> 5;
-        if (warps > 1) {
-            if ((threadIdx.x & 31) == 0) red[turn][0][threadIdx.x >> 5] = ss, red[turn][1][threadIdx.x >> 5] = dot;
-            __syncthreads();
-            ss = dot = 0.0f;
-            for (int k = 0; k < warps; ++k) ss += red[turn][0][k], dot += red[turn][1][k];
+        if ((threadIdx.x & 15) == 0) red[turn][threadIdx.x >> 4 & 1][threadIdx.x >> 5] = both;
+        __syncthreads();
+        if (VEC && p.stages > 0) {  // every thread has its part of the row: the stage takes another
+            if (threadIdx.x == 0) fetch(row + static_cast<int64_t>(p.stages) * gridDim.x, stage);
+            stage = stage + 1 == p.stages ? 0 : stage + 1;
+            phase ^= stage == 0;
+        }
+        float ss = 0.0f, dot = 0.0f;
+        for (int k = 0; k < warps; k += 16) {  // 16 warps' sums of each kind, added by the two halves of a warp
+            const int i = k + (threadIdx.x & 15);
+            float v = i < warps ? red[turn][threadIdx.x >> 4 & 1][i] : 0.0f;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            ss += __shfl_sync(0xffffffffu, v, 0);
+            dot += __shfl_sync(0xffffffffu, v, 16);
         }
         const float rstd = rsqrtf(ss * inv_width + p.eps);
         const F2 rstd2 = splat2(rstd), back = splat2(-dot * rstd * rstd * rstd * inv_width);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int col = (threadIdx.x + j * blockDim.x) * 8;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 dw[j][i] = fma2(g[j][i], mul2(r[j][i], rstd2), dw[j][i]);
                 o[j][i] = add2(o[j][i], fma2(mul2(g[j][i], w[j][i]), rstd2, mul2(r[j][i], back)));
             }
-            store8<T, VEC>(static_cast<T*>(d.dx) + row * p.width + col, p.width - col, o[j]);
+            store8<T, VEC>(static_cast<T*>(d.dx) + row * p.width, row_cols<VEC>(j, p.width, false), o[j]);
         }
     }
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int col = (threadIdx.x + j * blockDim.x) * 8;
-        store8<float, VEC>(d.part + static_cast<int64_t>(blockIdx.x) * p.width + col, p.width - col, dw[j]);
-    }
+    for (int j = 0; j < VPT; ++j)
+        store8<float, VEC>(d.part + static_cast<int64_t>(blockIdx.x) * p.width, row_cols<VEC>(j, p.width, false), dw[j]);
 }
 
 // out[c] = sum of part[.][c], in a fixed order.  blockDim = (32, 32).
@@ -329,8 +378,10 @@ __global__ void __launch_bounds__(1024) gdn_sum_columns_kernel(const float* part
     __shared__ float red[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x;
     float s = 0.0f;
-    if (c < width)
+    if (c < width) {
+#pragma unroll 8
         for (int i = threadIdx.y; i < rows; i += 32) s += part[static_cast<int64_t>(i) * width + c];
+    }
     red[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     s = lanes_sum<32>(red[threadIdx.x][threadIdx.y]);
@@ -352,15 +403,15 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
         const unsigned token = item / p.heads, head = item - token * p.heads;
         const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
         items[n] = item;
-        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, item < p.items ? 8 : 0);
-        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, item < p.items ? 8 : 0);
+        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, {0, 1, item < p.items ? 8 : 0});
+        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, {0, 1, item < p.items ? 8 : 0});
     }
     F2 w[4];
-    load_weight8<T, VEC>(p.weight, p.weight_f32, col, 8, w);
+    load_weight8<T, VEC>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
 #pragma unroll
     for (int n = 0; n < kGatedItems; ++n) {
         const unsigned item = items[n];
-        const int left = item < p.items ? 8 : 0;
+        const Cols all = {0, 1, item < p.items ? 8 : 0};
         const int64_t o = static_cast<int64_t>(item) * kHeadDim + col;
         F2 x[4], z[4], ss = splat2(0.0f);
         unpack8(rx[n], x);
@@ -371,11 +422,11 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(mul2(x[i], rstd), w[i]), mul2(z[i], sigmoid2(z[i])));
         if (!p.quant) {
-            store8<T, VEC>(static_cast<T*>(p.out) + o, left, x);
+            store8<T, VEC>(static_cast<T*>(p.out) + o, all, x);
         } else {
             const float amax = lanes_max<LANES>(abs_max8(x, kAmaxMin));
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + o, left, x, kFp8Max / amax);
-            if (col == 0 && left) p.scale[item] = amax / kFp8Max;
+            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + o, all, x, kFp8Max / amax);
+            if (col == 0 && item < p.items) p.scale[item] = amax / kFp8Max;
         }
     }
 }
@@ -390,18 +441,19 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const Gate
     __shared__ float red[kGroups][kHeadDim];
     const int group = threadIdx.x / LANES, col = (threadIdx.x % LANES) * 8;
     F2 w[4], dw[4];
-    load_weight8<T, VEC>(p.weight, p.weight_f32, col, 8, w);
+    load_weight8<T, VEC>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[i] = splat2(0.0f);
     Raw8<T> rx, rz, ry;
     auto fetch = [&](int64_t first) {
-        const int left = first + group < p.items ? 8 : 0;
-        const unsigned item = left ? static_cast<unsigned>(first + group) : 0;
+        const bool live = first + group < p.items;
+        const Cols all = {0, 1, live ? 8 : 0};
+        const unsigned item = live ? static_cast<unsigned>(first + group) : 0;
         const unsigned token = item / p.heads, head = item - token * p.heads;
         const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
-        rx = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, left);
-        rz = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, left);
-        ry = load8<T, VEC>(static_cast<const T*>(d.dy) + token * d.dy_stride + in, left);
+        rx = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, all);
+        rz = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, all);
+        ry = load8<T, VEC>(static_cast<const T*>(d.dy) + token * d.dy_stride + in, all);
     };
     const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
     int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups;
@@ -429,9 +481,9 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const Gate
             x[i] = fma2(mul2(mul2(dy[i], w[i]), gate), rstd2, mul2(x[i], back));
             z[i] = mul2(mul2(dyn, w[i]), fma2(gate, fma2(sig[i], splat2(-1.0f), splat2(1.0f)), sig[i]));
         }
-        const int left = item < p.items ? 8 : 0;
-        store8<T, VEC>(static_cast<T*>(d.dx) + item * kHeadDim + col, left, x);
-        store8<T, VEC>(static_cast<T*>(d.dz) + item * kHeadDim + col, left, z);
+        const Cols all = {0, 1, item < p.items ? 8 : 0};
+        store8<T, VEC>(static_cast<T*>(d.dx) + item * kHeadDim + col, all, x);
+        store8<T, VEC>(static_cast<T*>(d.dz) + item * kHeadDim + col, all, z);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -447,19 +499,24 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const Gate
     }
 }
 
-// Threads per row (a multiple of 32) and vectors per thread for a width.
+// Threads per row (a multiple of 32) and vectors of 8 elements per thread.
 struct RowShape {
     int threads, vpt;
 };
-static RowShape row_shape(int width) {
-    const int vecs = (width + 7) / 8;
-    int vpt = 1;
-    while ((vecs + vpt - 1) / vpt > (vpt == 4 ? 1024 : 256) && vpt < 4) vpt *= 2;
-    int threads = (vecs + vpt - 1) / vpt;
-    threads = (threads + 31) / 32 * 32;
-    return {threads, vpt};
+static RowShape row_shape(int vecs, int vpt) { return {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt}; }
+// Forward.  Two vectors per thread halve the warps that a row's sum waits for
+// (32768 x 2048 bf16: 82.7 us, 93.0 with one); four where a scale per row adds
+// a second wait (65536 x 1024: 74.7 us, 82.9 with two; fp32 would spill the
+// occupancy: 146 us for 16384 x 4096, 130 with two).  Rows off the 16-byte
+// boundary hold twice the registers per vector, so fewer (16384 x 5333: 320 us
+// with two, 483 with four).
+static RowShape row_shape_forward(const NormParams& p, size_t elem) {
+    const int vecs = (p.width + 7) / 8;
+    if (!p.vec) return row_shape(vecs, vecs <= 512 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8);
+    if (p.quant == 1 && elem == 2 && vecs >= 128 && vecs <= 2048) return row_shape(vecs, 4);
+    return row_shape(vecs, vecs <= 32 ? 1 : vecs <= 512 ? 2 : vecs <= 2048 ? 4 : 8);
 }
-constexpr int kNormMaxWidth = 1024 * 8 * 4;
+constexpr int kNormMaxWidth = kNormThreads * 8 * 8;
 
 // Calls f with the vectors per thread and whether rows are whole vectors, as constants.
 template <int V>
@@ -467,7 +524,7 @@ using Int = std::integral_constant<int, V>;
 template <typename F>
 static void with_row_shape(int vpt, bool vec, F f) {
     const auto go = [&](auto n) { vec ? f(n, std::true_type{}) : f(n, std::false_type{}); };
-    vpt == 1 ? go(Int<1>{}) : vpt == 2 ? go(Int<2>{}) : go(Int<4>{});
+    vpt == 1 ? go(Int<1>{}) : vpt == 2 ? go(Int<2>{}) : vpt == 4 ? go(Int<4>{}) : go(Int<8>{});
 }
 template <typename F>
 static void with_head_shape(int head_dim, bool vec, F f) {
@@ -477,7 +534,7 @@ static void with_head_shape(int head_dim, bool vec, F f) {
 
 template <typename T>
 static cudaError_t launch_add_norm(const NormParams& p, cudaStream_t s) {
-    const RowShape r = row_shape(p.width);
+    const RowShape r = row_shape_forward(p, sizeof(T));
     const int per_cta = r.threads >= 256 ? 1 : 256 / r.threads;
     const dim3 block(r.threads, per_cta);
     const unsigned grid = static_cast<unsigned>((p.rows + per_cta - 1) / per_cta);
@@ -485,17 +542,19 @@ static cudaError_t launch_add_norm(const NormParams& p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// The backward pass holds the weight and its gradient's share too: fewer
-// vectors per thread, more threads.
-static RowShape row_shape_backward(int width) {
-    const int vecs = (width + 7) / 8, vpt = vecs <= 512 ? 1 : vecs <= 1024 ? 2 : 4;
-    return {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt};
+// Backward: the weight and its gradient's share are held too, so two vectors at
+// most while they fit (65536 x 4096 bf16: 332 us, 407 with one on twice the
+// threads, whose sums wait for twice the warps).
+static RowShape row_shape_backward(int width, bool vec) {
+    const int vecs = (width + 7) / 8;
+    if (!vec) return row_shape(vecs, vecs <= 1024 ? 1 : vecs <= 2048 ? 4 : 8);
+    return row_shape(vecs, vecs <= 32 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8);
 }
 
-static int norm_backward_ctas(int64_t rows, int width) {
-    const RowShape r = row_shape_backward(width);
-    const int per_sm = r.vpt > 1 ? 1 : 1024 / r.threads > 8 ? 8 : 1024 / r.threads;
-    const int64_t most = static_cast<int64_t>(kSmCount) * per_sm;
+static int norm_backward_ctas(int64_t rows, int width, bool vec) {
+    const RowShape r = row_shape_backward(width, vec);
+    const int per_sm = (r.vpt == 1 ? 1024 : 512) / r.threads;  // by registers
+    const int64_t most = static_cast<int64_t>(kSmCount) * (per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm);
     return static_cast<int>(rows < most ? (rows > 0 ? rows : 1) : most);
 }
 
@@ -505,14 +564,25 @@ static cudaError_t launch_sum_columns(const float* part, int rows, int width, fl
 }
 
 template <typename T>
-static cudaError_t launch_add_norm_backward(const NormParams& p, const NormGradParams& d, float* dweight, cudaStream_t s) {
-    const RowShape r = row_shape_backward(p.width);
-    const int grid = norm_backward_ctas(p.rows, p.width);
+static cudaError_t launch_add_norm_backward(NormParams p, const NormGradParams& d, float* dweight, cudaStream_t s) {
+    const RowShape r = row_shape_backward(p.width, p.vec);
+    const int grid = norm_backward_ctas(p.rows, p.width, p.vec);
+    // Rows in flight for about 200 KB of an SM's shared memory over its CTAs;
+    // fewer than two would not run ahead, and rows off the 16-byte boundary
+    // cannot be copied in bulk (65536 x 4096: 407 us, 536 without).
+    const int per_sm = (grid + kSmCount - 1) / kSmCount;
+    const size_t stage = 3 * static_cast<size_t>(p.width) * sizeof(T);
+    const int fit = static_cast<int>((200 << 10) / per_sm / stage);
+    p.stages = !p.vec || fit < 2 ? 0 : fit < kNormStages ? fit : kNormStages;
+    const int smem = static_cast<int>(p.stages * stage);
+    cudaError_t e = cudaSuccess;
     with_row_shape(r.vpt, p.vec, [&](auto vpt, auto vec) {
-        gdn_add_norm_backward_kernel<T, vpt(), vec()><<<grid, r.threads, 0, s>>>(p, d);
+        const auto kernel = gdn_add_norm_backward_kernel<T, vpt(), vec()>;
+        if (smem > (40 << 10)) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) kernel<<<grid, r.threads, smem, s>>>(p, d);
     });
-    if (cudaError_t e = cudaGetLastError()) return e;
-    return launch_sum_columns(d.part, grid, p.width, dweight, s);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e != cudaSuccess ? e : launch_sum_columns(d.part, grid, p.width, dweight, s);
 }
 
 template <typename T>
@@ -577,6 +647,7 @@ static int add_norm_setup(const GdnAddNormArgs* a, NormParams& p) {
     p.out = a->output;
     p.new_residual = a->new_residual;
     p.scale = a->scale;
+    p.stages = 0;
     return GDN_OK;
 }
 
@@ -628,7 +699,8 @@ extern "C" int gdn_add_norm_launch(const GdnAddNormArgs* a, void* stream) {
 
 extern "C" size_t gdn_add_norm_backward_workspace_size(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1 || width > kNormMaxWidth) return 0;
-    return static_cast<size_t>(norm_backward_ctas(rows, static_cast<int>(width))) * width * sizeof(float);
+    const int a = norm_backward_ctas(rows, static_cast<int>(width), true), b = norm_backward_ctas(rows, static_cast<int>(width), false);
+    return static_cast<size_t>(a > b ? a : b) * width * sizeof(float);
 }
 
 extern "C" int gdn_add_norm_backward_launch(const GdnAddNormArgs* a, const GdnNormGradArgs* g, void* workspace,

@@ -254,18 +254,6 @@ __device__ __forceinline__ bool scan_bounds(const ScanParams& p, int64_t n, int6
     return true;
 }
 
-struct Gates {
-    float l, g, beta, z;
-};
-__device__ __forceinline__ Gates scan_gates(float rate, float dt_bias, float a, float b) {
-    Gates r;
-    r.z = a + dt_bias;
-    r.l = -rate * (fmaxf(r.z, 0.0f) + log1pf(expf(-fabsf(r.z))));
-    r.g = expf(r.l);
-    r.beta = 1.0f / (1.0f + expf(-b));
-    return r;
-}
-
 // A piece of the recurrence is an affine map of the state before it,
 // h -> A h + H, as (A0, A1, H0, H1) for a thread's two channels.  A piece in
 // which a sequence starts does not depend on the state before it: A = -0
@@ -477,6 +465,39 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     cluster_arrive();
     const int tokens = static_cast<int>(p.tokens);
     const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
+    const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
+    const F2 rate = pack2(ok0 ? -kLog2e * expf(p.A_log[c]) : 0.0f, ok1 ? -kLog2e * expf(p.A_log[c + 1]) : 0.0f);
+    const T* x0 = static_cast<const T*>(p.x) + c;
+    const T* a0 = static_cast<const T*>(p.a) + c;
+    const T* b0 = static_cast<const T*>(p.b) + c;
+    T* out0 = static_cast<T*>(p.out) + c;
+    const bool all_channels = c0 + kScanCh <= p.channels;
+    const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && all_channels;
+    constexpr int kBatch = 4;
+    RawPair<T> x[kPiece], a[kPiece], b[kPiece];
+    auto fetch = [&](int k, int from) {  // kBatch tokens of tile k
+        const int t0 = (k * R + rank) * kTile + warp * kPiece;
+        if (whole && k < steps && t0 + kPiece <= tokens) {
+#pragma unroll
+            for (int j = from; j < from + kBatch; ++j) {
+                x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
+                a[j] = load_raw(row_at<const T>(a0, t0 + j, p.a_stride));
+                b[j] = load_raw(row_at<const T>(b0, t0 + j, p.b_stride));
+            }
+        } else {
+#pragma unroll
+            for (int j = from; j < from + kBatch; ++j) {
+                const bool live = k < steps && t0 + j < tokens;
+                x[j] = load_raw_part(row_at<const T>(x0, t0 + j, p.x_stride), live && ok0, live && ok1);
+                a[j] = load_raw_part(row_at<const T>(a0, t0 + j, p.a_stride), live && ok0, live && ok1);
+                b[j] = load_raw_part(row_at<const T>(b0, t0 + j, p.b_stride), live && ok0, live && ok1);
+            }
+        }
+    };
+    if (warp < W) {
+#pragma unroll
+        for (int i = 0; i < kPiece; i += kBatch) fetch(0, i);
+    }
     scan_empty_sequences(p, p.state, p.new_state, c0, rank * blockDim.x + threadIdx.x, R * blockDim.x);
     cluster_wait();  // every CTA of the cluster runs and has its barriers
 
@@ -542,37 +563,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
         return;
     }
 
-    const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
-    const F2 rate = pack2(ok0 ? -kLog2e * expf(p.A_log[c]) : 0.0f, ok1 ? -kLog2e * expf(p.A_log[c + 1]) : 0.0f);
-    const T* x0 = static_cast<const T*>(p.x) + c;
-    const T* a0 = static_cast<const T*>(p.a) + c;
-    const T* b0 = static_cast<const T*>(p.b) + c;
-    T* out0 = static_cast<T*>(p.out) + c;
-    const bool all_channels = c0 + kScanCh <= p.channels;
-    const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && all_channels;
-    constexpr int kBatch = 4;
-    RawPair<T> x[kPiece], a[kPiece], b[kPiece];
-    auto fetch = [&](int k, int from) {  // kBatch tokens of tile k
-        const int t0 = (k * R + rank) * kTile + warp * kPiece;
-        if (whole && k < steps && t0 + kPiece <= tokens) {
-#pragma unroll
-            for (int j = from; j < from + kBatch; ++j) {
-                x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
-                a[j] = load_raw(row_at<const T>(a0, t0 + j, p.a_stride));
-                b[j] = load_raw(row_at<const T>(b0, t0 + j, p.b_stride));
-            }
-        } else {
-#pragma unroll
-            for (int j = from; j < from + kBatch; ++j) {
-                const bool live = k < steps && t0 + j < tokens;
-                x[j] = load_raw_part(row_at<const T>(x0, t0 + j, p.x_stride), live && ok0, live && ok1);
-                a[j] = load_raw_part(row_at<const T>(a0, t0 + j, p.a_stride), live && ok0, live && ok1);
-                b[j] = load_raw_part(row_at<const T>(b0, t0 + j, p.b_stride), live && ok0, live && ok1);
-            }
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < kPiece; i += kBatch) fetch(0, i);
     Spans span = {0, 0, 0, 0, 0};
     uint32_t ends = 0;  // of the tile before
     for (int k = 0; k <= steps; ++k) {
@@ -986,29 +976,82 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
     if (ok1) d.dA_log[c + 1] = s.y * kLn2, d.ddt_bias[c + 1] = s.w;
 }
 
-// One or a few tokens per sequence: element (sequence, channel) per thread.
-// The thread reads its state element before it writes it, so state may be
-// new_state.
-template <typename T>
-__global__ void __launch_bounds__(128) gdn_scan_step_kernel(const ScanParams p, int64_t steps) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
+// One or a few tokens per sequence, V channels of one sequence per thread (4
+// where every row starts on a boundary of four elements, else 1).  All of a
+// thread's reads of a token come before its writes, so state may be new_state.
+template <typename T, int V>
+__global__ void __launch_bounds__(128) gdn_scan_step_kernel(const ScanParams p, int steps) {
+    const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
     if (c >= p.channels) return;
-    const float rate = expf(p.A_log[c]), dtb = p.dt_bias[c];
-    for (int64_t n = blockIdx.y; n < p.seqs; n += gridDim.y) {
-        float h = p.state[n * p.channels + c];
-        for (int64_t t = n * steps; t < (n + 1) * steps; ++t) {
-            const Gates q = scan_gates(rate, dtb, to_f32(row_at<const T>(p.a, t, p.a_stride)[c]),
-                                       to_f32(row_at<const T>(p.b, t, p.b_stride)[c]));
-            h = q.g * h + q.beta * to_f32(row_at<const T>(p.x, t, p.x_stride)[c]);
-            row_at<T>(p.out, t, p.out_stride)[c] = from_f32<T>(h);
+    constexpr int P = V == 1 ? 1 : V / 2;  // pairs; a lone channel is its pair's first
+    using Row = std::conditional_t<V == 1, T, std::conditional_t<sizeof(T) == 4, uint4, uint2>>;
+    const auto pairs = [](const Row& r, F2 (&f)[P]) {
+        if constexpr (V == 1) {
+            f[0] = pack2(to_f32(r), 0.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) f[i] = load_pair<T>(reinterpret_cast<const T*>(&r) + 2 * i);
         }
-        p.new_state[n * p.channels + c] = h;
+    };
+    const auto floats = [](const float* q, F2 (&f)[P]) {
+        if constexpr (V == 1) {
+            f[0] = pack2(*q, 0.0f);
+        } else {
+            const float4 v = *reinterpret_cast<const float4*>(q);
+            f[0] = pack2(v.x, v.y);
+            f[1] = pack2(v.z, v.w);
+        }
+    };
+    F2 rate[P], dtb[P];
+    floats(p.A_log + c, rate);
+    floats(p.dt_bias + c, dtb);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const float2 v = unpack2(rate[i]);
+        rate[i] = pack2(-kLog2e * expf(v.x), -kLog2e * expf(v.y));
     }
-}
-
-static size_t scan_backward_workspace_bytes(int64_t tokens, int64_t seqs, int64_t channels) {
-    (void)tokens;
-    return static_cast<size_t>(2 * (seqs > 0 ? seqs : 1) * channels) * sizeof(float);
+    for (int64_t n = blockIdx.y; n < p.seqs; n += gridDim.y) {
+        F2 h[P];
+        floats(p.state + n * p.channels + c, h);
+        for (int64_t t = n * steps; t < (n + 1) * steps; ++t) {
+            const Row rx = *reinterpret_cast<const Row*>(row_at<const T>(p.x, t, p.x_stride) + c);
+            const Row ra = *reinterpret_cast<const Row*>(row_at<const T>(p.a, t, p.a_stride) + c);
+            const Row rb = *reinterpret_cast<const Row*>(row_at<const T>(p.b, t, p.b_stride) + c);
+            F2 x[P], z[P], b[P];
+            pairs(rx, x);
+            pairs(ra, z);
+            pairs(rb, b);
+#pragma unroll
+            for (int i = 0; i < P; ++i) z[i] = add2(z[i], dtb[i]);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                F2 one[1] = {z[i]};
+                decays(one, rate[i]);
+                h[i] = fma2(one[0], h[i], mul2(sigmoid2(b[i]), x[i]));
+            }
+            T* out = row_at<T>(p.out, t, p.out_stride) + c;
+            if constexpr (V == 1) {
+                *out = from_f32<T>(unpack2(h[0]).x);
+            } else {
+                T e[V];
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float2 v = unpack2(h[i]);
+                    e[2 * i] = from_f32<T>(v.x);
+                    e[2 * i + 1] = from_f32<T>(v.y);
+                }
+                *reinterpret_cast<Row*>(out) = *reinterpret_cast<const Row*>(e);
+            }
+        }
+        float* ns = p.new_state + n * p.channels + c;
+        const float2 v = unpack2(h[0]);
+        if constexpr (V == 1) {
+            *ns = v.x;
+        } else {
+            const float2 w = unpack2(h[1]);
+            *reinterpret_cast<float4*>(ns) = make_float4(v.x, v.y, w.x, w.y);
+        }
+    }
 }
 
 // `kernel` with gridDim = (cluster, groups of kScanCh channels); `attr` outlives the launch.
@@ -1097,8 +1140,16 @@ static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParam
 
 template <typename T>
 static cudaError_t launch_scan_step(const ScanParams& p, int64_t steps, cudaStream_t s) {
-    const dim3 grid((p.channels + 127) / 128, static_cast<unsigned>(p.seqs < 65535 ? p.seqs : 65535));
-    gdn_scan_step_kernel<T><<<grid, 128, 0, s>>>(p, steps);
+    const auto rows = [](const void* q, uint32_t stride) { return aligned(q, 4 * sizeof(T)) && stride % (4 * sizeof(T)) == 0; };
+    const bool vec = p.channels % 4 == 0 && rows(p.x, p.x_stride) && rows(p.a, p.a_stride) && rows(p.b, p.b_stride) &&
+                     rows(p.out, p.out_stride) && aligned(p.state, 16) && aligned(p.new_state, 16) && aligned(p.A_log, 16) &&
+                     aligned(p.dt_bias, 16);
+    const int per_cta = vec ? 512 : 128;
+    const dim3 grid((p.channels + per_cta - 1) / per_cta, static_cast<unsigned>(p.seqs < 65535 ? p.seqs : 65535));
+    if (vec)
+        gdn_scan_step_kernel<T, 4><<<grid, 128, 0, s>>>(p, static_cast<int>(steps));
+    else
+        gdn_scan_step_kernel<T, 1><<<grid, 128, 0, s>>>(p, static_cast<int>(steps));
     return cudaGetLastError();
 }
 
