@@ -189,18 +189,28 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t a, uint32_t bar, uint32_t
                  : "memory");
 }
 // The scans' CTA: 15 map warps and a chain warp (four warps to a scheduler,
-// so 128 registers a thread), 64 channels wide.
-constexpr int kScanCh = 64, kScanWarps = 15, kScanThreads = 32 * (kScanWarps + 1);
+// so 128 registers a thread).  A lane owns two channels; a warp is one strip of
+// 64 channels, or two strips of 32 on different tokens.
+constexpr int kScanWarps = 15, kScanThreads = 32 * (kScanWarps + 1);
+template <int STRIPS>
+struct Strips {
+    static constexpr int kLanes = 32 / STRIPS, kChannels = 2 * kLanes;
+    int strip, lane;  // this thread's strip, and its place there
+    __device__ Strips() : strip((threadIdx.x & 31) / kLanes), lane((threadIdx.x & 31) % kLanes) {}
+    // Piece i of a tile (in token order) is strip i % STRIPS of warp i / STRIPS;
+    // its word in an array [warps][step / 32][32] at this thread's channels.
+    __device__ __forceinline__ int word(int i, int step) const { return i / STRIPS * step + i % STRIPS * kLanes + lane; }
+};
 // Tokens per map warp and tile: a thread's inputs of the next tile wait in
 // registers (forward) and what its gates gave in shared memory (backward).
 template <typename T>
 constexpr int kScanPiece = sizeof(T) == 4 ? 4 : 8;
-constexpr int kGradPiece = 4, kGradTile = kScanWarps * kGradPiece;
+constexpr int kGradPiece = 4, kGradRows = kScanWarps * kGradPiece;
 constexpr int kScanMaxCluster = 16;
 
 // The carry into every kScanCkpt-th packed token is kept for the backward
 // pass, which recomputes the states of a tile from it.
-constexpr int kScanCkpt = kGradTile;
+constexpr int kScanCkpt = kGradRows;
 
 struct ScanParams {
     const void* x;
@@ -278,14 +288,16 @@ __device__ __forceinline__ bool all_finite(F2 v) {
     const float2 f = unpack2(v);
     return fabsf(f.x) <= 3.402823466e38f && fabsf(f.y) <= 3.402823466e38f;
 }
-// The product of maps[0], maps[step], ... of n pieces, and to before[32 i] the
-// product of those ahead of piece i (out of line: the slow form).
+// The product of n pieces' maps, and to before[.] the product of those ahead
+// of each (out of line: the slow form).
+template <int STRIPS>
 __device__ __noinline__ Map2 chain_select(const float4* maps, int n, int step, float4* before) {
+    const Strips<STRIPS> me;
     Map2 r = {splat2(1.0f), splat2(0.0f)};
     for (int i = 0; i < n; ++i) {
-        const float4 m = maps[i * step];
+        const float4 m = maps[me.word(i, step)];
         const float2 a = unpack2(r.A), h = unpack2(r.H);
-        before[i * 32] = make_float4(a.x, a.y, h.x, h.y);
+        if (i % STRIPS == me.strip) before[me.word(i, 32)] = make_float4(a.x, a.y, h.x, h.y);
         r.H = apply_map_select(m, r.H);
         r.A = pack2(is_start(m.x) ? m.x : a.x * m.x, is_start(m.y) ? m.y : a.y * m.y);
     }
@@ -381,6 +393,29 @@ __device__ __noinline__ void store_state_of_token(const void* cu, bool is64, int
     if (c + 1 < channels) row[c + 1] = v.y;
 }
 
+// The same for a warp whose strips hold token t and those `apart` tokens on;
+// `which` has bit i set for the strips (bit i * apart) that want it.  The whole warp calls.
+template <int STRIPS>
+__device__ __forceinline__ F2 state_of_strips(const ScanParams& p, const float* state, uint32_t which, int apart, int64_t t,
+                                              int c, int strip, F2 other) {
+#pragma unroll
+    for (int i = 0; i < STRIPS; ++i)
+        if (which >> (i * apart) & 1) {
+            const F2 v = state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), state, p.channels, t + i * apart, c);
+            if (strip == i) other = v;
+        }
+    return other;
+}
+template <int STRIPS>
+__device__ __forceinline__ void store_state_of_strips(const ScanParams& p, float* state, uint32_t which, int apart, int64_t t,
+                                                      int c, int strip, F2 h) {
+#pragma unroll
+    for (int i = 0; i < STRIPS; ++i)
+        if (which >> (i * apart) & 1)
+            store_state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), state, p.channels, t + i * apart,
+                                 strip == i ? c : p.channels, h);
+}
+
 // Two neighbouring elements as they are stored, read past the L1 cache.
 template <typename T>
 struct RawPair {
@@ -412,9 +447,9 @@ template <typename T>
 __device__ __forceinline__ F2 raw_to_f2(RawPair<T> r) { return load_pair<T>(&r); }
 
 // Sequences without a token pass their state on; bad offsets are reported.
-__device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const float* from, float* to, int c0, int first,
-                                                     int step) {
-    const int c1 = min(p.channels, c0 + kScanCh);
+__device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const float* from, float* to, int c0, int c1,
+                                                     int first, int step) {
+    c1 = min(p.channels, c1);
     for (int64_t n = first; n < p.seqs; n += step) {
         int64_t t0, t1;
         scan_bounds(p, n, t0, t1);
@@ -424,9 +459,8 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 }
 
 // The packed scan in one pass over the data.  A cluster of R CTAs takes 64
-// channels and walks the packed tokens, whatever sequences they belong to, R
-// tiles at a time: ragged batches and one long sequence load the GPU alike.
-// A lane owns two channels.
+// (or 32) channels and walks the packed tokens, whatever sequences they belong
+// to, R tiles at a time: ragged batches and one long sequence load the GPU alike.
 //   map warp    g and u = beta x of its piece of the tile's tokens, chained
 //               into the maps from the piece's start, to shared memory (its
 //               own words: no other warp reads them but the piece's last);
@@ -439,18 +473,20 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 //               order (the same bits on every run).
 // So the gates' arithmetic, which is what the kernel is made of, has a whole
 // tile's time to hide the cluster's exchange behind.
-template <typename T>
+template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanParams p) {
-    constexpr int W = kScanWarps, kPiece = kScanPiece<T>, kTile = W * kPiece;
+    constexpr int W = kScanWarps, kPiece = kScanPiece<T>, kRows = W * kPiece, kTile = STRIPS * kRows;
+    constexpr int kSpan = STRIPS * kPiece;  // a warp's tokens
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ F2 s_in[2][32];  // the state at the tile's start
     __shared__ __align__(8) uint64_t s_bar[6];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int R = cluster_size(), rank = cluster_rank();
-    float4* maps = reinterpret_cast<float4*>(smem) + lane;  // [2][kTile][32]: of each token, from its piece's start
-    float4* befores = maps + 2 * kTile * 32;                // [2][W][32]: of each piece, from the tile's start
-    float4* ranks = befores + 2 * W * 32;                   // [2][R][32]: the cluster's tiles
-    const int c0 = blockIdx.y * kScanCh, c = c0 + 2 * lane;
+    const Strips<STRIPS> me;
+    float4* maps = reinterpret_cast<float4*>(smem);  // [2][kRows][32]: of each token, from its piece's start
+    float4* befores = maps + 2 * kRows * 32;         // [2][W][32]: of each piece, from the tile's start
+    float4* ranks = befores + 2 * W * 32;            // [2][R][32]: the cluster's tiles
+    const int c0 = blockIdx.y * me.kChannels, c = c0 + 2 * me.lane;
     const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
     const uint32_t full = tc05::smem_u32(s_bar), ready = full + 16, arrived = full + 32;
     if (threadIdx.x == 0) {
@@ -471,13 +507,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     const T* a0 = static_cast<const T*>(p.a) + c;
     const T* b0 = static_cast<const T*>(p.b) + c;
     T* out0 = static_cast<T*>(p.out) + c;
-    const bool all_channels = c0 + kScanCh <= p.channels;
+    const bool all_channels = c0 + me.kChannels <= p.channels;
     const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && all_channels;
     constexpr int kBatch = 4;
     RawPair<T> x[kPiece], a[kPiece], b[kPiece];
     auto fetch = [&](int k, int from) {  // kBatch tokens of tile k
-        const int t0 = (k * R + rank) * kTile + warp * kPiece;
-        if (whole && k < steps && t0 + kPiece <= tokens) {
+        const int w0 = (k * R + rank) * kTile + warp * kSpan, t0 = w0 + me.strip * kPiece;
+        if (whole && k < steps && w0 + kSpan <= tokens) {
 #pragma unroll
             for (int j = from; j < from + kBatch; ++j) {
                 x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
@@ -498,7 +534,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
 #pragma unroll
         for (int i = 0; i < kPiece; i += kBatch) fetch(0, i);
     }
-    scan_empty_sequences(p, p.state, p.new_state, c0, rank * blockDim.x + threadIdx.x, R * blockDim.x);
+    scan_empty_sequences(p, p.state, p.new_state, c0, c0 + me.kChannels, rank * blockDim.x + threadIdx.x, R * blockDim.x);
     cluster_wait();  // every CTA of the cluster runs and has its barriers
 
     if (warp == W) {
@@ -506,30 +542,30 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
         for (int k = 0; k < steps; ++k) {
             const int buf = k & 1, phase = k >> 1 & 1;
             if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-            const float4* last = maps + (buf * kTile + kPiece - 1) * 32;  // a piece's whole map is its last token's
+            const float4* last = maps + (buf * kRows + kPiece - 1) * 32;  // a piece's whole map is its last token's
             float4* before = befores + buf * W * 32;
             F2 A = splat2(1.0f), H = splat2(0.0f);
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float4 m = last[w * kPiece * 32];
+            for (int i = 0; i < STRIPS * W; ++i) {
+                const float4 m = last[me.word(i, kPiece * 32)];
                 const float2 va = unpack2(A), vh = unpack2(H);
-                before[w * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                if (i % STRIPS == me.strip) before[me.word(i, 32)] = make_float4(va.x, va.y, vh.x, vh.y);
                 H = apply_map(m, H);
                 A = mul2(A, pack2(m.x, m.y));
             }
             if (__any_sync(0xffffffffu, has_nan(A) || has_nan(H))) {
-                const Map2 all = chain_select(last, W, kPiece * 32, before);
+                const Map2 all = chain_select<STRIPS>(last, STRIPS * W, kPiece * 32, before);
                 A = all.A, H = all.H;
             }
             const float2 va = unpack2(A), vh = unpack2(H);
-            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32);
+            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32 + lane);
             // A slot is written again two tiles on: by then this CTA has every
             // CTA's map of tile k + 1, sent after that CTA had read tile k's.
             for (int r = 0; r < R; ++r)
                 st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
             if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
             if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
-            const float4* all = ranks + buf * R * 32;
+            const float4* all = ranks + buf * R * 32 + lane;
             F2 in = carry;
 #pragma unroll 4
             for (int r = 0; r < rank; ++r) in = apply_map(all[r * 32], in);
@@ -544,19 +580,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
             __syncwarp();
             if (lane == 0) tc05::mbar_arrive(ready + 8 * buf);
             carry = next;
+            __syncwarp();  // the chain's words from both strips
             if (p.ckpt) {
 #pragma unroll
                 for (int i = 0; i < kTile; i += kScanCkpt) {
                     const int t = (k * R + rank) * kTile + i;
                     F2 at = in;
                     if (i) {  // the token before it: its piece's start, and on from there
-                        at = apply_map_select(before[(i - 1) / kPiece * 32], at);
-                        at = apply_map_select(maps[(buf * kTile + i - 1) * 32], at);
+                        const int piece = (i - 1) / kPiece, row = buf * kRows + (i - 1) % kPiece;
+                        at = apply_map_select(before[me.word(piece, 32)], at);
+                        at = apply_map_select(maps[row * 32 + me.word(piece, kPiece * 32)], at);
                     }
                     const float2 v = unpack2(at);
                     float* ck = p.ckpt + static_cast<int64_t>(t / kScanCkpt) * p.channels;
-                    if (t < tokens && ok0) ck[c] = v.x;
-                    if (t < tokens && ok1) ck[c + 1] = v.y;
+                    if (t < tokens && me.strip == 0 && ok0) ck[c] = v.x;
+                    if (t < tokens && me.strip == 0 && ok1) ck[c + 1] = v.y;
                 }
             }
         }
@@ -567,10 +605,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     uint32_t ends = 0;  // of the tile before
     for (int k = 0; k <= steps; ++k) {
         if (k < steps) {
-            const int t0 = (k * R + rank) * kTile + warp * kPiece, buf = k & 1;
-            token_spans<kPiece>(p, t0, span);
-            const uint32_t special = span.start | (~span.covered & kAllTokens<kPiece>);
-            float4* m = maps + (buf * kTile + warp * kPiece) * 32;
+            const int w0 = (k * R + rank) * kTile + warp * kSpan, buf = k & 1;
+            token_spans<kSpan>(p, w0, span);
+            const uint32_t special = span.start | (~span.covered & kAllTokens<kSpan>);
+            const uint32_t mine = special >> me.strip * kPiece, covered = span.covered >> me.strip * kPiece;
+            float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
             F2 A = splat2(1.0f), H = splat2(0.0f);  // the map up to each token
 #pragma unroll
             for (int i = 0; i < kPiece; i += kBatch) {
@@ -596,15 +635,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                 } else {
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
-                        F2 before = H;
-                        if (special >> (i + j) & 1) {
-                            A = splat2(-0.0f);
-                            before = state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.state, p.channels,
-                                                    t0 + i + j, c);
-                        } else {
-                            A = mul2(A, z[j]);
-                        }
-                        H = span.covered >> (i + j) & 1 ? fma2(z[j], before, u[j]) : splat2(0.0f);
+                        const F2 before = state_of_strips<STRIPS>(p, p.state, span.start >> (i + j), kPiece, w0 + i + j, c,
+                                                                  me.strip, H);
+                        A = mine >> (i + j) & 1 ? splat2(-0.0f) : mul2(A, z[j]);
+                        H = covered >> (i + j) & 1 ? fma2(z[j], before, u[j]) : splat2(0.0f);
                         put(j);
                     }
                 }
@@ -613,10 +647,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
             if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
         }
         if (k > 0) {
-            const int buf = (k - 1) & 1, t0 = ((k - 1) * R + rank) * kTile + warp * kPiece;
+            const int buf = (k - 1) & 1, w0 = ((k - 1) * R + rank) * kTile + warp * kSpan, t0 = w0 + me.strip * kPiece;
             if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-            const float4* m = maps + (buf * kTile + warp * kPiece) * 32;
-            const float4 before = befores[(buf * W + warp) * 32];
+            const float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
+            const float4 before = befores[(buf * W + warp) * 32 + lane];
             const F2 tile_in = s_in[buf][lane];
             F2 in = apply_map(before, tile_in), h[kPiece];
             const bool finite = !__any_sync(0xffffffffu, !all_finite(tile_in) || !all_finite(in));
@@ -629,16 +663,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                 for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
             }
             T* out = row_at<T>(out0, t0, p.out_stride);
-            if (ends == 0 && t0 + kPiece <= tokens && p.out_pairs && all_channels) {
+            if (ends == 0 && w0 + kSpan <= tokens && p.out_pairs && all_channels) {
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) store_pair(row_at<T>(out, j, p.out_stride), h[j], true, true, true);
             } else {
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) {
                     if (t0 + j < tokens) store_pair(row_at<T>(out, j, p.out_stride), h[j], p.out_pairs, ok0, ok1);
-                    if (ends >> j & 1)
-                        store_state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.new_state, p.channels, t0 + j, c,
-                                             h[j]);
+                    store_state_of_strips<STRIPS>(p, p.new_state, ends >> j, kPiece, w0 + j, c, me.strip, h[j]);
                 }
             }
         }
@@ -651,7 +683,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
 // reads only what it wrote.
 template <typename T>
 struct GradTile {  // 16-bit inputs: 32 bytes
-    static constexpr size_t kBytes = 2 * kGradTile * 32 * 32;
+    static constexpr size_t kBytes = 2 * kGradRows * 32 * 32;
     float4* base;
     __device__ GradTile(unsigned char* smem, int lane) : base(reinterpret_cast<float4*>(smem) + lane) {}
     __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<T> x, RawPair<T> dy) {
@@ -670,12 +702,12 @@ struct GradTile {  // 16-bit inputs: 32 bytes
 };
 template <>
 struct GradTile<float> {  // 40 bytes
-    static constexpr size_t kBytes = 2 * kGradTile * 32 * 40;
+    static constexpr size_t kBytes = 2 * kGradRows * 32 * 40;
     float4* base;
     float2* sigs;
     __device__ GradTile(unsigned char* smem, int lane)
         : base(reinterpret_cast<float4*>(smem) + lane),
-          sigs(reinterpret_cast<float2*>(smem + 2 * kGradTile * 32 * 32) + lane) {}
+          sigs(reinterpret_cast<float2*>(smem + 2 * kGradRows * 32 * 32) + lane) {}
     __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<float> x, RawPair<float> dy) {
         const float2 a = unpack2(t), b = unpack2(beta);
         base[2 * i * 32] = make_float4(a.x, a.y, b.x, b.y);
@@ -703,20 +735,21 @@ struct GradTile<float> {  // 40 bytes
 // writes its piece's gradients a tile later, when both ends are known.  The
 // sums over tokens stay in registers to the end, and are added over the CTA's
 // warps and the cluster's CTAs in order.
-template <typename T>
+template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
-    constexpr int W = kScanWarps, kPiece = kGradPiece, kTile = kGradTile;
+    constexpr int W = kScanWarps, kPiece = kGradPiece, kRows = kGradRows, kTile = STRIPS * kRows, kSpan = STRIPS * kPiece;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float4 s_ends[2][32];  // the state before the tile, the gradient behind it
     __shared__ __align__(8) uint64_t s_bar[7];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int R = cluster_size(), rank = cluster_rank();
     GradTile<T> vals(smem, lane);
-    float4* state_maps = reinterpret_cast<float4*>(smem + GradTile<T>::kBytes) + lane;  // [2][W][32], and then what precedes
-    float4* grad_maps = state_maps + 2 * W * 32;                                        // [2][W][32], and then what follows
-    float4* ranks = grad_maps + 2 * W * 32;                                             // [2][R][32]
+    const Strips<STRIPS> me;
+    float4* state_maps = reinterpret_cast<float4*>(smem + GradTile<T>::kBytes);  // [2][W][32], and then what precedes
+    float4* grad_maps = state_maps + 2 * W * 32;                                 // [2][W][32], and then what follows
+    float4* ranks = grad_maps + 2 * W * 32;                                      // [2][R][32]
     float4* cta_sums = ranks + 2 * R * 32;  // [R][32], the first CTA's: others write while it still works
-    const int c0 = blockIdx.y * kScanCh, c = c0 + 2 * lane;
+    const int c0 = blockIdx.y * me.kChannels, c = c0 + 2 * me.lane;
     const bool ok0 = c < p.channels, ok1 = c + 1 < p.channels;
     const uint32_t full = tc05::smem_u32(s_bar), ready = full + 16, arrived = full + 32, summed = full + 48;
     if (threadIdx.x == 0) {
@@ -731,9 +764,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
         tc05::fence_mbar_init();
     }
     cluster_arrive();
-    const int tokens = static_cast<int>(p.tokens), seqs = static_cast<int>(p.seqs);
+    const int tokens = static_cast<int>(p.tokens);
     const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
-    scan_empty_sequences(p, d.d_new_state, d.d_state, c0, rank * blockDim.x + threadIdx.x, R * blockDim.x);
+    scan_empty_sequences(p, d.d_new_state, d.d_state, c0, c0 + me.kChannels, rank * blockDim.x + threadIdx.x, R * blockDim.x);
     cluster_wait();  // every CTA of the cluster runs and has its barriers
     // first token of the CTA's tile of step k; before the first token when there is none left
     auto tile_start = [&](int k) { return (tiles - 1 - (k * R + rank)) * kTile; };
@@ -756,11 +789,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             auto chain = [&](float4* m, bool back) {  // in place: a piece's map makes way for what comes before it
                 Map2 all = {splat2(1.0f), splat2(0.0f)};
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const int w = back ? W - 1 - i : i;
-                    const float4 e = m[w * 32];
+                for (int i = 0; i < STRIPS * W; ++i) {
+                    const int n = back ? STRIPS * W - 1 - i : i, word = me.word(n, 32);
+                    const float4 e = m[word];
                     const float2 va = unpack2(all.A), vh = unpack2(all.H);
-                    m[w * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                    if (STRIPS > 1) __syncwarp();  // every strip has read the word
+                    if (n % STRIPS == me.strip) m[word] = make_float4(va.x, va.y, vh.x, vh.y);
                     const F2 A = pack2(e.x, e.y);
                     const float2 r = unpack2(fma2(A, all.H, pack2(e.z, e.w))), a = unpack2(mul2(all.A, A));
                     all.H = pack2(is_start(e.x) ? e.z : r.x, is_start(e.y) ? e.w : r.y);
@@ -770,7 +804,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             };
             const Map2 all_grad = chain(grad_maps + buf * W * 32, true);
             const float2 va = unpack2(all_grad.A), vh = unpack2(all_grad.H);
-            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32);
+            const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32 + lane);
             // A slot is written again two tiles on: by then this CTA has every
             // CTA's map of the tile between, sent after that CTA had read this one's.
             for (int r = 0; r < R; ++r)
@@ -778,7 +812,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             chain(state_maps + buf * W * 32, false);
             if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
             if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
-            const float4* every = ranks + buf * R * 32;
+            const float4* every = ranks + buf * R * 32 + lane;
             F2 in = carry;
 #pragma unroll 4
             for (int r = 0; r < rank; ++r) in = apply_map(every[r * 32], in);
@@ -799,16 +833,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
         const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
         const float2 decay = make_float2(ok0 ? expf(p.A_log[c]) : 0.0f, ok1 ? expf(p.A_log[c + 1]) : 0.0f);
         const F2 rate = pack2(-kLog2e * decay.x, -kLog2e * decay.y), minus_decay = pack2(-decay.x, -decay.y);
-        const bool all_channels = c0 + kScanCh <= p.channels;
+        const bool all_channels = c0 + me.kChannels <= p.channels;
         const bool whole = p.x_pairs && p.a_pairs && p.b_pairs && d.dy_pairs && all_channels;
         RawPair<T> x[kPiece], a[kPiece], b[kPiece], dy[kPiece];
         auto fetch = [&](int k) {
-            const int t0 = k < steps ? tile_start(k) + warp * kPiece : -kTile;
+            const int w0 = k < steps ? tile_start(k) + warp * kSpan : -kTile, t0 = w0 + me.strip * kPiece;
             const T* x0 = static_cast<const T*>(p.x) + c;
             const T* a0 = static_cast<const T*>(p.a) + c;
             const T* b0 = static_cast<const T*>(p.b) + c;
             const T* dy0 = static_cast<const T*>(d.dy) + c;
-            if (whole && t0 >= 0 && t0 + kPiece <= tokens) {
+            if (whole && w0 >= 0 && w0 + kSpan <= tokens) {
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) {
                     x[j] = load_raw(row_at<const T>(x0, t0 + j, p.x_stride));
@@ -819,7 +853,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             } else {
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) {
-                    const bool live = t0 >= 0 && t0 + j < tokens;
+                    const bool live = w0 >= 0 && t0 + j < tokens;
                     x[j] = load_raw_part(row_at<const T>(x0, t0 + j, p.x_stride), live && ok0, live && ok1);
                     a[j] = load_raw_part(row_at<const T>(a0, t0 + j, p.a_stride), live && ok0, live && ok1);
                     b[j] = load_raw_part(row_at<const T>(b0, t0 + j, p.b_stride), live && ok0, live && ok1);
@@ -831,12 +865,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
         Spans span = {0, 0, 0, 0, 0}, done = span;
         for (int k = 0; k <= steps; ++k) {
             if (k < steps) {
-                const int t0 = tile_start(k) + warp * kPiece, buf = k & 1;
-                if (t0 >= 0)
-                    token_spans<kPiece>(p, t0, span);
+                const int w0 = tile_start(k) + warp * kSpan, buf = k & 1;
+                if (w0 >= 0)
+                    token_spans<kSpan>(p, w0, span);
                 else
                     span = {0, 0, 0, 0, 0};
-                const bool special = (span.start | span.end | (~span.covered & kAllTokens<kPiece>)) != 0;
+                const bool special = (span.start | span.end | (~span.covered & kAllTokens<kSpan>)) != 0;
                 F2 z[kPiece], e[kPiece], u[kPiece], in[kPiece];
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) z[j] = add2(raw_to_f2<T>(a[j]), dtb);
@@ -851,7 +885,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                     const float2 q = make_float2(rcp_approx(1.0f + w.x), rcp_approx(1.0f + w.y));
                     sig[j] = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
                     const F2 beta = sigmoid2(raw_to_f2<T>(b[j]));
-                    vals.put(buf * kTile + warp * kPiece + j, z[j], beta, sig[j], x[j], dy[j]);
+                    vals.put(buf * kRows + warp * kPiece + j, z[j], beta, sig[j], x[j], dy[j]);
                     z[j] = exp2_2(z[j]);
                     u[j] = mul2(beta, raw_to_f2<T>(x[j]));
                     in[j] = raw_to_f2<T>(dy[j]);
@@ -868,33 +902,34 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) E = mul2(z[j], add2(in[j], E));
                 } else {
+                    const int at = me.strip * kPiece;
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        const bool covered = span.covered >> j & 1, start = span.start >> j & 1;
-                        if (start) H = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
+                        const bool covered = span.covered >> (at + j) & 1, start = span.start >> (at + j) & 1;
+                        H = state_of_strips<STRIPS>(p, p.state, span.start >> j, kPiece, w0 + j, c, me.strip, H);
                         A = start || !covered ? splat2(-0.0f) : mul2(A, z[j]);
                         H = covered ? fma2(z[j], H, u[j]) : splat2(0.0f);
                     }
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) {
-                        const bool covered = span.covered >> j & 1, end = span.end >> j & 1;
-                        if (end) E = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
+                        const bool covered = span.covered >> (at + j) & 1, end = span.end >> (at + j) & 1;
+                        E = state_of_strips<STRIPS>(p, d.d_new_state, span.end >> j, kPiece, w0 + j, c, me.strip, E);
                         B = end || !covered ? splat2(-0.0f) : mul2(B, z[j]);
                         E = covered ? mul2(z[j], add2(in[j], E)) : splat2(0.0f);
                     }
                 }
                 const float2 va = unpack2(A), vh = unpack2(H), vb = unpack2(B), ve = unpack2(E);
-                state_maps[(buf * W + warp) * 32] = make_float4(va.x, va.y, vh.x, vh.y);
-                grad_maps[(buf * W + warp) * 32] = make_float4(vb.x, vb.y, ve.x, ve.y);
+                state_maps[(buf * W + warp) * 32 + lane] = make_float4(va.x, va.y, vh.x, vh.y);
+                grad_maps[(buf * W + warp) * 32 + lane] = make_float4(vb.x, vb.y, ve.x, ve.y);
                 __syncwarp();
                 if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
             }
             if (k > 0 && tile_start(k - 1) >= 0) {
-                const int buf = (k - 1) & 1, t0 = tile_start(k - 1) + warp * kPiece;
+                const int buf = (k - 1) & 1, w0 = tile_start(k - 1) + warp * kSpan, t0 = w0 + me.strip * kPiece;
                 if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
                 const float4 ends = s_ends[buf][lane];
                 const F2 tile_h = pack2(ends.x, ends.y), tile_e = pack2(ends.z, ends.w);
-                const float4 hm = state_maps[(buf * W + warp) * 32], em = grad_maps[(buf * W + warp) * 32];
+                const float4 hm = state_maps[(buf * W + warp) * 32 + lane], em = grad_maps[(buf * W + warp) * 32 + lane];
                 F2 h = apply_map(hm, tile_h), e = apply_map(em, tile_e);
                 if (__any_sync(0xffffffffu, !all_finite(tile_h) || !all_finite(tile_e))) {
                     h = apply_map_select(hm, tile_h);
@@ -903,40 +938,40 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                 // whole pieces inside one sequence go without a branch
                 auto finish = [&](auto inside) {
                     constexpr bool kInside = decltype(inside)::value;
+                    const uint32_t covered = done.covered >> me.strip * kPiece;
                     F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        vals.get(buf * kTile + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
+                        vals.get(buf * kRows + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
                         g[j] = exp2_2(t[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        if (!kInside && (done.start >> j & 1))
-                            h = state_of_token(p.cu, p.cu_is_int64, seqs, p.state, p.channels, t0 + j, c);
+                        if (!kInside) h = state_of_strips<STRIPS>(p, p.state, done.start >> j, kPiece, w0 + j, c, me.strip, h);
                         before[j] = h;
                         h = fma2(g[j], h, mul2(beta[j], xs[j]));
-                        if (!kInside && !(done.covered >> j & 1)) h = splat2(0.0f);
+                        if (!kInside && !(covered >> j & 1)) h = splat2(0.0f);
                     }
                     T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
                     T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
                     T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) {
-                        if (!kInside && (done.end >> j & 1))
-                            e = state_of_token(p.cu, p.cu_is_int64, seqs, d.d_new_state, p.channels, t0 + j, c);
+                        if (!kInside)
+                            e = state_of_strips<STRIPS>(p, d.d_new_state, done.end >> j, kPiece, w0 + j, c, me.strip, e);
                         const F2 G = add2(dys[j], e);
                         e = mul2(g[j], G);
                         const F2 dl = mul2(e, before[j]);
                         F2 vx = mul2(G, beta[j]), va = mul2(mul2(dl, minus_decay), sig[j]);
                         F2 vb = mul2(mul2(vx, xs[j]), fma2(beta[j], splat2(-1.0f), splat2(1.0f)));
-                        if (!kInside && !(done.covered >> j & 1)) {
+                        if (!kInside && !(covered >> j & 1)) {
                             vx = va = vb = e = splat2(0.0f);
                         } else {
                             sum_A = fma2(dl, t[j], sum_A);
                             sum_dt = add2(sum_dt, va);
                         }
-                        if (!kInside && (done.start >> j & 1))
-                            store_state_of_token(p.cu, p.cu_is_int64, seqs, d.d_state, p.channels, t0 + j, c, e);
+                        if (!kInside)
+                            store_state_of_strips<STRIPS>(p, d.d_state, done.start >> j, kPiece, w0 + j, c, me.strip, e);
                         if (kInside || t0 + j < tokens) {
                             store_pair(row_at<T>(dx, j, d.dx_stride), vx, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
                             store_pair(row_at<T>(da, j, d.da_stride), va, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
@@ -944,7 +979,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                         }
                     }
                 };
-                if ((done.start | done.end) == 0 && done.covered == kAllTokens<kPiece> && all_channels && d.grad_pairs)
+                if ((done.start | done.end) == 0 && done.covered == kAllTokens<kSpan> && all_channels && d.grad_pairs)
                     finish(std::true_type{});
                 else
                     finish(std::false_type{});
@@ -955,8 +990,15 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
     // sums over the CTA's warps, in order, then over the cluster's CTAs
     __syncthreads();
     const float2 va = unpack2(sum_A), vd = unpack2(sum_dt);
-    float4* sums = state_maps;  // nobody reads the maps any more
-    if (warp < W) sums[warp * 32] = make_float4(va.x, va.y, vd.x, vd.y);
+    float4 part = make_float4(va.x, va.y, vd.x, vd.y);
+    if (STRIPS > 1) {  // the other strip's tokens
+        part.x += __shfl_xor_sync(0xffffffffu, part.x, 16);
+        part.y += __shfl_xor_sync(0xffffffffu, part.y, 16);
+        part.z += __shfl_xor_sync(0xffffffffu, part.z, 16);
+        part.w += __shfl_xor_sync(0xffffffffu, part.w, 16);
+    }
+    float4* sums = state_maps + lane;  // nobody reads the maps any more
+    if (warp < W) sums[warp * 32] = part;
     __syncthreads();
     if (warp != 0) return;
     auto add_up = [](const float4* v, int n) {
@@ -967,10 +1009,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
         }
         return s;
     };
-    st_cluster_f4(tc05::smem_u32(cta_sums + rank * 32), summed, 0, add_up(sums, W));
+    st_cluster_f4(tc05::smem_u32(cta_sums + rank * 32 + lane), summed, 0, add_up(sums, W));
     if (rank != 0) return;
     if (!tc05::mbar_wait(summed, 0)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-    const float4 s = add_up(cta_sums, R);
+    const float4 s = add_up(cta_sums + lane, R);
+    if (me.strip != 0) return;
     constexpr float kLn2 = 0.6931471805599453f;  // l = ln 2 log2 g
     if (ok0) d.dA_log[c] = s.x * kLn2, d.ddt_bias[c] = s.z;
     if (ok1) d.dA_log[c + 1] = s.y * kLn2, d.ddt_bias[c + 1] = s.w;
@@ -1054,10 +1097,10 @@ __global__ void __launch_bounds__(128) gdn_scan_step_kernel(const ScanParams p, 
     }
 }
 
-// `kernel` with gridDim = (cluster, groups of kScanCh channels); `attr` outlives the launch.
-static cudaLaunchConfig_t scan_config(int cluster, int channels, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
+// `kernel` with gridDim = (cluster, groups of channels); `attr` outlives the launch.
+static cudaLaunchConfig_t scan_config(int cluster, unsigned groups, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster, (channels + kScanCh - 1) / kScanCh);
+    cfg.gridDim = dim3(cluster, groups);
     cfg.blockDim = dim3(kScanThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -1078,7 +1121,7 @@ static int active_clusters(Kernel kernel, int n, size_t smem, size_t most, int (
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
     if (cache[dev][n] == 0) {
         cudaLaunchAttribute attr[1];
-        const cudaLaunchConfig_t cfg = scan_config(n, kScanCh, smem, nullptr, attr);
+        const cudaLaunchConfig_t cfg = scan_config(n, 1, smem, nullptr, attr);
         int got = 0;
         const bool ok =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) == cudaSuccess &&
@@ -1090,52 +1133,64 @@ static int active_clusters(Kernel kernel, int n, size_t smem, size_t most, int (
     return cache[dev][n];
 }
 
-// CTAs per cluster.  A cluster's CTAs sit in one GPC, so how many clusters run
-// at once depends on their size in steps (of 16 tiles' CTAs on a B200: 33
-// clusters of 4, 22 of 6, 15 of 8 or 9); the size taken is the one with the
-// fewest tiles in a row, waves x tiles / size.  `active` gives the clusters
-// that run at once.
+// CTAs per cluster, and the tiles that a CTA then walks one after another.  A
+// cluster's CTAs sit in one GPC, so how many clusters run at once depends on
+// their size in steps (on a B200 33 clusters of 4, 22 of 6, 15 of 8 or 9); the
+// size with the fewest tiles in a row, waves x tiles / size, is taken.  `active`
+// gives the clusters that run at once.
+struct ClusterShape {
+    int size;
+    int64_t steps;
+};
 template <typename Active>
-static int scan_cluster(int64_t tiles, int channels, Active active) {
-    const int64_t groups = (channels + kScanCh - 1) / kScanCh;
-    int best = 0;
-    int64_t best_steps = INT64_MAX;
+static ClusterShape scan_cluster(int64_t tiles, int64_t groups, Active active) {
+    ClusterShape best = {0, INT64_MAX};
     for (int r = 1; r <= kScanMaxCluster && (r == 1 || r <= tiles); ++r) {
         const int64_t n = active(r);
         if (n < 1) continue;
         const int64_t steps = (groups + n - 1) / n * ((tiles + r - 1) / r);
-        if (steps < best_steps) best = r, best_steps = steps;
+        if (steps < best.steps) best = {r, steps};
     }
     return best;
 }
 
-// Launches `kernel` in clusters of the best size; smem(r) bytes for size r.
+// A kernel with one and with two strips to a warp: `rows` tokens per strip and
+// tile, smem(r) bytes in clusters of r.  Two strips of 32 channels make twice the groups and
+// half the tiles: better clusters for few channels (1 x 40000 x 1024: 16 groups
+// in clusters of 6 fill 96 SMs, 32 in clusters of 4 fill 128).
 template <typename Smem, typename... Params, typename... Args>
-static cudaError_t launch_scan_clusters(void (*kernel)(Params...), int (*cache)[kScanMaxCluster + 1], int64_t tiles,
-                                        int channels, Smem smem, cudaStream_t s, Args... args) {
-    const int r = scan_cluster(tiles, channels, [&](int n) {
-        return active_clusters(kernel, n, smem(n), smem(kScanMaxCluster), cache);
-    });
-    if (r == 0) return cudaErrorInvalidConfiguration;
+static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Params...), int (*cache)[64][kScanMaxCluster + 1],
+                                        int64_t tokens, int rows, int channels, Smem smem, cudaStream_t s, Args... args) {
+    const int64_t groups[2] = {(channels + 63) / 64, (channels + 31) / 32};
+    void (*const kernels[2])(Params...) = {one, two};
+    ClusterShape shape[2];
+    for (int i = 0; i < 2; ++i) {
+        const int tile = rows * (i + 1);
+        shape[i] = scan_cluster((tokens + tile - 1) / tile, groups[i], [&](int n) {
+            return active_clusters(kernels[i], n, smem(n), smem(kScanMaxCluster), cache[i]);
+        });
+    }
+    const int i = shape[1].steps < shape[0].steps ? 1 : 0;
+    if (shape[i].size == 0) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = scan_config(r, channels, smem(r), s, attr);
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    const cudaLaunchConfig_t cfg = scan_config(shape[i].size, static_cast<unsigned>(groups[i]), smem(shape[i].size), s, attr);
+    return cudaLaunchKernelEx(&cfg, kernels[i], static_cast<Params>(args)...);
 }
 
 template <typename T>
 static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
-    constexpr int kTile = kScanWarps * kScanPiece<T>;
-    static int cache[64][kScanMaxCluster + 1];
-    const auto smem = [](int r) { return (2 * kTile + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
-    return launch_scan_clusters(gdn_scan_kernel<T>, cache, (p.tokens + kTile - 1) / kTile, p.channels, smem, s, p);
+    constexpr int kRows = kScanWarps * kScanPiece<T>;
+    static int cache[2][64][kScanMaxCluster + 1];
+    const auto smem = [](int r) { return (2 * kRows + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
+    return launch_scan_clusters(gdn_scan_kernel<T, 1>, gdn_scan_kernel<T, 2>, cache, p.tokens, kRows, p.channels, smem, s, p);
 }
 
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
-    static int cache[64][kScanMaxCluster + 1];
+    static int cache[2][64][kScanMaxCluster + 1];
     const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kScanWarps + 3 * r) * 32 * sizeof(float4); };
-    return launch_scan_clusters(gdn_scan_backward_kernel<T>, cache, (p.tokens + kGradTile - 1) / kGradTile, p.channels, smem,
-                                s, p, d);
+    return launch_scan_clusters(gdn_scan_backward_kernel<T, 1>, gdn_scan_backward_kernel<T, 2>, cache, p.tokens, kGradRows,
+                                p.channels, smem, s, p, d);
 }
 
 template <typename T>
