@@ -787,18 +787,29 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             state = checkpoint(k + 1);
             if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
             auto chain = [&](float4* m, bool back) {  // in place: a piece's map makes way for what comes before it
+                constexpr int kAhead = 5;  // maps read together
+                static_assert(W % kAhead == 0, "whole batches");
                 Map2 all = {splat2(1.0f), splat2(0.0f)};
 #pragma unroll
-                for (int i = 0; i < STRIPS * W; ++i) {
-                    const int n = back ? STRIPS * W - 1 - i : i, word = me.word(n, 32);
-                    const float4 e = m[word];
-                    const float2 va = unpack2(all.A), vh = unpack2(all.H);
-                    if (STRIPS > 1) __syncwarp();  // every strip has read the word
-                    if (n % STRIPS == me.strip) m[word] = make_float4(va.x, va.y, vh.x, vh.y);
-                    const F2 A = pack2(e.x, e.y);
-                    const float2 r = unpack2(fma2(A, all.H, pack2(e.z, e.w))), a = unpack2(mul2(all.A, A));
-                    all.H = pack2(is_start(e.x) ? e.z : r.x, is_start(e.y) ? e.w : r.y);
-                    all.A = pack2(is_start(e.x) ? e.x : a.x, is_start(e.y) ? e.y : a.y);
+                for (int i = 0; i < STRIPS * W; i += kAhead) {
+                    float4 e[kAhead];
+                    int word[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        word[j] = me.word(back ? STRIPS * W - 1 - i - j : i + j, 32);
+                        e[j] = m[word[j]];
+                    }
+                    if (STRIPS > 1) __syncwarp();  // both strips have read the words
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const int n = back ? STRIPS * W - 1 - i - j : i + j;
+                        const float2 va = unpack2(all.A), vh = unpack2(all.H);
+                        if (n % STRIPS == me.strip) m[word[j]] = make_float4(va.x, va.y, vh.x, vh.y);
+                        const F2 A = pack2(e[j].x, e[j].y);
+                        const float2 r = unpack2(fma2(A, all.H, pack2(e[j].z, e[j].w))), a = unpack2(mul2(all.A, A));
+                        all.H = pack2(is_start(e[j].x) ? e[j].z : r.x, is_start(e[j].y) ? e[j].w : r.y);
+                        all.A = pack2(is_start(e[j].x) ? e[j].x : a.x, is_start(e[j].y) ? e[j].y : a.y);
+                    }
                 }
                 return all;
             };
