@@ -267,10 +267,10 @@ __device__ __forceinline__ bool scan_bounds(const ScanParams& p, int64_t n, int6
 // A piece of the recurrence is an affine map of the state before it,
 // h -> A h + H, as (A0, A1, H0, H1) for a thread's two channels.  A piece in
 // which a sequence starts does not depend on the state before it: A = -0
-// says so (decays are >= +0, and a product keeps the sign).  The fast forms
-// multiply all the same, which drops a finite state; an infinity or a NaN
-// would cross into the next sequence as a NaN, so a chain that ends in one is
-// done again with the forms that select.
+// says so (decays are >= +0).  The fast forms multiply all the same, which
+// drops a finite state; an infinity or a NaN would cross into the next sequence
+// as a NaN, so a chain that ends in one is done again with the forms that
+// select.
 __device__ __forceinline__ bool is_start(float a) { return __float_as_uint(a) == 0x80000000u; }
 __device__ __forceinline__ F2 apply_map(float4 m, F2 h) { return fma2(pack2(m.x, m.y), h, pack2(m.z, m.w)); }
 __device__ __forceinline__ F2 apply_map_select(float4 m, F2 h) {
@@ -545,14 +545,23 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
             const float4* last = maps + (buf * kRows + kPiece - 1) * 32;  // a piece's whole map is its last token's
             float4* before = befores + buf * W * 32;
             F2 A = splat2(1.0f), H = splat2(0.0f);
+            uint32_t sx = 0, sy = 0;  // the sign of A, kept apart: the product would lose it in two starts
+            const auto factor = [&] {
+                const float2 a = unpack2(A);
+                return make_float2(__uint_as_float((__float_as_uint(a.x) & 0x7fffffffu) | (sx & 0x80000000u)),
+                                   __uint_as_float((__float_as_uint(a.y) & 0x7fffffffu) | (sy & 0x80000000u)));
+            };
 #pragma unroll
             for (int i = 0; i < STRIPS * W; ++i) {
                 const float4 m = last[me.word(i, kPiece * 32)];
-                const float2 va = unpack2(A), vh = unpack2(H);
+                const float2 va = factor(), vh = unpack2(H);
                 if (i % STRIPS == me.strip) before[me.word(i, 32)] = make_float4(va.x, va.y, vh.x, vh.y);
                 H = apply_map(m, H);
                 A = mul2(A, pack2(m.x, m.y));
+                sx |= __float_as_uint(m.x), sy |= __float_as_uint(m.y);
             }
+            const float2 signed_A = factor();
+            A = pack2(signed_A.x, signed_A.y);
             if (__any_sync(0xffffffffu, has_nan(A) || has_nan(H))) {
                 const Map2 all = chain_select<STRIPS>(last, STRIPS * W, kPiece * 32, before);
                 A = all.A, H = all.H;
@@ -580,27 +589,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
             __syncwarp();
             if (lane == 0) tc05::mbar_arrive(ready + 8 * buf);
             carry = next;
-            __syncwarp();  // the chain's words from both strips
-            if (p.ckpt) {
-#pragma unroll
-                for (int i = 0; i < kTile; i += kScanCkpt) {
-                    const int t = (k * R + rank) * kTile + i;
-                    F2 at = in;
-                    if (i) {  // the token before it: its piece's start, and on from there
-                        const int piece = (i - 1) / kPiece, row = buf * kRows + (i - 1) % kPiece;
-                        at = apply_map_select(before[me.word(piece, 32)], at);
-                        at = apply_map_select(maps[row * 32 + me.word(piece, kPiece * 32)], at);
-                    }
-                    const float2 v = unpack2(at);
-                    float* ck = p.ckpt + static_cast<int64_t>(t / kScanCkpt) * p.channels;
-                    if (t < tokens && me.strip == 0 && ok0) ck[c] = v.x;
-                    if (t < tokens && me.strip == 0 && ok1) ck[c + 1] = v.y;
-                }
+            if (p.ckpt && k == 0 && rank == 0 && me.strip == 0) {  // ahead of the first token, for completeness
+                if (ok0) p.ckpt[c] = 0.0f;
+                if (ok1) p.ckpt[c + 1] = 0.0f;
             }
         }
         return;
     }
 
+    // the piece's token whose state is the next checkpoint, if it has one (tiles are whole checkpoints)
+    const int kept = kScanCkpt - 1 - (warp * kSpan + me.strip * kPiece) % kScanCkpt;
+    static_assert(kTile % kScanCkpt == 0, "whole checkpoints");
     Spans span = {0, 0, 0, 0, 0};
     uint32_t ends = 0;  // of the tile before
     for (int k = 0; k <= steps; ++k) {
@@ -661,6 +660,15 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                 in = apply_map_select(before, tile_in);
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
+            }
+            if (p.ckpt && kept < kPiece && t0 + kept + 1 < tokens) {
+                F2 v = h[0];
+#pragma unroll
+                for (int j = 1; j < kPiece; ++j)
+                    if (j == kept) v = h[j];
+                float* ck = p.ckpt + static_cast<int64_t>((t0 + kept + 1) / kScanCkpt) * p.channels + c;
+                if (ok0) ck[0] = unpack2(v).x;
+                if (ok1) ck[1] = unpack2(v).y;
             }
             T* out = row_at<T>(out0, t0, p.out_stride);
             if (ends == 0 && w0 + kSpan <= tokens && p.out_pairs && all_channels) {
@@ -786,25 +794,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             const F2 state_in = state;
             state = checkpoint(k + 1);
             if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-            auto chain = [&](float4* m, bool back) {  // in place: a piece's map makes way for what comes before it
-                constexpr int kAhead = 5;  // maps read together
+            // In place: a piece's map makes way for what comes before it (a lane's
+            // words are its own).
+            auto chain = [&](float4* m, int step) {  // a word every `step`
+                constexpr int kAhead = 5;            // maps read together
                 static_assert(W % kAhead == 0, "whole batches");
                 Map2 all = {splat2(1.0f), splat2(0.0f)};
 #pragma unroll
-                for (int i = 0; i < STRIPS * W; i += kAhead) {
+                for (int i = 0; i < STRIPS * W; i += kAhead, m += kAhead * step) {
                     float4 e[kAhead];
-                    int word[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) e[j] = m[j * step];
 #pragma unroll
                     for (int j = 0; j < kAhead; ++j) {
-                        word[j] = me.word(back ? STRIPS * W - 1 - i - j : i + j, 32);
-                        e[j] = m[word[j]];
-                    }
-                    if (STRIPS > 1) __syncwarp();  // both strips have read the words
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        const int n = back ? STRIPS * W - 1 - i - j : i + j;
                         const float2 va = unpack2(all.A), vh = unpack2(all.H);
-                        if (n % STRIPS == me.strip) m[word[j]] = make_float4(va.x, va.y, vh.x, vh.y);
+                        m[j * step] = make_float4(va.x, va.y, vh.x, vh.y);
                         const F2 A = pack2(e[j].x, e[j].y);
                         const float2 r = unpack2(fma2(A, all.H, pack2(e[j].z, e[j].w))), a = unpack2(mul2(all.A, A));
                         all.H = pack2(is_start(e[j].x) ? e[j].z : r.x, is_start(e[j].y) ? e[j].w : r.y);
@@ -813,14 +817,24 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                 }
                 return all;
             };
-            const Map2 all_grad = chain(grad_maps + buf * W * 32, true);
-            const float2 va = unpack2(all_grad.A), vh = unpack2(all_grad.H);
+            // Pieces in token order are kLanes words apart.  With two strips, the
+            // lanes of one chain the states, forward, and those of the other the
+            // gradients, backward, in one go.
+            float4* first_state = state_maps + buf * W * 32 + me.lane;
+            float4* last_grad = grad_maps + buf * W * 32 + (STRIPS * W - 1) * me.kLanes + me.lane;
+            const bool states = STRIPS > 1 && me.strip == 0;
+            const Map2 all_grad = chain(states ? first_state : last_grad, states ? me.kLanes : -me.kLanes);
+            float2 va = unpack2(all_grad.A), vh = unpack2(all_grad.H);
+            if (STRIPS > 1) {
+                va.x = __shfl_sync(0xffffffffu, va.x, lane | 16), va.y = __shfl_sync(0xffffffffu, va.y, lane | 16);
+                vh.x = __shfl_sync(0xffffffffu, vh.x, lane | 16), vh.y = __shfl_sync(0xffffffffu, vh.y, lane | 16);
+            }
             const uint32_t to = tc05::smem_u32(ranks + (buf * R + rank) * 32 + lane);
             // A slot is written again two tiles on: by then this CTA has every
             // CTA's map of the tile between, sent after that CTA had read this one's.
             for (int r = 0; r < R; ++r)
                 st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
-            chain(state_maps + buf * W * 32, false);
+            if (STRIPS == 1) chain(first_state, me.kLanes);
             if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
             if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
             const float4* every = ranks + buf * R * 32 + lane;
@@ -873,7 +887,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             }
         };
         fetch(0);
-        Spans span = {0, 0, 0, 0, 0}, done = span;
+        Spans span = {0, 0, 0, 0, 0};
+        struct {
+            uint32_t start, end, covered;
+        } done = {0, 0, 0};  // of the tile before
         for (int k = 0; k <= steps; ++k) {
             if (k < steps) {
                 const int w0 = tile_start(k) + warp * kSpan, buf = k & 1;
@@ -882,53 +899,49 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                 else
                     span = {0, 0, 0, 0, 0};
                 const bool special = (span.start | span.end | (~span.covered & kAllTokens<kSpan>)) != 0;
-                F2 z[kPiece], e[kPiece], u[kPiece], in[kPiece];
+                F2 z[kPiece], g[kPiece], e[kPiece];
 #pragma unroll
-                for (int j = 0; j < kPiece; ++j) z[j] = add2(raw_to_f2<T>(a[j]), dtb);
-                F2 sig[kPiece];
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) sig[j] = z[j];
-                log2_decays(z, e, rate);
+                for (int j = 0; j < kPiece; ++j) g[j] = z[j] = add2(raw_to_f2<T>(a[j]), dtb);
+                log2_decays(g, e, rate);
+                F2 A = splat2(1.0f), H = splat2(0.0f), B = splat2(1.0f), E = splat2(0.0f);
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) {
                     // sigmoid(z) = 1 / (1 + e) or e / (1 + e), e = exp(-|z|)
-                    const float2 v = unpack2(sig[j]), w = unpack2(e[j]);
+                    const float2 v = unpack2(z[j]), w = unpack2(e[j]);
                     const float2 q = make_float2(rcp_approx(1.0f + w.x), rcp_approx(1.0f + w.y));
-                    sig[j] = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
+                    const F2 sig = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
                     const F2 beta = sigmoid2(raw_to_f2<T>(b[j]));
-                    vals.put(buf * kRows + warp * kPiece + j, z[j], beta, sig[j], x[j], dy[j]);
-                    z[j] = exp2_2(z[j]);
-                    u[j] = mul2(beta, raw_to_f2<T>(x[j]));
-                    in[j] = raw_to_f2<T>(dy[j]);
+                    vals.put(buf * kRows + warp * kPiece + j, g[j], beta, sig, x[j], dy[j]);
+                    g[j] = exp2_2(g[j]);
+                    z[j] = mul2(beta, raw_to_f2<T>(x[j]));
                 }
-                fetch(k + 1);
-                F2 A = splat2(1.0f), H = splat2(0.0f), B = splat2(1.0f), E = splat2(0.0f);
                 if (!special) {
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        A = mul2(A, z[j]);
-                        H = fma2(z[j], H, u[j]);
+                        A = mul2(A, g[j]);
+                        H = fma2(g[j], H, z[j]);
                     }
                     B = A;
 #pragma unroll
-                    for (int j = kPiece - 1; j >= 0; --j) E = mul2(z[j], add2(in[j], E));
+                    for (int j = kPiece - 1; j >= 0; --j) E = mul2(g[j], add2(raw_to_f2<T>(dy[j]), E));
                 } else {
                     const int at = me.strip * kPiece;
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
                         const bool covered = span.covered >> (at + j) & 1, start = span.start >> (at + j) & 1;
                         H = state_of_strips<STRIPS>(p, p.state, span.start >> j, kPiece, w0 + j, c, me.strip, H);
-                        A = start || !covered ? splat2(-0.0f) : mul2(A, z[j]);
-                        H = covered ? fma2(z[j], H, u[j]) : splat2(0.0f);
+                        A = start || !covered ? splat2(-0.0f) : mul2(A, g[j]);
+                        H = covered ? fma2(g[j], H, z[j]) : splat2(0.0f);
                     }
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) {
                         const bool covered = span.covered >> (at + j) & 1, end = span.end >> (at + j) & 1;
                         E = state_of_strips<STRIPS>(p, d.d_new_state, span.end >> j, kPiece, w0 + j, c, me.strip, E);
-                        B = end || !covered ? splat2(-0.0f) : mul2(B, z[j]);
-                        E = covered ? mul2(z[j], add2(in[j], E)) : splat2(0.0f);
+                        B = end || !covered ? splat2(-0.0f) : mul2(B, g[j]);
+                        E = covered ? mul2(g[j], add2(raw_to_f2<T>(dy[j]), E)) : splat2(0.0f);
                     }
                 }
+                fetch(k + 1);
                 const float2 va = unpack2(A), vh = unpack2(H), vb = unpack2(B), ve = unpack2(E);
                 state_maps[(buf * W + warp) * 32 + lane] = make_float4(va.x, va.y, vh.x, vh.y);
                 grad_maps[(buf * W + warp) * 32 + lane] = make_float4(vb.x, vb.y, ve.x, ve.y);
@@ -995,7 +1008,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                 else
                     finish(std::false_type{});
             }
-            done = span;
+            done = {span.start, span.end, span.covered};
         }
     }
     // sums over the CTA's warps, in order, then over the cluster's CTAs

@@ -151,27 +151,33 @@ def test_scan_tokens_of_no_sequence(pkg, cuda_dev, head, tail):
 
 
 @gpu
-def test_scan_sequences_do_not_leak(pkg, cuda_dev):
-    """NaN and infinity in one sequence leave its neighbours alone, forward and backward."""
-    lens = [40, 100, 3, 200]
-    i = make(lens, 64, torch.bfloat16, cuda_dev)
+@pytest.mark.parametrize("lens", [[40, 100, 3, 200], [40, 130, 20, 300], [3, 250, 9, 9, 9, 300], [1, 125, 8, 8, 8, 8, 400]],
+                         ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("C", [64, 1024])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_scan_sequences_do_not_leak(pkg, cuda_dev, lens, C, dtype):
+    """NaN and infinity in the second sequence leave its neighbours alone, forward and backward, with any
+    number of sequences starting in the tile where it ends."""
+    i = make(lens, C, dtype, cuda_dev)
+    T, N, t0, t1 = sum(lens), len(lens), lens[0], lens[0] + lens[1]
+    others = [n for n in range(N) if n != 1]
     good = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
     good_grads = backward(pkg, i)
+    keep = torch.ones(T, dtype=torch.bool, device=cuda_dev)
+    keep[t0:t1] = False
     for bad in (float("nan"), float("inf")):
         j = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in i.items()}
-        j["x"][60] = bad
+        j["x"][t0 + 20] = bad
         j["state"][1] = bad
-        j["dy"][70] = bad
+        j["dy"][t0 + 30] = bad
         j["dns"][1] = bad
         y, ns = pkg.recurrence.launch_scan(*gates(j), j["cu"], j["state"])
-        keep = torch.ones(343, dtype=torch.bool, device=cuda_dev)
-        keep[40:140] = False
-        assert torch.equal(y[keep], good[0][keep]) and not y[60].isfinite().any()
-        assert torch.equal(ns[[0, 2, 3]], good[1][[0, 2, 3]])
+        assert torch.equal(y[keep], good[0][keep]) and not y[t0 + 20].isfinite().any()
+        assert torch.equal(ns[others], good[1][others])
         grads = backward(pkg, j)
         for g, w in zip(grads[:3], good_grads[:3]):
             assert torch.equal(g[keep], w[keep])
-        assert torch.equal(grads[5][[0, 2, 3]], good_grads[5][[0, 2, 3]])
+        assert torch.equal(grads[5][others], good_grads[5][others])
 
 
 @gpu
