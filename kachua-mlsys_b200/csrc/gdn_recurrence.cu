@@ -94,9 +94,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // the smallest maximal relative error (Lawson): 1.9e-7.  lg2.approx is not
 // usable here: its error near 1 is absolute (2^-22), and softplus of a
 // strongly negative argument is a tiny number whose relative error the
-// recurrence multiplies by its memory.  ex2.approx serves for 2^t: measured,
-// within 1.2 units in the last place for t in [-20, 0], and off by 0.05 to 0.1
-// on average for t in [-0.01, 0], where a decay's memory is long.
+// recurrence multiplies by its memory.
 template <int N>
 __device__ __forceinline__ void log2_decays(F2 (&z)[N], F2 (&u)[N], F2 rate) {
     constexpr float kLog1p[8] = {0.9999998211860657f, -0.4999740421772003f, 0.33275479078292847f, -0.24495463073253632f, 0.17745240032672882f, -0.10768169909715652f, 0.04408962279558182f, -0.008539206348359585f};
@@ -116,16 +114,32 @@ __device__ __forceinline__ void log2_decays(F2 (&z)[N], F2 (&u)[N], F2 rate) {
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] = mul2(rate, fma2(u[i], r[i], z[i]));
 }
-__device__ __forceinline__ F2 exp2_2(F2 t) {
-    const float2 v = unpack2(t);
-    return pack2(ex2_approx(v.x), ex2_approx(v.y));
+// t -> 2^t of N pairs, t <= 0.  ex2.approx is within 1.2 units in the last
+// place, but off in one direction (measured: by 0.05 of them on average at
+// -0.001, 0.2 at -0.01), which a decay's memory of a thousand tokens adds up to
+// 1e-5.  So decays above 2^-0.25 are 1 + t q(t), q fitted like the polynomial
+// above (3e-9; 0.4 units, 0.001 on average).
+template <int N>
+__device__ __forceinline__ void exp2_decays(F2 (&t)[N]) {
+    constexpr float kExp2[4] = {0.693146824836731f, 0.24021293222904205f, 0.05534094199538231f, 0.008836725726723671f};
+    F2 q[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = fma2(splat2(kExp2[3]), t[i], splat2(kExp2[2]));
+#pragma unroll
+    for (int d = 1; d >= 0; --d)
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = fma2(q[i], t[i], splat2(kExp2[d]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float2 v = unpack2(t[i]), near = unpack2(fma2(q[i], t[i], splat2(1.0f)));
+        t[i] = pack2(v.x > -0.25f ? near.x : ex2_approx(v.x), v.y > -0.25f ? near.y : ex2_approx(v.y));
+    }
 }
 template <int N>
 __device__ __forceinline__ void decays(F2 (&z)[N], F2 rate) {
     F2 u[N];
     log2_decays(z, u, rate);
-#pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = exp2_2(z[i]);
+    exp2_decays(z);
 }
 __device__ __forceinline__ F2 sigmoid2(F2 b) {
     const float2 e = unpack2(mul2(b, splat2(-kLog2e)));
@@ -912,9 +926,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                     const F2 sig = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
                     const F2 beta = sigmoid2(raw_to_f2<T>(b[j]));
                     vals.put(buf * kRows + warp * kPiece + j, g[j], beta, sig, x[j], dy[j]);
-                    g[j] = exp2_2(g[j]);
                     z[j] = mul2(beta, raw_to_f2<T>(x[j]));
                 }
+                exp2_decays(g);
                 if (!special) {
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
@@ -967,8 +981,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
                         vals.get(buf * kRows + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
-                        g[j] = exp2_2(t[j]);
+                        g[j] = t[j];
                     }
+                    exp2_decays(g);
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
                         if (!kInside) h = state_of_strips<STRIPS>(p, p.state, done.start >> j, kPiece, w0 + j, c, me.strip, h);
