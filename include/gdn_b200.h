@@ -271,8 +271,8 @@ int gdn_prefill_launch_noalloc(const GdnPrefillArgs* args, void* stream);
  *   h_t = g_t h_{t-1} + sigmoid(b_t) x_t,  g_t = exp(-exp(A_log) softplus(a_t + dt_bias)),  y_t = h_t
  *   x, a, b     [T, C] of `dtype`; *_stride elements between tokens (>= C),
  *               channels contiguous: column blocks of one projection's output
- *               need no copy.  Any alignment; rows on 16-byte boundaries are
- *               read as vectors.
+ *               need no copy.  Any alignment; rows that start on a boundary of
+ *               two elements are read two at a time.  Strides up to 2^29.
  *   A_log, dt_bias fp32 [C]
  *   state       fp32 [N, C] or NULL (zero); must not alias new_state
  *   cu_seqlens  int32 or int64 [N + 1], non-decreasing, cu[0] >= 0, cu[N] <= T

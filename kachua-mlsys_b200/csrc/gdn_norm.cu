@@ -100,7 +100,8 @@ __device__ __forceinline__ Raw8<T> load8(const T* row, Cols c) {
             for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(row + c.first)[i];
         }
     } else {
-        // all loads first, from the row's start where the column is outside
+        // all loads first, from the row's start where the column is outside:
+        // `row` is a row of the tensor even where none of the columns counts
         T e[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = row[c.in(i) ? c.first + i * c.step : 0];
@@ -399,12 +400,12 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
     unsigned items[kGatedItems];
 #pragma unroll
     for (int n = 0; n < kGatedItems; ++n) {
-        const unsigned item = (blockIdx.x * kGatedItems + n) * kGroups + threadIdx.x / LANES;
+        items[n] = (blockIdx.x * kGatedItems + n) * kGroups + threadIdx.x / LANES;
+        const unsigned item = items[n] < p.items ? items[n] : 0;
         const unsigned token = item / p.heads, head = item - token * p.heads;
         const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
-        items[n] = item;
-        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, {0, 1, item < p.items ? 8 : 0});
-        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, {0, 1, item < p.items ? 8 : 0});
+        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
+        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
     }
     F2 w[4];
     load_weight8<T, VEC>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _capi
-from .recurrence import DTYPES, _call, _dense, _fault, _need, _ptr, _rows
+from .recurrence import DTYPES, _call, _dense, _fault, _like, _need, _ptr, _rows
 
 QUANT = {None: _capi.QUANT_NONE, "row": _capi.QUANT_ROW, "group": _capi.QUANT_GROUP}
 GROUP = 128
@@ -73,20 +73,20 @@ def launch_add_norm(x, residual, weight, eps=1e-6, output=None, new_residual=Non
     if residual is not None:
         res_stride = _rows(residual, "residual", x.dtype, rows, width, dev)
         if new_residual is None:
-            new_residual = torch.empty((rows, width), dtype=x.dtype, device=dev)
+            new_residual = _like(x)
         else:
             _dense(new_residual, "new_residual", x.dtype, (rows, width), dev)
     else:
         _need(new_residual is None, "new_residual needs a residual")
     odt = torch.float8_e4m3fn if quant else x.dtype
     if output is None:
-        output = torch.empty((rows, width), dtype=odt, device=dev)
+        output = _like(x, odt)
     else:
         _dense(output, "output", odt, (rows, width), dev)
     if quant:
         scale_shape = (rows, 1 if quant == "row" else width // GROUP)
         if scale is None:
-            scale = torch.empty(scale_shape, dtype=torch.float32, device=dev)
+            scale = x.new_empty(scale_shape, dtype=torch.float32)
         else:
             _dense(scale, "scale", torch.float32, scale_shape, dev)
     else:
@@ -112,13 +112,13 @@ def launch_add_norm_backward(d_output, new_residual, weight, eps=1e-6, d_new_res
     dy_stride = _rows(d_output, "d_output", dt, rows, width, dev)
     dr_stride = 0 if d_new_residual is None else _rows(d_new_residual, "d_new_residual", dt, rows, width, dev)
     if dx is None:
-        dx = torch.empty((rows, width), dtype=dt, device=dev)
+        dx = _like(new_residual)
     else:
         _dense(dx, "dx", dt, (rows, width), dev)
-    d_weight = torch.empty(width, dtype=torch.float32, device=dev)
+    d_weight = _like(weight, torch.float32)
     lib = _capi.load()
     need = int(lib.gdn_add_norm_backward_workspace_size(rows, width))
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    workspace = weight.new_empty(need, dtype=torch.uint8)
     args = _capi.GdnAddNormArgs(_ptr(new_residual), None, r_stride, 0, _ptr(weight), wdt, DTYPES[dt], 0, eps, rows, width,
                                 None, None, None)
     g = _capi.GdnNormGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_residual), dr_stride, _ptr(dx), None, _ptr(d_weight))
@@ -176,13 +176,15 @@ def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):
     dev = x.device
     odt = torch.float8_e4m3fn if quant else x.dtype
     if output is None:
-        output = torch.empty(shape, dtype=odt, device=dev)
+        output = _like(x, odt)
+        if output.shape != shape:
+            output = output.view(shape)
     else:
         _dense(output, "output", odt, shape, dev)
-    _need(tokens == 0 or output.data_ptr() != z.data_ptr(), "output must not be z")
+        _need(tokens == 0 or output.data_ptr() != z.data_ptr(), "output must not be z")
     if quant:
         if scale is None:
-            scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+            scale = x.new_empty(shape[:-1], dtype=torch.float32)
         else:
             _dense(scale, "scale", torch.float32, shape[:-1], dev)
     else:
@@ -223,17 +225,17 @@ def launch_gated_norm_backward(d_output, x, z, weight, eps=1e-6, dx=None, dz=Non
         d_output = d_output.view(-1, heads, dim)
     dys = _heads(d_output, "d_output", x.dtype, x.shape, dev)
     if dx is None:
-        dx = torch.empty(shape, dtype=x.dtype, device=dev)
+        dx = _like(x).view(shape)
     else:
         _dense(dx, "dx", x.dtype, shape, dev)
     if dz is None:
-        dz = torch.empty(shape, dtype=x.dtype, device=dev)
+        dz = _like(x).view(shape)
     else:
         _dense(dz, "dz", x.dtype, shape, dev)
-    d_weight = torch.empty(dim, dtype=torch.float32, device=dev)
+    d_weight = _like(weight, torch.float32)
     lib = _capi.load()
     need = int(lib.gdn_gated_norm_backward_workspace_size(tokens, heads, dim))
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    workspace = weight.new_empty(need, dtype=torch.uint8)
     args = _capi.GdnGatedNormArgs(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype], 0, eps, tokens, heads, dim,
                                   None, None)
     g = _capi.GdnNormGradArgs(_ptr(d_output), dys, None, 0, _ptr(dx), _ptr(dz), _ptr(d_weight))
