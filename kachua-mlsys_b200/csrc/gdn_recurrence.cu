@@ -323,24 +323,42 @@ __device__ __noinline__ F2 fold_select(const float4* maps, int n, int step, F2 h
     return h;
 }
 
-__device__ __forceinline__ int64_t cu_at(const void* cu, bool is64, int64_t n) {
-    return is64 ? static_cast<const int64_t*>(cu)[n] : static_cast<const int32_t*>(cu)[n];
+// The sequences' offsets: the caller's, or (up to kScanCuMost sequences) a copy
+// in shared memory as 32-bit integers, where a search takes a tenth of the time.
+constexpr int kScanCuMost = 1023;
+struct Offsets {
+    const void* cu;
+    bool is64;
+    int seqs;
+    __device__ __forceinline__ int64_t at(int n) const {
+        return is64 ? static_cast<const int64_t*>(cu)[n] : static_cast<const int32_t*>(cu)[n];
+    }
+};
+// Every thread calls; a barrier has to follow before the offsets are used.
+__device__ __forceinline__ Offsets scan_offsets(const ScanParams& p, int* copy) {
+    if (p.seqs > kScanCuMost) return {p.cu, p.cu_is_int64, static_cast<int>(p.seqs)};
+    for (int i = threadIdx.x; i <= p.seqs; i += blockDim.x) {
+        const int64_t v = scan_cu(p, i);
+        copy[i] = v < -1 ? -1 : v > 0x7fffffffLL ? 0x7fffffff : static_cast<int>(v);  // bad ones stay bad
+    }
+    return {copy, false, static_cast<int>(p.seqs)};
 }
 
 // First sequence that ends behind packed token t (seqs if none), by the whole
-// warp.  Out of line, like everything that only tiles with a sequence's start
-// or end need: the loop over whole tiles has to fit the instruction cache.
-__device__ __noinline__ int seq_of_token(const void* cu, bool is64, int seqs, int64_t t) {
+// warp.  Out of line and, below, in loops that are not unrolled, like
+// everything that only pieces with a sequence's start or end need: it is cold
+// code whenever it runs, and what it costs is its size.
+__device__ __noinline__ int seq_of_token(Offsets o, int64_t t) {
     const int lane = threadIdx.x & 31;
-    int lo = 0, hi = seqs;
+    int lo = 0, hi = o.seqs;
     while (hi - lo > 32) {
         const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step - 1;
-        const int n = __popc(__ballot_sync(0xffffffffu, i < hi && cu_at(cu, is64, i + 1) <= t));
+        const int n = __popc(__ballot_sync(0xffffffffu, i < hi && o.at(i + 1) <= t));
         lo += n * step;
         hi = min(hi, lo + step);
     }
     const int i = lo + lane;
-    return lo + __popc(__ballot_sync(0xffffffffu, i < hi && cu_at(cu, is64, i + 1) <= t));
+    return lo + __popc(__ballot_sync(0xffffffffu, i < hi && o.at(i + 1) <= t));
 }
 
 // Which of W (up to 32) tokens from t on start a sequence, end one,
@@ -352,14 +370,14 @@ struct Spans {
 };
 template <int W>
 constexpr uint32_t kAllTokens = 0xffffffffu >> (32 - W);
-__device__ __noinline__ Spans find_spans(const void* cu, bool is64, int seqs, int64_t tokens, int64_t t, int width) {
+__device__ __noinline__ Spans find_spans(Offsets o, int64_t tokens, int64_t t, int width) {
     const int lane = threadIdx.x & 31;
     Spans s = {0, 0, 0, 0, 0};
     const int64_t stop = t + width < tokens ? t + width : tokens;
     if (t >= stop) return s;
-    for (int n = seq_of_token(cu, is64, seqs, t); n < seqs; n += 32) {
+    for (int n = seq_of_token(o, t); n < o.seqs; n += 32) {
         int64_t b = stop, e = stop;
-        if (n + lane < seqs) b = cu_at(cu, is64, n + lane), e = cu_at(cu, is64, n + lane + 1);
+        if (n + lane < o.seqs) b = o.at(n + lane), e = o.at(n + lane + 1);
         uint32_t st = 0, en = 0, cov = 0;
         int lo = 0, hi = 0;
         if (e > b && b < stop && e > t) {
@@ -380,54 +398,45 @@ __device__ __noinline__ Spans find_spans(const void* cu, bool is64, int seqs, in
 }
 // The same, with `s` of an earlier tile: tiles inside one sequence cost two comparisons.
 template <int W>
-__device__ __forceinline__ void token_spans(const ScanParams& p, int64_t t, Spans& s) {
+__device__ __forceinline__ void token_spans(const Offsets& o, int64_t tokens, int64_t t, Spans& s) {
     if (t > s.lo && t + W < s.hi) {
         s.start = s.end = 0;
         s.covered = kAllTokens<W>;
     } else {
-        s = find_spans(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), p.tokens, t, W);
+        s = find_spans(o, tokens, t, W);
     }
 }
 
-// Channels c and c + 1 of a state's row for packed token t's sequence (zeros without a state).
-__device__ __noinline__ F2 state_of_token(const void* cu, bool is64, int seqs, const float* state, int channels, int64_t t,
-                                          int c) {
-    const int n = seq_of_token(cu, is64, seqs, t);
-    if (state == nullptr || n >= seqs) return splat2(0.0f);
-    const float* row = state + static_cast<int64_t>(n) * channels;
-    return pack2(c < channels ? row[c] : 0.0f, c + 1 < channels ? row[c + 1] : 0.0f);
+// Channels c and c + 1 of the state rows of the sequences that packed token t
+// (in strip 0) and those `apart` tokens on (in the next strips) belong to;
+// `which` has bit i * apart set for the strips that want theirs, the others keep
+// `other`.  The whole warp calls; nothing here waits for the rows.
+template <int STRIPS>
+__device__ __forceinline__ F2 state_of_strips(const Offsets& o, const float* state, int channels, uint32_t which, int apart,
+                                              int64_t t, int c, int strip, F2 other) {
+#pragma unroll
+    for (int i = 0; i < STRIPS; ++i)
+        if (which >> (i * apart) & 1) {
+            const int n = seq_of_token(o, t + i * apart);
+            if (strip == i) {
+                float v0 = 0.0f, v1 = 0.0f;
+                const float* row = state + static_cast<int64_t>(n) * channels;
+                if (state != nullptr && n < o.seqs && c < channels) v0 = row[c];
+                if (state != nullptr && n < o.seqs && c + 1 < channels) v1 = row[c + 1];
+                other = pack2(v0, v1);
+            }
+        }
+    return other;
 }
-__device__ __noinline__ void store_state_of_token(const void* cu, bool is64, int seqs, float* state, int channels, int64_t t,
-                                                  int c, F2 h) {
-    const int n = seq_of_token(cu, is64, seqs, t);
-    if (state == nullptr || n >= seqs) return;
+// Lanes with `mine` store theirs for packed token t's sequence.  The whole warp calls.
+__device__ __forceinline__ void store_state_of_strip(const Offsets& o, float* state, int channels, int64_t t, int c, bool mine,
+                                                     F2 h) {
+    const int n = seq_of_token(o, t);
+    if (!mine || state == nullptr || n >= o.seqs) return;
     const float2 v = unpack2(h);
     float* row = state + static_cast<int64_t>(n) * channels;
     if (c < channels) row[c] = v.x;
     if (c + 1 < channels) row[c + 1] = v.y;
-}
-
-// The same for a warp whose strips hold token t and those `apart` tokens on;
-// `which` has bit i set for the strips (bit i * apart) that want it.  The whole warp calls.
-template <int STRIPS>
-__device__ __forceinline__ F2 state_of_strips(const ScanParams& p, const float* state, uint32_t which, int apart, int64_t t,
-                                              int c, int strip, F2 other) {
-#pragma unroll
-    for (int i = 0; i < STRIPS; ++i)
-        if (which >> (i * apart) & 1) {
-            const F2 v = state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), state, p.channels, t + i * apart, c);
-            if (strip == i) other = v;
-        }
-    return other;
-}
-template <int STRIPS>
-__device__ __forceinline__ void store_state_of_strips(const ScanParams& p, float* state, uint32_t which, int apart, int64_t t,
-                                                      int c, int strip, F2 h) {
-#pragma unroll
-    for (int i = 0; i < STRIPS; ++i)
-        if (which >> (i * apart) & 1)
-            store_state_of_token(p.cu, p.cu_is_int64, static_cast<int>(p.seqs), state, p.channels, t + i * apart,
-                                 strip == i ? c : p.channels, h);
 }
 
 // Two neighbouring elements as they are stored, read past the L1 cache.
@@ -494,6 +503,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ F2 s_in[2][32];  // the state at the tile's start
     __shared__ __align__(8) uint64_t s_bar[6];
+    __shared__ int s_cu[kScanCuMost + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int R = cluster_size(), rank = cluster_rank();
     const Strips<STRIPS> me;
@@ -512,11 +522,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
         }
         tc05::fence_mbar_init();
     }
-    cluster_arrive();
     const int tokens = static_cast<int>(p.tokens);
     const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
-    const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
-    const F2 rate = pack2(ok0 ? -kLog2e * expf(p.A_log[c]) : 0.0f, ok1 ? -kLog2e * expf(p.A_log[c + 1]) : 0.0f);
     const T* x0 = static_cast<const T*>(p.x) + c;
     const T* a0 = static_cast<const T*>(p.a) + c;
     const T* b0 = static_cast<const T*>(p.b) + c;
@@ -548,6 +555,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
 #pragma unroll
         for (int i = 0; i < kPiece; i += kBatch) fetch(0, i);
     }
+    const Offsets offsets = scan_offsets(p, s_cu);
+    cluster_arrive();
+    const F2 dtb = pack2(ok0 ? p.dt_bias[c] : 0.0f, ok1 ? p.dt_bias[c + 1] : 0.0f);
+    const F2 rate = pack2(ok0 ? -kLog2e * expf(p.A_log[c]) : 0.0f, ok1 ? -kLog2e * expf(p.A_log[c + 1]) : 0.0f);
     scan_empty_sequences(p, p.state, p.new_state, c0, c0 + me.kChannels, rank * blockDim.x + threadIdx.x, R * blockDim.x);
     cluster_wait();  // every CTA of the cluster runs and has its barriers
 
@@ -619,9 +630,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     for (int k = 0; k <= steps; ++k) {
         if (k < steps) {
             const int w0 = (k * R + rank) * kTile + warp * kSpan, buf = k & 1;
-            token_spans<kSpan>(p, w0, span);
+            token_spans<kSpan>(offsets, tokens, w0, span);
             const uint32_t special = span.start | (~span.covered & kAllTokens<kSpan>);
-            const uint32_t mine = special >> me.strip * kPiece, covered = span.covered >> me.strip * kPiece;
             float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
             F2 A = splat2(1.0f), H = splat2(0.0f);  // the map up to each token
 #pragma unroll
@@ -645,15 +655,28 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                         H = fma2(z[j], H, u[j]);
                         put(j);
                     }
-                } else {
+                } else {  // g and u for now
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
-                        const F2 before = state_of_strips<STRIPS>(p, p.state, span.start >> (i + j), kPiece, w0 + i + j, c,
-                                                                  me.strip, H);
-                        A = mine >> (i + j) & 1 ? splat2(-0.0f) : mul2(A, z[j]);
-                        H = covered >> (i + j) & 1 ? fma2(z[j], before, u[j]) : splat2(0.0f);
-                        put(j);
+                        const float2 vg = unpack2(z[j]), vu = unpack2(u[j]);
+                        m[(i + j) * 32] = make_float4(vg.x, vg.y, vu.x, vu.y);
                     }
+                }
+            }
+            if (special) {
+                const uint32_t fresh = special >> me.strip * kPiece, covered = span.covered >> me.strip * kPiece;
+                A = splat2(1.0f);
+                H = splat2(0.0f);
+#pragma unroll 1
+                for (int j = 0; j < kPiece; ++j) {
+                    const float4 gu = m[j * 32];
+                    const F2 g = pack2(gu.x, gu.y), u = pack2(gu.z, gu.w);
+                    const F2 before = state_of_strips<STRIPS>(offsets, p.state, p.channels, span.start >> j, kPiece, w0 + j, c,
+                                                              me.strip, H);
+                    A = fresh >> j & 1 ? splat2(-0.0f) : mul2(A, g);
+                    H = covered >> j & 1 ? fma2(g, before, u) : splat2(0.0f);
+                    const float2 va = unpack2(A), vh = unpack2(H);
+                    m[j * 32] = make_float4(va.x, va.y, vh.x, vh.y);
                 }
             }
             __syncwarp();
@@ -685,15 +708,19 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                 if (ok1) ck[1] = unpack2(v).y;
             }
             T* out = row_at<T>(out0, t0, p.out_stride);
-            if (ends == 0 && w0 + kSpan <= tokens && p.out_pairs && all_channels) {
+            if (w0 + kSpan <= tokens && p.out_pairs && all_channels) {
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) store_pair(row_at<T>(out, j, p.out_stride), h[j], true, true, true);
             } else {
 #pragma unroll
-                for (int j = 0; j < kPiece; ++j) {
+                for (int j = 0; j < kPiece; ++j)
                     if (t0 + j < tokens) store_pair(row_at<T>(out, j, p.out_stride), h[j], p.out_pairs, ok0, ok1);
-                    store_state_of_strips<STRIPS>(p, p.new_state, ends >> j, kPiece, w0 + j, c, me.strip, h[j]);
-                }
+            }
+#pragma unroll 1
+            for (uint32_t left = ends; left; left &= left - 1) {  // sequences that end here
+                const int t = __ffs(left) - 1;
+                store_state_of_strip(offsets, p.new_state, p.channels, w0 + t, c, me.strip == t / kPiece,
+                                     apply_map_select(m[t % kPiece * 32], in));
             }
         }
         ends = span.end;
@@ -763,6 +790,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float4 s_ends[2][32];  // the state before the tile, the gradient behind it
     __shared__ __align__(8) uint64_t s_bar[7];
+    __shared__ int s_cu[kScanCuMost + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int R = cluster_size(), rank = cluster_rank();
     GradTile<T> vals(smem, lane);
@@ -785,6 +813,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
         tc05::mbar_expect_tx(summed, R * 512);
         tc05::fence_mbar_init();
     }
+    const Offsets offsets = scan_offsets(p, s_cu);
     cluster_arrive();
     const int tokens = static_cast<int>(p.tokens);
     const int tiles = (tokens + kTile - 1) / kTile, steps = (tiles + R - 1) / R;
@@ -909,7 +938,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
             if (k < steps) {
                 const int w0 = tile_start(k) + warp * kSpan, buf = k & 1;
                 if (w0 >= 0)
-                    token_spans<kSpan>(p, w0, span);
+                    token_spans<kSpan>(offsets, tokens, w0, span);
                 else
                     span = {0, 0, 0, 0, 0};
                 const bool special = (span.start | span.end | (~span.covered & kAllTokens<kSpan>)) != 0;
@@ -940,19 +969,26 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                     for (int j = kPiece - 1; j >= 0; --j) E = mul2(g[j], add2(raw_to_f2<T>(dy[j]), E));
                 } else {
                     const int at = me.strip * kPiece;
-#pragma unroll
+                    F2 t, beta, sig, xs, dys;
+#pragma unroll 1
                     for (int j = 0; j < kPiece; ++j) {
+                        vals.get(buf * kRows + warp * kPiece + j, t, beta, sig, xs, dys);
                         const bool covered = span.covered >> (at + j) & 1, start = span.start >> (at + j) & 1;
-                        H = state_of_strips<STRIPS>(p, p.state, span.start >> j, kPiece, w0 + j, c, me.strip, H);
-                        A = start || !covered ? splat2(-0.0f) : mul2(A, g[j]);
-                        H = covered ? fma2(g[j], H, z[j]) : splat2(0.0f);
+                        F2 g1[1] = {t};
+                        exp2_decays(g1);
+                        H = state_of_strips<STRIPS>(offsets, p.state, p.channels, span.start >> j, kPiece, w0 + j, c, me.strip, H);
+                        A = start || !covered ? splat2(-0.0f) : mul2(A, g1[0]);
+                        H = covered ? fma2(g1[0], H, mul2(beta, xs)) : splat2(0.0f);
                     }
-#pragma unroll
+#pragma unroll 1
                     for (int j = kPiece - 1; j >= 0; --j) {
+                        vals.get(buf * kRows + warp * kPiece + j, t, beta, sig, xs, dys);
                         const bool covered = span.covered >> (at + j) & 1, end = span.end >> (at + j) & 1;
-                        E = state_of_strips<STRIPS>(p, d.d_new_state, span.end >> j, kPiece, w0 + j, c, me.strip, E);
-                        B = end || !covered ? splat2(-0.0f) : mul2(B, g[j]);
-                        E = covered ? mul2(g[j], add2(raw_to_f2<T>(dy[j]), E)) : splat2(0.0f);
+                        F2 g1[1] = {t};
+                        exp2_decays(g1);
+                        E = state_of_strips<STRIPS>(offsets, d.d_new_state, p.channels, span.end >> j, kPiece, w0 + j, c, me.strip, E);
+                        B = end || !covered ? splat2(-0.0f) : mul2(B, g1[0]);
+                        E = covered ? mul2(g1[0], add2(dys, E)) : splat2(0.0f);
                     }
                 }
                 fetch(k + 1);
@@ -973,55 +1009,79 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(cons
                     h = apply_map_select(hm, tile_h);
                     e = apply_map_select(em, tile_e);
                 }
-                // whole pieces inside one sequence go without a branch
-                auto finish = [&](auto inside) {
-                    constexpr bool kInside = decltype(inside)::value;
-                    const uint32_t covered = done.covered >> me.strip * kPiece;
+                T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
+                T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
+                T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
+                const int row0 = buf * kRows + warp * kPiece;
+                // one token's gradients from the state before it; e moves on to the token before
+                const auto token = [&](F2 g, F2 before, F2 t, F2 beta, F2 sig, F2 xs, F2 dys, F2& vx, F2& va, F2& vb) {
+                    const F2 G = add2(dys, e);
+                    e = mul2(g, G);
+                    const F2 dl = mul2(e, before);
+                    vx = mul2(G, beta);
+                    va = mul2(mul2(dl, minus_decay), sig);
+                    vb = mul2(mul2(vx, xs), fma2(beta, splat2(-1.0f), splat2(1.0f)));
+                    return dl;
+                };
+                if ((done.start | done.end) == 0 && done.covered == kAllTokens<kSpan> && all_channels && d.grad_pairs) {
                     F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        vals.get(buf * kRows + warp * kPiece + j, t[j], beta[j], sig[j], xs[j], dys[j]);
+                        vals.get(row0 + j, t[j], beta[j], sig[j], xs[j], dys[j]);
                         g[j] = t[j];
                     }
                     exp2_decays(g);
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        if (!kInside) h = state_of_strips<STRIPS>(p, p.state, done.start >> j, kPiece, w0 + j, c, me.strip, h);
                         before[j] = h;
                         h = fma2(g[j], h, mul2(beta[j], xs[j]));
-                        if (!kInside && !(covered >> j & 1)) h = splat2(0.0f);
                     }
-                    T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
-                    T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
-                    T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) {
-                        if (!kInside)
-                            e = state_of_strips<STRIPS>(p, d.d_new_state, done.end >> j, kPiece, w0 + j, c, me.strip, e);
-                        const F2 G = add2(dys[j], e);
-                        e = mul2(g[j], G);
-                        const F2 dl = mul2(e, before[j]);
-                        F2 vx = mul2(G, beta[j]), va = mul2(mul2(dl, minus_decay), sig[j]);
-                        F2 vb = mul2(mul2(vx, xs[j]), fma2(beta[j], splat2(-1.0f), splat2(1.0f)));
-                        if (!kInside && !(covered >> j & 1)) {
-                            vx = va = vb = e = splat2(0.0f);
-                        } else {
-                            sum_A = fma2(dl, t[j], sum_A);
+                        F2 vx, va, vb;
+                        const F2 dl = token(g[j], before[j], t[j], beta[j], sig[j], xs[j], dys[j], vx, va, vb);
+                        sum_A = fma2(dl, t[j], sum_A);
+                        sum_dt = add2(sum_dt, va);
+                        store_pair(row_at<T>(dx, j, d.dx_stride), vx, true, true, true);
+                        store_pair(row_at<T>(da, j, d.da_stride), va, true, true, true);
+                        store_pair(row_at<T>(db, j, d.db_stride), vb, true, true, true);
+                    }
+                } else {
+                    const int at = me.strip * kPiece;
+                    F2 before[kPiece], t, beta, sig, xs, dys;
+#pragma unroll 1
+                    for (int j = 0; j < kPiece; ++j) {
+                        vals.get(row0 + j, t, beta, sig, xs, dys);
+                        F2 g[1] = {t};
+                        exp2_decays(g);
+                        h = state_of_strips<STRIPS>(offsets, p.state, p.channels, done.start >> j, kPiece, w0 + j, c, me.strip, h);
+                        before[j] = h;
+                        h = done.covered >> (at + j) & 1 ? fma2(g[0], h, mul2(beta, xs)) : splat2(0.0f);
+                    }
+#pragma unroll 1
+                    for (int j = kPiece - 1; j >= 0; --j) {
+                        vals.get(row0 + j, t, beta, sig, xs, dys);
+                        F2 g[1] = {t}, vx, va, vb;
+                        exp2_decays(g);
+                        e = state_of_strips<STRIPS>(offsets, d.d_new_state, p.channels, done.end >> j, kPiece, w0 + j, c, me.strip, e);
+                        const F2 dl = token(g[0], before[j], t, beta, sig, xs, dys, vx, va, vb);
+                        if (done.covered >> (at + j) & 1) {
+                            sum_A = fma2(dl, t, sum_A);
                             sum_dt = add2(sum_dt, va);
+                        } else {
+                            vx = va = vb = e = splat2(0.0f);
                         }
-                        if (!kInside)
-                            store_state_of_strips<STRIPS>(p, d.d_state, done.start >> j, kPiece, w0 + j, c, me.strip, e);
-                        if (kInside || t0 + j < tokens) {
-                            store_pair(row_at<T>(dx, j, d.dx_stride), vx, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
-                            store_pair(row_at<T>(da, j, d.da_stride), va, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
-                            store_pair(row_at<T>(db, j, d.db_stride), vb, kInside || d.grad_pairs, kInside || ok0, kInside || ok1);
+#pragma unroll
+                        for (int i = 0; i < STRIPS; ++i)
+                            if (done.start >> (i * kPiece + j) & 1)
+                                store_state_of_strip(offsets, d.d_state, p.channels, w0 + i * kPiece + j, c, me.strip == i, e);
+                        if (t0 + j < tokens) {
+                            store_pair(row_at<T>(dx, j, d.dx_stride), vx, d.grad_pairs, ok0, ok1);
+                            store_pair(row_at<T>(da, j, d.da_stride), va, d.grad_pairs, ok0, ok1);
+                            store_pair(row_at<T>(db, j, d.db_stride), vb, d.grad_pairs, ok0, ok1);
                         }
                     }
-                };
-                if ((done.start | done.end) == 0 && done.covered == kAllTokens<kSpan> && all_channels && d.grad_pairs)
-                    finish(std::true_type{});
-                else
-                    finish(std::false_type{});
+                }
             }
             done = {span.start, span.end, span.covered};
         }
