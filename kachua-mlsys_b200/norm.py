@@ -15,7 +15,6 @@ asynchronously; errors in arguments raise ``ValueError`` before a launch.
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -23,6 +22,8 @@ import torch
 from . import _capi
 from .recurrence import DTYPES, _call, _dense, _fault, _like, _need, _ptr, _rows
 
+_pack_add, _pack_gated, _pack_grad = (
+    _capi.packer(t) for t in (_capi.GdnAddNormArgs, _capi.GdnGatedNormArgs, _capi.GdnNormGradArgs))
 QUANT = {None: _capi.QUANT_NONE, "row": _capi.QUANT_ROW, "group": _capi.QUANT_GROUP}
 GROUP = 128
 MAX_WIDTH = 32768
@@ -91,9 +92,9 @@ def launch_add_norm(x, residual, weight, eps=1e-6, output=None, new_residual=Non
             _dense(scale, "scale", torch.float32, scale_shape, dev)
     else:
         _need(scale is None, "scale needs quant")
-    args = _capi.GdnAddNormArgs(_ptr(x), _ptr(residual), x_stride, res_stride, _ptr(weight), wdt, DTYPES[x.dtype],
+    args = _pack_add(_ptr(x), _ptr(residual), x_stride, res_stride, _ptr(weight), wdt, DTYPES[x.dtype],
                                 QUANT[quant], eps, rows, width, _ptr(output), _ptr(new_residual), _ptr(scale))
-    _call(_capi.load().gdn_add_norm_launch, "gdn_add_norm_launch", dev, ctypes.byref(args))
+    _call(_capi.load().gdn_add_norm_launch, "gdn_add_norm_launch", dev, args)
     summed = x if residual is None else new_residual
     return (output, summed, scale) if quant else (output, summed)
 
@@ -119,10 +120,9 @@ def launch_add_norm_backward(d_output, new_residual, weight, eps=1e-6, d_new_res
     lib = _capi.load()
     need = int(lib.gdn_add_norm_backward_workspace_size(rows, width))
     workspace = weight.new_empty(need, dtype=torch.uint8)
-    args = _capi.GdnAddNormArgs(_ptr(new_residual), None, r_stride, 0, _ptr(weight), wdt, DTYPES[dt], 0, eps, rows, width,
-                                None, None, None)
-    g = _capi.GdnNormGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_residual), dr_stride, _ptr(dx), None, _ptr(d_weight))
-    _call(lib.gdn_add_norm_backward_launch, "gdn_add_norm_backward_launch", dev, ctypes.byref(args), ctypes.byref(g),
+    args = _pack_add(_ptr(new_residual), 0, r_stride, 0, _ptr(weight), wdt, DTYPES[dt], 0, eps, rows, width, 0, 0, 0)
+    g = _pack_grad(_ptr(d_output), dy_stride, _ptr(d_new_residual), dr_stride, _ptr(dx), 0, _ptr(d_weight))
+    _call(lib.gdn_add_norm_backward_launch, "gdn_add_norm_backward_launch", dev, args, g,
           _ptr(workspace), need)
     return dx, d_weight
 
@@ -189,12 +189,12 @@ def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):
             _dense(scale, "scale", torch.float32, shape[:-1], dev)
     else:
         _need(scale is None, "scale needs quant")
-    args = _capi.GdnGatedNormArgs(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype],
+    args = _pack_gated(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype],
                                   _capi.QUANT_GROUP if quant else _capi.QUANT_NONE, eps, tokens, heads, dim,
                                   _ptr(output), _ptr(scale))
 
     def launch():
-        _call(_capi.load().gdn_gated_norm_launch, "gdn_gated_norm_launch", dev, ctypes.byref(args))
+        _call(_capi.load().gdn_gated_norm_launch, "gdn_gated_norm_launch", dev, args)
 
     return launch, output, scale
 
@@ -236,11 +236,10 @@ def launch_gated_norm_backward(d_output, x, z, weight, eps=1e-6, dx=None, dz=Non
     lib = _capi.load()
     need = int(lib.gdn_gated_norm_backward_workspace_size(tokens, heads, dim))
     workspace = weight.new_empty(need, dtype=torch.uint8)
-    args = _capi.GdnGatedNormArgs(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype], 0, eps, tokens, heads, dim,
-                                  None, None)
-    g = _capi.GdnNormGradArgs(_ptr(d_output), dys, None, 0, _ptr(dx), _ptr(dz), _ptr(d_weight))
-    _call(lib.gdn_gated_norm_backward_launch, "gdn_gated_norm_backward_launch", dev, ctypes.byref(args),
-          ctypes.byref(g), _ptr(workspace), need)
+    args = _pack_gated(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype], 0, eps, tokens, heads, dim, 0, 0)
+    g = _pack_grad(_ptr(d_output), dys, 0, 0, _ptr(dx), _ptr(dz), _ptr(d_weight))
+    _call(lib.gdn_gated_norm_backward_launch, "gdn_gated_norm_backward_launch", dev, args,
+          g, _ptr(workspace), need)
     return dx, dz, d_weight
 
 

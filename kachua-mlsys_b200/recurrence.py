@@ -21,12 +21,11 @@ anything launches; bad ``cu_seqlens`` values are reported through
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _capi
 
+_pack_scan, _pack_scan_grad = _capi.packer(_capi.GdnScanArgs), _capi.packer(_capi.GdnScanGradArgs)
 DTYPES = {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16, torch.float32: _capi.DTYPE_F32}
 
 
@@ -59,6 +58,14 @@ def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
     return stride
 
 
+def _rows_like(t, name: str, x, stride: int) -> int:
+    """``_rows`` of a tensor that mostly has the layout of ``x`` (checked, row stride ``stride``)."""
+    if (isinstance(t, torch.Tensor) and t.dtype == x.dtype and t.shape == x.shape and t.device == x.device
+            and t.stride() == x.stride()):
+        return stride
+    return _rows(t, name, x.dtype, *x.shape, x.device)
+
+
 def _dense(t, name: str, dtype, shape, device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
         _fault(t, name, dtype, shape, device)
@@ -68,6 +75,7 @@ def _dense(t, name: str, dtype, shape, device) -> None:
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _like(x, dtype=None) -> torch.Tensor:
@@ -78,7 +86,7 @@ def _like(x, dtype=None) -> torch.Tensor:
 def _call(fn, what: str, device, *args) -> None:
     """``fn(*args, current stream of device)`` with that device current."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -87,8 +95,8 @@ def _call(fn, what: str, device, *args) -> None:
         _capi.check(rc, what)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
@@ -103,7 +111,8 @@ def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
         raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
     if C < 1:
         raise ValueError("x must have at least one channel")
-    strides = _rows(x, "x", dtype, T, C, dev), _rows(a, "a", dtype, T, C, dev), _rows(b, "b", dtype, T, C, dev)
+    stride = _rows(x, "x", dtype, T, C, dev)
+    strides = (stride, _rows_like(a, "a", x, stride), _rows_like(b, "b", x, stride))
     _dense(A_log, "A_log", torch.float32, (C,), dev)
     _dense(dt_bias, "dt_bias", torch.float32, (C,), dev)
     return T, C, strides
@@ -160,13 +169,12 @@ def empty_checkpoints(x) -> torch.Tensor:
 
 
 def _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, seqs, output, new_state, checkpoints):
-    cu64 = cu_seqlens is not None and cu_seqlens.dtype == torch.int64
-    rows = x.shape[0]
-    return _capi.GdnScanArgs(
-        _ptr(x), _ptr(a), _ptr(b), *strides, _ptr(A_log), _ptr(dt_bias), _ptr(state), _ptr(cu_seqlens),
-        _capi.GDN_SEQLENS_INT64 if cu64 else _capi.GDN_SEQLENS_INT32, DTYPES[x.dtype], rows, seqs, x.shape[1],
-        _ptr(output), 0 if output is None else output.stride(0) if rows > 1 else x.shape[1], _ptr(new_state),
-        _ptr(checkpoints))
+    rows, C = x.shape
+    return _pack_scan(
+        x.data_ptr(), a.data_ptr(), b.data_ptr(), *strides, A_log.data_ptr(), dt_bias.data_ptr(), _ptr(state),
+        cu_seqlens.data_ptr(), _capi.GDN_SEQLENS_INT64 if cu_seqlens.dtype == torch.int64 else _capi.GDN_SEQLENS_INT32,
+        DTYPES[x.dtype], rows, seqs, C, _ptr(output), 0 if output is None else output.stride(0) if rows > 1 else C,
+        _ptr(new_state), _ptr(checkpoints))
 
 
 def launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None, output=None, new_state=None, checkpoints=None,
@@ -200,7 +208,7 @@ def launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None, output=None, ne
     if checkpoints is not None:
         _dense(checkpoints, "checkpoints", torch.float32, (_checkpoint_rows(T), C), x.device)
     args = _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, N, output, new_state, checkpoints)
-    _call(_capi.load().gdn_scan_launch, "gdn_scan_launch", x.device, ctypes.byref(args))
+    _call(_capi.load().gdn_scan_launch, "gdn_scan_launch", x.device, args)
     return output, new_state
 
 
@@ -240,9 +248,9 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
     dA_log, d_dt_bias = _like(A_log), _like(dt_bias)
     d_state = None if state is None else _like(state)
     args = _args(x, A_log, a, dt_bias, b, cu_seqlens, state, strides, N, None, None, checkpoints)
-    g = _capi.GdnScanGradArgs(_ptr(d_output), dy_stride, _ptr(d_new_state), *(_ptr(t) for t in grads), *grad_strides,
+    g = _pack_scan_grad(_ptr(d_output), dy_stride, _ptr(d_new_state), *(_ptr(t) for t in grads), *grad_strides,
                               _ptr(dA_log), _ptr(d_dt_bias), _ptr(d_state))
-    _call(_capi.load().gdn_scan_backward_launch, "gdn_scan_backward_launch", dev, ctypes.byref(args), ctypes.byref(g))
+    _call(_capi.load().gdn_scan_backward_launch, "gdn_scan_backward_launch", dev, args, g)
     return (*grads, dA_log, d_dt_bias, d_state)
 
 
@@ -278,10 +286,9 @@ def launch_step(x, A_log, a, dt_bias, b, state, output=None, new_state=None):
         new_state = _like(state)
     elif new_state is not state:
         _dense(new_state, "new_state", torch.float32, (B, C), dev)
-    args = _capi.GdnScanArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), *strides, A_log.data_ptr(), dt_bias.data_ptr(),
-                             state.data_ptr(), None, 0, DTYPES[x.dtype], rows, B, C, output.data_ptr(), C,
-                             new_state.data_ptr(), None)
-    _call(_capi.load().gdn_scan_step_launch, "gdn_scan_step_launch", dev, ctypes.byref(args), tokens)
+    args = _pack_scan(x.data_ptr(), a.data_ptr(), b.data_ptr(), *strides, A_log.data_ptr(), dt_bias.data_ptr(),
+                      state.data_ptr(), 0, 0, DTYPES[x.dtype], rows, B, C, output.data_ptr(), C, new_state.data_ptr(), 0)
+    _call(_capi.load().gdn_scan_step_launch, "gdn_scan_step_launch", dev, args, tokens)
     return output, new_state
 
 
