@@ -202,10 +202,13 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t a, uint32_t bar, uint32_t
                  "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(rb)
                  : "memory");
 }
-// The scans' CTA: 15 map warps and a chain warp (four warps to a scheduler,
-// so 128 registers a thread).  A lane owns two channels; a warp is one strip of
-// 64 channels, or two strips of 32 on different tokens.
-constexpr int kScanWarps = 15, kScanThreads = 32 * (kScanWarps + 1);
+
+// The scans' CTAs, one to an SM: map warps and a chain warp, the same number to
+// each of the four schedulers, so 96 registers a thread forward (16 warps of
+// 128: 3 % slower) and 128 backward.  A lane owns two channels; a warp is one
+// strip of 64 channels, or two strips of 32 on different tokens.
+constexpr int kScanWarps = 19, kScanThreads = 32 * (kScanWarps + 1);
+constexpr int kGradWarps = 15, kGradThreads = 32 * (kGradWarps + 1);
 template <int STRIPS>
 struct Strips {
     static constexpr int kLanes = 32 / STRIPS, kChannels = 2 * kLanes;
@@ -219,7 +222,7 @@ struct Strips {
 // registers (forward) and what its gates gave in shared memory (backward).
 template <typename T>
 constexpr int kScanPiece = sizeof(T) == 4 ? 4 : 8;
-constexpr int kGradPiece = 4, kGradRows = kScanWarps * kGradPiece;
+constexpr int kGradPiece = 4, kGradRows = kGradWarps * kGradPiece;
 constexpr int kScanMaxCluster = 16;
 
 // The carry into every kScanCkpt-th packed token is kept for the backward
@@ -497,9 +500,9 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 // So the gates' arithmetic, which is what the kernel is made of, has a whole
 // tile's time to hide the cluster's exchange behind.
 // Bound by instruction issue: 80 warp instructions per token and pair of
-// channels, 60 % of the slots with four warps to a scheduler.  Measured (bf16):
-// 1 x 16384 x 4096 150 us, 3.6 TB/s of inputs and outputs, 55 % of the copy
-// rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 178 us.  A thread per
+// channels, 64 % of the slots with five warps to a scheduler.  Measured (bf16):
+// 1 x 16384 x 4096 143 us, 3.8 TB/s of inputs and outputs, 57 % of the copy
+// rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 174 us.  A thread per
 // sequence and channel took 42 ms for the second.
 template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanParams p) {
@@ -627,9 +630,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
         return;
     }
 
-    // the piece's token whose state is the next checkpoint, if it has one (tiles are whole checkpoints)
-    const int kept = kScanCkpt - 1 - (warp * kSpan + me.strip * kPiece) % kScanCkpt;
-    static_assert(kTile % kScanCkpt == 0, "whole checkpoints");
     Spans span = {0, 0, 0, 0, 0};
     uint32_t ends = 0;  // of the tile before
     for (int k = 0; k <= steps; ++k) {
@@ -703,6 +703,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
             }
+            // the piece's token whose state is the next checkpoint, if it has one
+            const int kept = kScanCkpt - 1 - t0 % kScanCkpt;
             if (p.ckpt && kept < kPiece && t0 + kept + 1 < tokens) {
                 F2 v = h[0];
 #pragma unroll
@@ -792,8 +794,8 @@ struct GradTile<float> {  // 40 bytes
 // forward pass; measured (bf16): 1 x 16384 x 4096 270 us, 3.5 TB/s;
 // 8 x 4096 x 1024 177 us.
 template <typename T, int STRIPS>
-__global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
-    constexpr int W = kScanWarps, kPiece = kGradPiece, kRows = kGradRows, kTile = STRIPS * kRows, kSpan = STRIPS * kPiece;
+__global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
+    constexpr int W = kGradWarps, kPiece = kGradPiece, kRows = kGradRows, kTile = STRIPS * kRows, kSpan = STRIPS * kPiece;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float4 s_ends[2][32];  // the state before the tile, the gradient behind it
     __shared__ __align__(8) uint64_t s_bar[7];
@@ -1206,10 +1208,10 @@ __global__ void __launch_bounds__(128) gdn_scan_step_kernel(const ScanParams p, 
 }
 
 // `kernel` with gridDim = (cluster, groups of channels); `attr` outlives the launch.
-static cudaLaunchConfig_t scan_config(int cluster, unsigned groups, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
+static cudaLaunchConfig_t scan_config(int cluster, unsigned groups, int threads, size_t smem, cudaStream_t s, cudaLaunchAttribute* attr) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster, groups);
-    cfg.blockDim = dim3(kScanThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     attr->id = cudaLaunchAttributeClusterDimension;
@@ -1224,12 +1226,12 @@ static cudaLaunchConfig_t scan_config(int cluster, unsigned groups, size_t smem,
 // device and size; the kernel's attributes are set with it, for `most` bytes of
 // shared memory.
 template <typename Kernel>
-static int active_clusters(Kernel kernel, int n, size_t smem, size_t most, int (*cache)[kScanMaxCluster + 1]) {
+static int active_clusters(Kernel kernel, int n, int threads, size_t smem, size_t most, int (*cache)[kScanMaxCluster + 1]) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
     if (cache[dev][n] == 0) {
         cudaLaunchAttribute attr[1];
-        const cudaLaunchConfig_t cfg = scan_config(n, 1, smem, nullptr, attr);
+        const cudaLaunchConfig_t cfg = scan_config(n, 1, threads, smem, nullptr, attr);
         int got = 0;
         const bool ok =
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) == cudaSuccess &&
@@ -1269,20 +1271,20 @@ static ClusterShape scan_cluster(int64_t tiles, int64_t groups, Active active) {
 // 128, 89 us).
 template <typename Smem, typename... Params, typename... Args>
 static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Params...), int (*cache)[64][kScanMaxCluster + 1],
-                                        int64_t tokens, int rows, int channels, Smem smem, cudaStream_t s, Args... args) {
+                                        int64_t tokens, int rows, int threads, int channels, Smem smem, cudaStream_t s, Args... args) {
     const int64_t groups[2] = {(channels + 63) / 64, (channels + 31) / 32};
     void (*const kernels[2])(Params...) = {one, two};
     ClusterShape shape[2];
     for (int i = 0; i < 2; ++i) {
         const int tile = rows * (i + 1);
         shape[i] = scan_cluster((tokens + tile - 1) / tile, groups[i], [&](int n) {
-            return active_clusters(kernels[i], n, smem(n), smem(kScanMaxCluster), cache[i]);
+            return active_clusters(kernels[i], n, threads, smem(n), smem(kScanMaxCluster), cache[i]);
         });
     }
     const int i = shape[1].steps < shape[0].steps ? 1 : 0;
     if (shape[i].size == 0) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = scan_config(shape[i].size, static_cast<unsigned>(groups[i]), smem(shape[i].size), s, attr);
+    const cudaLaunchConfig_t cfg = scan_config(shape[i].size, static_cast<unsigned>(groups[i]), threads, smem(shape[i].size), s, attr);
     return cudaLaunchKernelEx(&cfg, kernels[i], static_cast<Params>(args)...);
 }
 
@@ -1291,15 +1293,15 @@ static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
     constexpr int kRows = kScanWarps * kScanPiece<T>;
     static int cache[2][64][kScanMaxCluster + 1];
     const auto smem = [](int r) { return (2 * kRows + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
-    return launch_scan_clusters(gdn_scan_kernel<T, 1>, gdn_scan_kernel<T, 2>, cache, p.tokens, kRows, p.channels, smem, s, p);
+    return launch_scan_clusters(gdn_scan_kernel<T, 1>, gdn_scan_kernel<T, 2>, cache, p.tokens, kRows, kScanThreads, p.channels, smem, s, p);
 }
 
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
     static int cache[2][64][kScanMaxCluster + 1];
-    const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kScanWarps + 3 * r) * 32 * sizeof(float4); };
+    const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kGradWarps + 3 * r) * 32 * sizeof(float4); };
     return launch_scan_clusters(gdn_scan_backward_kernel<T, 1>, gdn_scan_backward_kernel<T, 2>, cache, p.tokens, kGradRows,
-                                p.channels, smem, s, p, d);
+                                kGradThreads, p.channels, smem, s, p, d);
 }
 
 template <typename T>
