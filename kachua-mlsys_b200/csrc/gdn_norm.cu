@@ -18,6 +18,7 @@
 // 32 heads of 128 gated 128 us (6.3), backward 223 us (6.0).
 #include <cuda_fp8.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace gdn {
@@ -34,7 +35,7 @@ struct NormParams {
     int64_t x_stride, residual_stride;
     const void* weight;
     bool weight_f32;
-    bool vec;  // every row starts on a 16-byte boundary and is whole vectors
+    int mode;   // kApart, kVec or kShift
     int quant;  // 0 none, 1 a scale per row, 2 a scale per 128 channels
     int64_t rows;
     int width;
@@ -81,37 +82,57 @@ template <typename T>
 struct Raw8 {
     uint4 v[sizeof(T) / 2];
 };
-// Which 8 elements of a row are a thread's j-th: neighbours where the row is
-// whole vectors on 16-byte boundaries (VEC), elsewhere `step` apart, so that a
-// warp's accesses touch neighbouring elements all the same.
+// How a row's elements are dealt to the threads, 8 at a time.
+constexpr int kApart = 0;  // any alignment: blockDim.x apart, so that a warp's accesses touch neighbours
+constexpr int kVec = 1;    // rows are whole 8-element vectors on 16-byte boundaries
+// Rows of 16 elements or more whose width is not a multiple of 8, contiguous or
+// apart by a multiple of 8 elements more: the vectors of the whole tensor, of
+// which a row's first and last are only partly its own (16384 x 5333 bf16: 145
+// us forward, 181 backward; dealt apart 300 and 385).
+constexpr int kShift = 2;
 struct Cols {
     int first, step, width;
-    __device__ __forceinline__ bool in(int i) const { return first + i * step < width; }
+    __device__ __forceinline__ bool in(int i) const {
+        return static_cast<unsigned>(first + i * step) < static_cast<unsigned>(width);
+    }
+    __device__ __forceinline__ bool whole() const { return first >= 0 && first + 8 <= width; }  // step 1
+    __device__ __forceinline__ bool any() const { return first < width && first + 7 * step >= 0; }
 };
-template <bool VEC>
-__device__ __forceinline__ Cols row_cols(int j, int width, bool groups) {
+// A thread's j-th; `m` elements lie between the boundary and the row's start (kShift).
+template <int MODE>
+__device__ __forceinline__ Cols row_cols(int j, int width, bool groups, int m) {
     const int t = threadIdx.x, n = blockDim.x;
-    return VEC || groups ? Cols{(t + j * n) * 8, 1, width} : Cols{j * 8 * n + t, n, width};
+    return MODE == kShift           ? Cols{(t + j * n) * 8 - m, 1, width}
+           : MODE == kVec || groups ? Cols{(t + j * n) * 8, 1, width}
+                                    : Cols{j * 8 * n + t, n, width};
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load8(const T* row, Cols c) {
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_vec8(const T* p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
+}
+// A shifted row's first and last vectors come with their neighbours' elements,
+// for own8 to drop, but for the end of the tensor's `last` row.
+template <typename T, int MODE>
+__device__ __forceinline__ Raw8<T> load8(const T* row, Cols c, bool last = true) {
     Raw8<T> r = {};
-    if constexpr (VEC) {
-        if (c.in(0)) {
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(row + c.first)[i];
-        }
-    } else {
-        // all loads first, from the row's start where the column is outside:
-        // `row` is a row of the tensor even where none of the columns counts
-        T e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = row[c.in(i) ? c.first + i * c.step : 0];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = c.in(i) ? e[i] : from_f32<T>(0.0f);
-        memcpy(&r, e, sizeof(r));
+    if constexpr (MODE == kVec) {
+        if (c.in(0)) r = load_vec8(row + c.first);
+        return r;
     }
+    if (MODE == kShift && !c.any()) return r;
+    if (MODE == kShift && (!last || c.first + 8 <= c.width)) return load_vec8(row + c.first);
+    // all loads first, from the row's start where the column is outside:
+    // `row` is a row of the tensor even where none of the columns counts
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = row[c.in(i) ? c.first + i * c.step : 0];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = c.in(i) ? e[i] : from_f32<T>(0.0f);
+    memcpy(&r, e, sizeof(r));
     return r;
 }
 template <typename T>
@@ -120,7 +141,18 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& r, F2 (&f)[4]) {
     for (int i = 0; i < 4; ++i) f[i] = load_pair<T>(reinterpret_cast<const T*>(&r) + 2 * i);
 }
 
-template <typename T, bool VEC>
+template <int MODE>
+__device__ __forceinline__ void own8(F2 (&f)[4], Cols c) {
+    if (MODE == kShift && !c.whole()) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = unpack2(f[i]);
+            f[i] = pack2(c.in(2 * i) ? v.x : 0.0f, c.in(2 * i + 1) ? v.y : 0.0f);
+        }
+    }
+}
+
+template <typename T, int MODE>
 __device__ __forceinline__ void store8(T* row, Cols c, const F2 (&f)[4]) {
     Raw8<T> r;
     T* e = reinterpret_cast<T*>(&r);
@@ -130,28 +162,26 @@ __device__ __forceinline__ void store8(T* row, Cols c, const F2 (&f)[4]) {
         e[2 * i] = from_f32<T>(v.x);
         e[2 * i + 1] = from_f32<T>(v.y);
     }
-    if constexpr (VEC) {
-        if (c.in(0)) {
+    if (MODE == kVec ? c.in(0) : MODE == kShift && c.whole()) {
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + c.first)[i] = r.v[i];
-        }
-    } else {
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + c.first)[i] = r.v[i];
+    } else if (MODE != kVec) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (c.in(i)) row[c.first + i * c.step] = e[i];
     }
 }
 
-template <bool VEC>
+template <int MODE>
 __device__ __forceinline__ void store8_e4m3(uint8_t* row, Cols c, const F2 (&f)[4], float inv) {
     uint2 u;
     uint16_t* h = reinterpret_cast<uint16_t*>(&u);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         h[i] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[i], splat2(inv))), __NV_SATFINITE, __NV_E4M3);
-    if constexpr (VEC) {
-        if (c.in(0)) *reinterpret_cast<uint2*>(row + c.first) = u;
-    } else {
+    if (MODE == kVec ? c.in(0) : MODE == kShift && c.whole()) {
+        *reinterpret_cast<uint2*>(row + c.first) = u;
+    } else if (MODE != kVec) {
         const uint8_t* e = reinterpret_cast<const uint8_t*>(&u);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -159,12 +189,42 @@ __device__ __forceinline__ void store8_e4m3(uint8_t* row, Cols c, const F2 (&f)[
     }
 }
 
-template <typename T, bool VEC>
+// Weights of a shifted row are off the boundary: an inner vector's come from two
+// neighbouring vectors of w, moved by the row's m (element by element, 16384 x
+// 5333 takes 10 us longer forward).
+template <typename W>
+__device__ __forceinline__ bool load_shifted8(const W* w, Cols c, F2 (&f)[4]) {
+    const int m = -c.first & 7, at = c.first + m;  // elements at - m .. at - m + 7
+    if (at < 8 || at + 8 > c.width || (reinterpret_cast<uintptr_t>(w) & 15) != 0) return false;
+    F2 lo[4], hi[4];
+    unpack8(load_vec8(w + at - 8), lo);
+    unpack8(load_vec8(w + at), hi);
+    float e[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = unpack2(lo[i]), b = unpack2(hi[i]);
+        e[2 * i] = a.x, e[2 * i + 1] = a.y;
+        e[8 + 2 * i] = b.x, e[9 + 2 * i] = b.y;
+    }
+    const int by = 8 - m;  // the result is e[by .. by + 7]
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) {
+#pragma unroll
+        for (int i = 0; i < 16 - k; ++i)
+            if (i < 7 + k) e[i] = by & k ? e[i + k] : e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = pack2(e[2 * i], e[2 * i + 1]);
+    return true;
+}
+template <typename T, int MODE>
 __device__ __forceinline__ void load_weight8(const void* w, bool f32, Cols c, F2 (&f)[4]) {
+    if (MODE == kShift && (f32 ? load_shifted8(static_cast<const float*>(w), c, f) : load_shifted8(static_cast<const T*>(w), c, f)))
+        return;
     if (f32)
-        unpack8(load8<float, VEC>(static_cast<const float*>(w), c), f);
+        unpack8(load8<float, MODE == kVec ? kVec : kApart>(static_cast<const float*>(w), c), f);
     else
-        unpack8(load8<T, VEC>(static_cast<const T*>(w), c), f);
+        unpack8(load8<T, MODE == kVec ? kVec : kApart>(static_cast<const T*>(w), c), f);
 }
 
 // Maxima keep a NaN (fmaxf drops it): a row that holds one gets a NaN scale.
@@ -220,7 +280,7 @@ __device__ __forceinline__ float lanes_sum_pair(float a, float b) {
 }
 
 // blockDim = (threads per row, rows per CTA), 8 VPT elements of a row per thread.
-template <typename T, int VPT, bool VEC>
+template <typename T, int VPT, int MODE>
 __global__ void __launch_bounds__(kNormThreads) gdn_add_norm_kernel(const NormParams p) {
     __shared__ float red_sum[kNormWarps], red_max[kNormWarps];
     const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -230,11 +290,12 @@ __global__ void __launch_bounds__(kNormThreads) gdn_add_norm_kernel(const NormPa
     const T* res = static_cast<const T*>(p.residual) + (live && p.residual ? row * p.residual_stride : 0);
     const int64_t out = row * p.width;
     const bool groups = p.quant == 2;
+    const int m = MODE == kShift ? static_cast<int>(out & 7) : 0;
     Raw8<T> rx[VPT], rr[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        rx[j] = load8<T, VEC>(x, row_cols<VEC>(j, width, groups));
-        if (p.residual) rr[j] = load8<T, VEC>(res, row_cols<VEC>(j, width, groups));
+        rx[j] = load8<T, MODE>(x, row_cols<MODE>(j, width, groups, m), row >= p.rows - 1);
+        if (p.residual) rr[j] = load8<T, MODE>(res, row_cols<MODE>(j, width, groups, m), row >= p.rows - 1);
     }
     F2 r[VPT][4], ss = splat2(0.0f);
 #pragma unroll
@@ -245,36 +306,39 @@ __global__ void __launch_bounds__(kNormThreads) gdn_add_norm_kernel(const NormPa
             unpack8(rr[j], f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[j][i] = add2(r[j][i], f[i]);
-            store8<T, VEC>(static_cast<T*>(p.new_residual) + out, row_cols<VEC>(j, width, groups), r[j]);
+        }
+        own8<MODE>(r[j], row_cols<MODE>(j, width, groups, m));
+        if (p.residual) {
+            store8<T, MODE>(static_cast<T*>(p.new_residual) + out, row_cols<MODE>(j, width, groups, m), r[j]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss = fma2(r[j][i], r[j][i], ss);
     }
     const float rstd = rsqrtf(row_reduce<false>(sum2(ss), red_sum) / static_cast<float>(p.width) + p.eps);
-    float m = 0.0f;
+    float amax8 = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const Cols c = row_cols<VEC>(j, width, groups);
+        const Cols c = row_cols<MODE>(j, width, groups, m);
         F2 w[4];
-        load_weight8<T, VEC>(p.weight, p.weight_f32, c, w);
+        load_weight8<T, MODE>(p.weight, p.weight_f32, c, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[j][i] = mul2(mul2(r[j][i], splat2(rstd)), w[i]);
         if (p.quant == 0) {
-            store8<T, VEC>(static_cast<T*>(p.out) + out, c, r[j]);
+            store8<T, MODE>(static_cast<T*>(p.out) + out, c, r[j]);
         } else if (groups) {  // 16 threads hold a group's 128 channels
             const float amax = lanes_max<16>(c.in(0) ? abs_max8(r[j], kAmaxMin) : kAmaxMin);
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out, c, r[j], kFp8Max / amax);
+            store8_e4m3<MODE>(static_cast<uint8_t*>(p.out) + out, c, r[j], kFp8Max / amax);
             if (c.in(0) && (threadIdx.x & 15) == 0)
                 p.scale[row * (p.width / kQuantGroup) + c.first / kQuantGroup] = amax / kFp8Max;
-        } else if (c.in(0)) {
-            m = abs_max8(r[j], m);
+        } else if (c.any()) {
+            amax8 = abs_max8(r[j], amax8);
         }
     }
     if (p.quant == 1) {
-        const float amax = max_keep_nan(row_reduce<true>(m, red_max), kAmaxMin), inv = kFp8Max / amax;
+        const float amax = max_keep_nan(row_reduce<true>(amax8, red_max), kAmaxMin), inv = kFp8Max / amax;
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + out, row_cols<VEC>(j, width, false), r[j], inv);
+            store8_e4m3<MODE>(static_cast<uint8_t*>(p.out) + out, row_cols<MODE>(j, width, false, m), r[j], inv);
         if (width > 0 && threadIdx.x == 0) p.scale[row] = amax / kFp8Max;
     }
 }
@@ -283,26 +347,32 @@ __global__ void __launch_bounds__(kNormThreads) gdn_add_norm_kernel(const NormPa
 // keeps its share of dweight in registers.  With p.stages > 0 the rows of x, dy
 // and dr arrive in shared memory by bulk copies, p.stages rows ahead of use
 // (without them a row's loads would wait for the row before it).
-template <typename T, int VPT, bool VEC>
+template <typename T, int VPT, int MODE>
 __global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_backward_kernel(const NormParams p, const NormGradParams d) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float red[2][2][kNormWarps];
     __shared__ __align__(8) uint64_t s_bar[kNormStages];
+    // kShift: gridDim.x is a multiple of 8 where a CTA has several rows
+    const int m = MODE == kShift ? static_cast<int>(static_cast<int64_t>(blockIdx.x) * p.width & 7) : 0;
     F2 dw[VPT][4], w[VPT][4];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        load_weight8<T, VEC>(p.weight, p.weight_f32, row_cols<VEC>(j, p.width, false), w[j]);
+        load_weight8<T, MODE>(p.weight, p.weight_f32, row_cols<MODE>(j, p.width, false, m), w[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dw[j][i] = splat2(0.0f);
     }
-    const uint32_t row_bytes = p.width * sizeof(T), bar = tc05::smem_u32(s_bar);
+    // A shifted row is copied with what its first and last vectors hold of its
+    // neighbours, which the last row has only on one side: its end is read directly.
+    const int slot = (m + p.width + 7) / 8 * 8, slot_max = (MODE == kShift ? p.width + 14 : p.width) / 8 * 8;
+    const uint32_t bar = tc05::smem_u32(s_bar);
     auto fetch = [&](int64_t row, int stage) {  // by one thread
         if (row >= p.rows) return;
-        const uint32_t to = tc05::smem_u32(smem) + stage * 3 * row_bytes;
-        tc05::mbar_expect_tx(bar + 8 * stage, row_bytes * (d.dr ? 3 : 2));
-        tc05::bulk_g2s(to, static_cast<const T*>(p.x) + row * p.x_stride, row_bytes, bar + 8 * stage);
-        tc05::bulk_g2s(to + row_bytes, static_cast<const T*>(d.dy) + row * d.dy_stride, row_bytes, bar + 8 * stage);
-        if (d.dr) tc05::bulk_g2s(to + 2 * row_bytes, static_cast<const T*>(d.dr) + row * d.dr_stride, row_bytes, bar + 8 * stage);
+        const uint32_t to = tc05::smem_u32(smem) + stage * 3 * slot_max * sizeof(T), next = slot_max * sizeof(T);
+        const uint32_t bytes = (MODE == kShift && row == p.rows - 1 ? (m + p.width) / 8 * 8 : slot) * sizeof(T);
+        tc05::mbar_expect_tx(bar + 8 * stage, bytes * (d.dr ? 3 : 2));
+        tc05::bulk_g2s(to, static_cast<const T*>(p.x) + row * p.x_stride - m, bytes, bar + 8 * stage);
+        tc05::bulk_g2s(to + next, static_cast<const T*>(d.dy) + row * d.dy_stride - m, bytes, bar + 8 * stage);
+        if (d.dr) tc05::bulk_g2s(to + 2 * next, static_cast<const T*>(d.dr) + row * d.dr_stride - m, bytes, bar + 8 * stage);
     };
     if (p.stages > 0 && threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) tc05::mbar_init(bar + 8 * i, 1);
@@ -316,20 +386,24 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_b
         const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
         const T* dy = static_cast<const T*>(d.dy) + row * d.dy_stride;
         const T* dr = static_cast<const T*>(d.dr) + (d.dr ? row * d.dr_stride : 0);
-        if (VEC && p.stages > 0) {
+        const T *ex = x, *edy = dy, *edr = dr;  // for the end of the last row
+        if (MODE != kApart && p.stages > 0) {
             if (!tc05::mbar_wait(bar + 8 * stage, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-            x = reinterpret_cast<const T*>(smem + stage * 3 * row_bytes);
-            dy = x + p.width;
-            dr = dy + p.width;
+            x = reinterpret_cast<const T*>(smem) + stage * 3 * slot_max + m;
+            dy = x + slot_max;
+            dr = dy + slot_max;
         }
         F2 r[VPT][4], g[VPT][4], o[VPT][4], ss2 = splat2(0.0f), dot2 = splat2(0.0f);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const Cols c = row_cols<VEC>(j, p.width, false);
-            unpack8(load8<T, VEC>(x, c), r[j]);
-            unpack8(load8<T, VEC>(dy, c), g[j]);
+            const Cols c = row_cols<MODE>(j, p.width, false, m);
+            const bool last = row == p.rows - 1, end = MODE == kShift && last && c.first + 8 > p.width;
+            unpack8(load8<T, MODE>(end ? ex : x, c, last), r[j]);
+            unpack8(load8<T, MODE>(end ? edy : dy, c, last), g[j]);
+            own8<MODE>(r[j], c);
+            own8<MODE>(g[j], c);
             if (d.dr) {
-                unpack8(load8<T, VEC>(dr, c), o[j]);
+                unpack8(load8<T, MODE>(end ? edr : dr, c, last), o[j]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[j][i] = splat2(0.0f);
@@ -346,7 +420,7 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_b
         const int warps = blockDim.x >> 5;
         if ((threadIdx.x & 15) == 0) red[turn][threadIdx.x >> 4 & 1][threadIdx.x >> 5] = both;
         __syncthreads();
-        if (VEC && p.stages > 0) {  // every thread has its part of the row: the stage takes another
+        if (MODE != kApart && p.stages > 0) {  // every thread has its part of the row: the stage takes another
             if (threadIdx.x == 0) fetch(row + static_cast<int64_t>(p.stages) * gridDim.x, stage);
             stage = stage + 1 == p.stages ? 0 : stage + 1;
             phase ^= stage == 0;
@@ -369,12 +443,12 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_b
                 dw[j][i] = fma2(g[j][i], mul2(r[j][i], rstd2), dw[j][i]);
                 o[j][i] = add2(o[j][i], fma2(mul2(g[j][i], w[j][i]), rstd2, mul2(r[j][i], back)));
             }
-            store8<T, VEC>(static_cast<T*>(d.dx) + row * p.width, row_cols<VEC>(j, p.width, false), o[j]);
+            store8<T, MODE>(static_cast<T*>(d.dx) + row * p.width, row_cols<MODE>(j, p.width, false, m), o[j]);
         }
     }
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
-        store8<float, VEC>(d.part + static_cast<int64_t>(blockIdx.x) * p.width, row_cols<VEC>(j, p.width, false), dw[j]);
+        store8<float, MODE == kVec ? kVec : kApart>(d.part + static_cast<int64_t>(blockIdx.x) * p.width, row_cols<MODE>(j, p.width, false, m), dw[j]);
 }
 
 // out[c] = sum of part[.][c], in a fixed order.  blockDim = (32, 32).
@@ -395,7 +469,7 @@ __global__ void __launch_bounds__(1024) gdn_sum_columns_kernel(const float* part
 // LANES = head dim / 8 threads per head; item = (token, head), kGatedItems of
 // them per thread.
 constexpr int kGatedItems = 2;
-template <typename T, int LANES, bool VEC>
+template <typename T, int LANES, int MODE>
 __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormParams p) {
     constexpr int kHeadDim = LANES * 8, kGroups = 256 / LANES;
     const int col = (threadIdx.x % LANES) * 8;
@@ -407,11 +481,11 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
         const unsigned item = items[n] < p.items ? items[n] : 0;
         const unsigned token = item / p.heads, head = item - token * p.heads;
         const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
-        rx[n] = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
-        rz[n] = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
+        rx[n] = load8<T, MODE>(static_cast<const T*>(p.x) + token * p.x_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
+        rz[n] = load8<T, MODE>(static_cast<const T*>(p.z) + token * p.z_stride + in, {0, 1, items[n] < p.items ? 8 : 0});
     }
     F2 w[4];
-    load_weight8<T, VEC>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
+    load_weight8<T, MODE>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
 #pragma unroll
     for (int n = 0; n < kGatedItems; ++n) {
         const unsigned item = items[n];
@@ -426,10 +500,10 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(mul2(x[i], rstd), w[i]), mul2(z[i], sigmoid2(z[i])));
         if (!p.quant) {
-            store8<T, VEC>(static_cast<T*>(p.out) + o, all, x);
+            store8<T, MODE>(static_cast<T*>(p.out) + o, all, x);
         } else {
             const float amax = lanes_max<LANES>(abs_max8(x, kAmaxMin));
-            store8_e4m3<VEC>(static_cast<uint8_t*>(p.out) + o, all, x, kFp8Max / amax);
+            store8_e4m3<MODE>(static_cast<uint8_t*>(p.out) + o, all, x, kFp8Max / amax);
             if (col == 0 && item < p.items) p.scale[item] = amax / kFp8Max;
         }
     }
@@ -438,14 +512,14 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_kernel(const GatedNormPara
 // Every thread keeps the same 8 columns for all its items: dweight stays in
 // registers, and the CTA's groups are added in order at the end.  The next
 // item is on its way while one is worked on.
-template <typename T, int LANES, bool VEC>
+template <typename T, int LANES, int MODE>
 __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const GatedNormParams p,
                                                                        const GatedNormGradParams d) {
     constexpr int kHeadDim = LANES * 8, kGroups = 256 / LANES;
     __shared__ float red[kGroups][kHeadDim];
     const int group = threadIdx.x / LANES, col = (threadIdx.x % LANES) * 8;
     F2 w[4], dw[4];
-    load_weight8<T, VEC>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
+    load_weight8<T, MODE>(p.weight, p.weight_f32, {col, 1, kHeadDim}, w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[i] = splat2(0.0f);
     Raw8<T> rx, rz, ry;
@@ -455,9 +529,9 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const Gate
         const unsigned item = live ? static_cast<unsigned>(first + group) : 0;
         const unsigned token = item / p.heads, head = item - token * p.heads;
         const int64_t in = static_cast<int64_t>(head) * kHeadDim + col;
-        rx = load8<T, VEC>(static_cast<const T*>(p.x) + token * p.x_stride + in, all);
-        rz = load8<T, VEC>(static_cast<const T*>(p.z) + token * p.z_stride + in, all);
-        ry = load8<T, VEC>(static_cast<const T*>(d.dy) + token * d.dy_stride + in, all);
+        rx = load8<T, MODE>(static_cast<const T*>(p.x) + token * p.x_stride + in, all);
+        rz = load8<T, MODE>(static_cast<const T*>(p.z) + token * p.z_stride + in, all);
+        ry = load8<T, MODE>(static_cast<const T*>(d.dy) + token * d.dy_stride + in, all);
     };
     const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
     int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups;
@@ -486,8 +560,8 @@ __global__ void __launch_bounds__(256) gdn_gated_norm_backward_kernel(const Gate
             z[i] = mul2(mul2(dyn, w[i]), fma2(gate, fma2(sig[i], splat2(-1.0f), splat2(1.0f)), sig[i]));
         }
         const Cols all = {0, 1, item < p.items ? 8 : 0};
-        store8<T, VEC>(static_cast<T*>(d.dx) + item * kHeadDim + col, all, x);
-        store8<T, VEC>(static_cast<T*>(d.dz) + item * kHeadDim + col, all, z);
+        store8<T, MODE>(static_cast<T*>(d.dx) + item * kHeadDim + col, all, x);
+        store8<T, MODE>(static_cast<T*>(d.dz) + item * kHeadDim + col, all, z);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -510,15 +584,17 @@ struct RowShape {
 static RowShape row_shape(int vecs, int vpt) { return {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt}; }
 // Forward.  Two vectors per thread halve the warps that a row's sum waits for
 // (32768 x 2048 bf16: 82.7 us, 93.0 with one); four where a scale per row adds
-// a second wait (65536 x 1024: 74.7 us, 82.9 with two; fp32 would spill the
-// occupancy: 146 us for 16384 x 4096, 130 with two).  Rows off the 16-byte
-// boundary hold twice the registers per vector, so fewer (16384 x 5333: 320 us
+// a second wait (65536 x 1024: 74.7 us, 82.9 with two); but fp32 takes two up to
+// 1024 vectors, for its occupancy (16384 x 4096 with a scale per row: 130 us, 146
+// with four; 16384 x 6144: 196 and 206; shifted 16384 x 4097: 185 and 232).  Rows
+// dealt apart hold twice the registers per vector, so fewer (16384 x 5333: 320 us
 // with two, 483 with four).
+static int row_vecs(int width, int mode) { return (width + (mode == kShift ? 14 : 7)) / 8; }
 static RowShape row_shape_forward(const NormParams& p, size_t elem) {
-    const int vecs = (p.width + 7) / 8;
-    if (!p.vec) return row_shape(vecs, vecs <= 512 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8);
-    if (p.quant == 1 && elem == 2 && vecs >= 128 && vecs <= 2048) return row_shape(vecs, 4);
-    return row_shape(vecs, vecs <= 32 ? 1 : vecs <= 512 ? 2 : vecs <= 2048 ? 4 : 8);
+    const int vecs = row_vecs(p.width, p.mode);
+    if (p.mode == kApart) return row_shape(vecs, vecs <= 512 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8);
+    if (p.quant == 1 && elem == 2 && p.mode == kVec && vecs >= 128 && vecs <= 2048) return row_shape(vecs, 4);
+    return row_shape(vecs, vecs <= 32 ? 1 : vecs <= (elem == 4 ? 1024 : 512) ? 2 : vecs <= 2048 ? 4 : 8);
 }
 constexpr int kNormMaxWidth = kNormThreads * 8 * 8;
 
@@ -526,13 +602,13 @@ constexpr int kNormMaxWidth = kNormThreads * 8 * 8;
 template <int V>
 using Int = std::integral_constant<int, V>;
 template <typename F>
-static void with_row_shape(int vpt, bool vec, F f) {
-    const auto go = [&](auto n) { vec ? f(n, std::true_type{}) : f(n, std::false_type{}); };
+static void with_row_shape(int vpt, int mode, F f) {
+    const auto go = [&](auto n) { mode == kVec ? f(n, Int<kVec>{}) : mode == kShift ? f(n, Int<kShift>{}) : f(n, Int<kApart>{}); };
     vpt == 1 ? go(Int<1>{}) : vpt == 2 ? go(Int<2>{}) : vpt == 4 ? go(Int<4>{}) : go(Int<8>{});
 }
 template <typename F>
 static void with_head_shape(int head_dim, bool vec, F f) {
-    const auto go = [&](auto n) { vec ? f(n, std::true_type{}) : f(n, std::false_type{}); };
+    const auto go = [&](auto n) { vec ? f(n, Int<kVec>{}) : f(n, Int<kApart>{}); };
     head_dim == 64 ? go(Int<8>{}) : head_dim == 128 ? go(Int<16>{}) : go(Int<32>{});
 }
 
@@ -542,23 +618,24 @@ static cudaError_t launch_add_norm(const NormParams& p, cudaStream_t s) {
     const int per_cta = r.threads >= 256 ? 1 : 256 / r.threads;
     const dim3 block(r.threads, per_cta);
     const unsigned grid = static_cast<unsigned>((p.rows + per_cta - 1) / per_cta);
-    with_row_shape(r.vpt, p.vec, [&](auto vpt, auto vec) { gdn_add_norm_kernel<T, vpt(), vec()><<<grid, block, 0, s>>>(p); });
+    with_row_shape(r.vpt, p.mode, [&](auto vpt, auto mode) { gdn_add_norm_kernel<T, vpt(), mode()><<<grid, block, 0, s>>>(p); });
     return cudaGetLastError();
 }
 
 // Backward: the weight and its gradient's share are held too, so two vectors at
 // most while they fit (65536 x 4096 bf16: 332 us, 407 with one on twice the
 // threads, whose sums wait for twice the warps).
-static RowShape row_shape_backward(int width, bool vec) {
-    const int vecs = (width + 7) / 8;
-    if (!vec) return row_shape(vecs, vecs <= 1024 ? 1 : vecs <= 2048 ? 4 : 8);
+static RowShape row_shape_backward(int width, int mode) {
+    const int vecs = row_vecs(width, mode);
+    if (mode == kApart) return row_shape(vecs, vecs <= 1024 ? 1 : vecs <= 2048 ? 4 : 8);
     return row_shape(vecs, vecs <= 32 ? 1 : vecs <= 1024 ? 2 : vecs <= 2048 ? 4 : 8);
 }
 
-static int norm_backward_ctas(int64_t rows, int width, bool vec) {
-    const RowShape r = row_shape_backward(width, vec);
+static int norm_backward_ctas(int64_t rows, int width, int mode) {
+    const RowShape r = row_shape_backward(width, mode);
     const int per_sm = (r.vpt == 1 ? 1024 : 512) / r.threads;  // by registers
-    const int64_t most = static_cast<int64_t>(kSmCount) * (per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm);
+    int64_t most = static_cast<int64_t>(kSmCount) * (per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm);
+    if (mode == kShift) most = most / 8 * 8;  // a CTA's rows all start at the same place in a vector
     return static_cast<int>(rows < most ? (rows > 0 ? rows : 1) : most);
 }
 
@@ -569,19 +646,19 @@ static cudaError_t launch_sum_columns(const float* part, int rows, int width, fl
 
 template <typename T>
 static cudaError_t launch_add_norm_backward(NormParams p, const NormGradParams& d, float* dweight, cudaStream_t s) {
-    const RowShape r = row_shape_backward(p.width, p.vec);
-    const int grid = norm_backward_ctas(p.rows, p.width, p.vec);
+    const RowShape r = row_shape_backward(p.width, p.mode);
+    const int grid = norm_backward_ctas(p.rows, p.width, p.mode);
     // Rows in flight for about 200 KB of an SM's shared memory over its CTAs;
-    // fewer than two would not run ahead, and rows off the 16-byte boundary
-    // cannot be copied in bulk (65536 x 4096: 407 us, 536 without).
+    // fewer than two would not run ahead, and rows at any alignment cannot be
+    // copied in bulk (65536 x 4096: 407 us, 536 without).
     const int per_sm = (grid + kSmCount - 1) / kSmCount;
-    const size_t stage = 3 * static_cast<size_t>(p.width) * sizeof(T);
+    const size_t stage = 3 * 8 * static_cast<size_t>(row_vecs(p.width, p.mode)) * sizeof(T);
     const int fit = static_cast<int>((200 << 10) / per_sm / stage);
-    p.stages = !p.vec || fit < 2 ? 0 : fit < kNormStages ? fit : kNormStages;
+    p.stages = p.mode == kApart || fit < 2 ? 0 : fit < kNormStages ? fit : kNormStages;
     const int smem = static_cast<int>(p.stages * stage);
     cudaError_t e = cudaSuccess;
-    with_row_shape(r.vpt, p.vec, [&](auto vpt, auto vec) {
-        const auto kernel = gdn_add_norm_backward_kernel<T, vpt(), vec()>;
+    with_row_shape(r.vpt, p.mode, [&](auto vpt, auto mode) {
+        const auto kernel = gdn_add_norm_backward_kernel<T, vpt(), mode()>;
         if (smem > (40 << 10)) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e == cudaSuccess) kernel<<<grid, r.threads, smem, s>>>(p, d);
     });
@@ -619,6 +696,23 @@ static bool rows_vec(const void* p, int64_t stride_bytes, uintptr_t bytes = 16) 
     return p == nullptr || (aligned(p, bytes) && stride_bytes % static_cast<int64_t>(bytes) == 0);
 }
 
+// How rows of `width` elements that are `stride` apart can be read, all tensors
+// alike (absent ones NULL).
+struct RowsOf {
+    const void* p;
+    int64_t stride;
+};
+static int row_mode(int64_t width, uintptr_t es, std::initializer_list<RowsOf> tensors) {
+    const bool shift = width >= 16 && row_vecs(static_cast<int>(width), kShift) <= kNormThreads * 8;
+    int mode = width % 8 == 0 ? kVec : shift ? kShift : kApart;
+    for (const RowsOf& t : tensors) {
+        if (t.p == nullptr) continue;
+        const bool vec = rows_vec(t.p, t.stride * static_cast<int64_t>(es)), alike = aligned(t.p, 16) && (t.stride - width) % 8 == 0;
+        if (mode == kVec ? !vec : !alike) mode = kApart;
+    }
+    return mode;
+}
+
 static int add_norm_setup(const GdnAddNormArgs* a, NormParams& p) {
     if (a == nullptr) return GDN_ERR_NULL_POINTER;
     if (!dtype_ok(a->dtype) || (a->weight_dtype != GDN_DTYPE_F32 && a->weight_dtype != a->dtype)) return GDN_ERR_BAD_DTYPE;
@@ -634,16 +728,15 @@ static int add_norm_setup(const GdnAddNormArgs* a, NormParams& p) {
         !aligned(a->output, a->quant ? 1 : es) || !aligned(a->weight, dtype_bytes(a->weight_dtype)) ||
         !aligned(a->scale, 4))
         return GDN_ERR_MISALIGNED;
-    const int64_t row = a->width * static_cast<int64_t>(es);
     p.x = a->x;
     p.residual = a->residual;
     p.x_stride = a->x_stride;
     p.residual_stride = a->residual_stride;
     p.weight = a->weight;
     p.weight_f32 = a->weight_dtype == GDN_DTYPE_F32;
-    p.vec = a->width % 8 == 0 && rows_vec(a->x, a->x_stride * es) && rows_vec(a->residual, a->residual_stride * es) &&
-            rows_vec(a->new_residual, row) && aligned(a->weight, 16) &&
-            (a->quant ? aligned(a->output, 8) : rows_vec(a->output, row));
+    p.mode = row_mode(a->width, es, {{a->x, a->x_stride}, {a->residual, a->residual_stride}, {a->new_residual, a->width}});
+    if (a->quant ? !aligned(a->output, 8) : !aligned(a->output, 16)) p.mode = kApart;
+    if (p.mode == kVec && !aligned(a->weight, 16)) p.mode = kApart;
     p.quant = a->quant;
     p.rows = a->rows;
     p.width = static_cast<int>(a->width);
@@ -703,8 +796,12 @@ extern "C" int gdn_add_norm_launch(const GdnAddNormArgs* a, void* stream) {
 
 extern "C" size_t gdn_add_norm_backward_workspace_size(int64_t rows, int64_t width) {
     if (rows < 0 || width < 1 || width > kNormMaxWidth) return 0;
-    const int a = norm_backward_ctas(rows, static_cast<int>(width), true), b = norm_backward_ctas(rows, static_cast<int>(width), false);
-    return static_cast<size_t>(a > b ? a : b) * width * sizeof(float);
+    int most = 0;
+    for (int mode : {kApart, kVec, kShift}) {
+        const int n = norm_backward_ctas(rows, static_cast<int>(width), mode);
+        most = n > most ? n : most;
+    }
+    return static_cast<size_t>(most) * width * sizeof(float);
 }
 
 extern "C" int gdn_add_norm_backward_launch(const GdnAddNormArgs* a, const GdnNormGradArgs* g, void* workspace,
@@ -723,8 +820,9 @@ extern "C" int gdn_add_norm_backward_launch(const GdnAddNormArgs* a, const GdnNo
         !aligned(workspace, 16))
         return GDN_ERR_WORKSPACE;
     if (int rc = check_device()) return rc;
-    p.vec = p.vec && rows_vec(g->d_output, g->d_output_stride * es) &&
-            rows_vec(g->d_new_residual, g->d_new_residual_stride * es) && rows_vec(g->dx, a->width * es);
+    const int mode = row_mode(a->width, es, {{g->d_output, g->d_output_stride}, {g->d_new_residual, g->d_new_residual_stride},
+                                             {g->dx, a->width}});
+    if (mode != p.mode) p.mode = kApart;
     NormGradParams d;
     d.dy = g->d_output;
     d.dr = g->d_new_residual;

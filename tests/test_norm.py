@@ -10,7 +10,7 @@ from tests.conftest import state_rel_err
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 EPS = 1e-6
 gpu = pytest.mark.gpu
-WIDTHS = [1, 7, 8, 100, 128, 250, 256, 1000, 1024, 2048, 2056, 4096, 5333, 8192, 16384, 32768]
+WIDTHS = [1, 7, 8, 100, 128, 250, 256, 1000, 1024, 2048, 2056, 4096, 5333, 8192, 16384, 32761, 32767, 32768]
 
 
 def rnd(*shape, dtype=torch.float32, device="cpu", scale=1.0, seed=0):
@@ -68,7 +68,42 @@ def test_add_norm_backward(pkg, cuda_dev, rows, width, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("width", [8192, 20000, 32768])
+@pytest.mark.parametrize("width", [1, 7, 250, 1003, 5333])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_of_odd_widths(pkg, cuda_dev, width, dtype):
+    """More rows than the backward kernel has thread blocks, of widths where each row starts elsewhere in a
+    16-byte vector: the results, and what lies beside the rows stays as it was.  The tensors begin off the boundary
+    (the buffers' lengths are odd), on it and contiguous, and on it with 8 elements between rows; the last two are
+    summed alike."""
+    rows = 2003
+    buf = rnd(4, rows * (width + 8), dtype=dtype, device=cuda_dev)
+    x, res, dy, dr = (b.view(rows, width + 8)[:, :width] for b in buf)
+    w = 1 + rnd(width, device=cuda_dev, scale=0.1)
+    want_r, want_y = ref.add_norm(x, res, w, EPS)
+    want_dx, want_dw = ref.add_norm(None, None, w, EPS, dy=dy, dr=dr, summed=x)
+    n, out = rows * width, []
+    whole = [t.contiguous() for t in (x, res, dy, dr)]
+    apart = [torch.nn.functional.pad(t, (0, 8), value=9.0)[:, :width] for t in whole]
+    for a, b, c, d in ((x, res, dy, dr), whole, apart):
+        room = torch.full((3, (n + 71) // 8 * 8), 7.0, dtype=dtype, device=cuda_dev)
+        codes = torch.full((n + 64,), 7.0, device=cuda_dev).to(torch.float8_e4m3fn)
+        y, r, dx = (t[:n].view(rows, width) for t in room)
+        pkg.norm.launch_add_norm(a, b, w, EPS, output=y, new_residual=r)
+        q, _, scale = pkg.norm.launch_add_norm(a, b, w, EPS, quant="row", output=codes[:n].view(rows, width))
+        _, dw = pkg.norm.launch_add_norm_backward(c, a, w, EPS, d_new_residual=d, dx=dx)
+        ref.close(r, *want_r, "r")
+        ref.close(y, *want_y, "y")
+        ref.codes_ok(q, scale, *want_y, width)
+        ref.close(dx, *want_dx, "dx")
+        ref.close(dw, *want_dw, "dweight")
+        assert bool((room[:, n:] == 7).all()) and bool((codes[n:].float() == 7).all())
+        out.append([y.clone(), r.clone(), q.clone().float(), dx.clone(), dw])
+    for t, u in zip(*out[1:]):
+        assert torch.equal(t, u)
+
+
+@gpu
+@pytest.mark.parametrize("width", [8192, 20000, 32761, 32767, 32768])
 def test_add_norm_backward_wide(pkg, cuda_dev, width):
     x, _, w = make(40, width, torch.bfloat16, cuda_dev)
     dy = rnd(40, width, dtype=torch.bfloat16, device=cuda_dev, seed=8)

@@ -64,8 +64,19 @@ def check_backward(pkg, i, dns=True):
     return got
 
 
-# lengths that meet the edges of the kernels' tiles (60 and 120 tokens), and sequences of nothing
-LENS = [[1], [0], [2, 0, 0, 1], [59], [60], [61], [120], [121], [127], [128], [129], [5, 123, 128, 1, 255], [700], [64, 3, 0, 300, 1, 1, 1, 90], [1] * 200]
+# lengths that meet the edges of the kernels' pieces and tiles (60 and 120 tokens backward, 76 and 152 forward), and
+# sequences of nothing
+LENS = [[1], [0], [2, 0, 0, 1], [59], [60], [61], [120], [121], [127], [128], [129], [5, 123, 128, 1, 255], [700], [64, 3, 0, 300, 1, 1, 1, 90], [1] * 200,
+        [75], [76], [77], [151], [152], [153], [305], [76, 76, 1, 151], [1, 152, 3, 305]]
+
+
+@gpu
+@pytest.mark.parametrize("N", [1022, 1023, 1024, 1025])
+def test_scan_of_many_sequences(pkg, cuda_dev, N):
+    """Up to 1023 sequences the kernels keep the offsets in shared memory."""
+    i = make([(k * 7) % 4 for k in range(N)], 40, torch.bfloat16, cuda_dev)
+    check_forward(pkg, i)
+    check_backward(pkg, i)
 
 
 @gpu
