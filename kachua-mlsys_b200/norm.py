@@ -84,6 +84,8 @@ def launch_add_norm(x, residual, weight, eps=1e-6, output=None, new_residual=Non
         output = _like(x, odt)
     else:
         _dense(output, "output", odt, (rows, width), dev)
+        _need(rows == 0 or new_residual is None or output.data_ptr() != new_residual.data_ptr(),
+              "output must not be new_residual")
     if quant:
         scale_shape = (rows, 1 if quant == "row" else width // GROUP)
         if scale is None:
@@ -232,6 +234,7 @@ def launch_gated_norm_backward(d_output, x, z, weight, eps=1e-6, dx=None, dz=Non
         dz = _like(x).view(shape)
     else:
         _dense(dz, "dz", x.dtype, shape, dev)
+        _need(tokens == 0 or dz.data_ptr() != dx.data_ptr(), "dz must not be dx")
     d_weight = _like(weight, torch.float32)
     lib = _capi.load()
     need = int(lib.gdn_gated_norm_backward_workspace_size(tokens, heads, dim))

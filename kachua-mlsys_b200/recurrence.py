@@ -244,6 +244,7 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
             grad_strides.append(_rows(t, name, x.dtype, T, C, dev))
             _need(T == 0 or t.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr(), d_output.data_ptr()),
                   f"{name} must not overlap an input")
+            _need(T == 0 or all(t.data_ptr() != u.data_ptr() for u in grads), f"{name} must not overlap another gradient")
         grads.append(t)
     dA_log, d_dt_bias = _like(A_log), _like(dt_bias)
     d_state = None if state is None else _like(state)

@@ -411,6 +411,11 @@ def test_refusals(pkg, cuda_dev):
         n.launch_add_norm_backward(res[:2], x, w)
     with pytest.raises(ValueError, match="d_output must"):
         n.launch_gated_norm_backward(zh[:2], xh, zh, wh)
+    out = torch.empty_like(x)
+    with pytest.raises(ValueError, match="output must not be new_residual"):
+        n.launch_add_norm(x, res, w, output=out, new_residual=out)
+    with pytest.raises(ValueError, match="dz must not be dx"):
+        n.launch_gated_norm_backward(zh, xh, zh, wh, dx=out.view_as(xh), dz=out.view_as(xh))
 
 
 def test_cpu_tensors_are_refused(pkg):

@@ -480,6 +480,17 @@ def test_scan_refusals(pkg):
     _refuse(pkg, "non-decreasing", {**i, "cu": torch.tensor([0, 6, 4])}, check_seqlens=True)
 
 
+@gpu
+@pytest.mark.parametrize("same", [("dx", "da"), ("da", "db"), ("dx", "db")])
+def test_scan_gradients_apart(pkg, cuda_dev, same):
+    i = make([4, 6], 16, torch.bfloat16, cuda_dev)
+    out = torch.empty_like(i["x"])
+    with pytest.raises(ValueError, match="another gradient"):
+        backward(pkg, i, **dict.fromkeys(same, out))
+    with pytest.raises(ValueError, match="must not overlap an input"):
+        backward(pkg, i, **{same[0]: i["dy"]})
+
+
 def test_scan_capi_refusals(pkg):
     """Host-side checks come before any device call, so they answer without a GPU."""
     lib, C = pkg._capi.load(), pkg._capi
