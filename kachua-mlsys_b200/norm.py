@@ -40,7 +40,7 @@ def _weight(weight, width: int, dtype, device) -> int:
 def _row_inputs(x, weight, eps) -> tuple[int, int, int]:
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a [rows, width] tensor")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if x.dtype not in DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
@@ -131,7 +131,7 @@ def launch_add_norm_backward(d_output, new_residual, weight, eps=1e-6, d_new_res
 
 def _heads(t, name: str, dtype, shape, device) -> int:
     """Checks a [tokens, heads, dim] tensor whose tokens are contiguous; returns the token stride."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != shape:
         _fault(t, name, dtype, shape, device)
     tokens, heads, dim = shape
     step, head, inner = t.stride()
@@ -148,7 +148,7 @@ def _gated_inputs(x, z, weight, eps):
     """x and z as [tokens, heads, dim] with their token strides, and the weight's type."""
     if not isinstance(x, torch.Tensor) or x.dim() < 3:
         raise ValueError("x must be a [tokens, heads, dim] tensor")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if x.dtype not in DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")

@@ -46,7 +46,7 @@ def _fault(t, name: str, dtype, shape, device) -> None:
 # made only when there is something to say.
 def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
     """Checks a ``[rows, width]`` tensor with contiguous rows; returns its row stride."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != (rows, width):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != (rows, width):
         _fault(t, name, dtype, (rows, width), device)
     stride, inner = t.stride()
     if inner != 1 and width > 1:
@@ -58,16 +58,8 @@ def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
     return stride
 
 
-def _rows_like(t, name: str, x, stride: int) -> int:
-    """``_rows`` of a tensor that mostly has the layout of ``x`` (checked, row stride ``stride``)."""
-    if (isinstance(t, torch.Tensor) and t.dtype == x.dtype and t.shape == x.shape and t.device == x.device
-            and t.stride() == x.stride()):
-        return stride
-    return _rows(t, name, x.dtype, *x.shape, x.device)
-
-
 def _dense(t, name: str, dtype, shape, device) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != shape:
         _fault(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -103,18 +95,25 @@ def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
     """Checks what every entry point takes; returns (rows, channels, x, a and b strides)."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a [T, C] tensor")
-    dtype, dev = x.dtype, x.device
-    T, C = x.shape
-    if require_cuda and dev.type != "cuda":
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    T, C = shape
+    if require_cuda and not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if dtype not in DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
     if C < 1:
         raise ValueError("x must have at least one channel")
-    stride = _rows(x, "x", dtype, T, C, dev)
-    strides = (stride, _rows_like(a, "a", x, stride), _rows_like(b, "b", x, stride))
-    _dense(A_log, "A_log", torch.float32, (C,), dev)
-    _dense(dt_bias, "dt_bias", torch.float32, (C,), dev)
+    layout = x.stride()
+    stride = layout[0] if T > 1 and layout[1] == 1 and layout[0] >= C else _rows(x, "x", dtype, T, C, dev)
+    strides = [stride]
+    for t, name in ((a, "a"), (b, "b")):  # mostly in the layout of x
+        if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.shape == shape
+                and t.stride() == layout):
+            strides.append(stride)
+        else:
+            strides.append(_rows(t, name, dtype, T, C, dev))
+    for t, name in ((A_log, "A_log"), (dt_bias, "dt_bias")):
+        _dense(t, name, torch.float32, (C,), dev)
     return T, C, strides
 
 
