@@ -502,7 +502,7 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 // Bound by instruction issue: 80 warp instructions per token and pair of
 // channels, 64 % of the slots with five warps to a scheduler.  Measured (bf16):
 // 1 x 16384 x 4096 143 us, 3.8 TB/s of inputs and outputs, 57 % of the copy
-// rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 174 us.  A thread per
+// rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 172 us.  A thread per
 // sequence and channel took 42 ms for the second.
 template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanParams p) {
@@ -791,7 +791,7 @@ struct GradTile<float> {  // 40 bytes
 // writes its piece's gradients a tile later, when both ends are known.  The
 // sums over tokens stay in registers to the end, and are added over the CTA's
 // warps and the cluster's CTAs in order.  Bound by instruction issue like the
-// forward pass; measured (bf16): 1 x 16384 x 4096 270 us, 3.5 TB/s;
+// forward pass; measured (bf16): 1 x 16384 x 4096 279 us, 3.4 TB/s;
 // 8 x 4096 x 1024 177 us.
 template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
