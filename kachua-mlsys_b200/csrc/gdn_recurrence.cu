@@ -499,7 +499,7 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 //               order (the same bits on every run).
 // So the gates' arithmetic, which is what the kernel is made of, has a whole
 // tile's time to hide the cluster's exchange behind.
-// Bound by instruction issue: 80 warp instructions per token and pair of
+// Bound by instruction issue: 83 warp instructions per token and pair of
 // channels, 64 % of the slots with five warps to a scheduler.  Measured (bf16):
 // 1 x 16384 x 4096 143 us, 3.8 TB/s of inputs and outputs, 57 % of the copy
 // rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 172 us.  A thread per

@@ -205,6 +205,42 @@ def test_offsets_past_32_bits(pkg, cuda_dev):
 
 
 @gpu
+@pytest.mark.parametrize("width", [17, 250, 1003, 5333])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_of_odd_widths_do_not_leak(pkg, cuda_dev, bad, width):
+    """A vector of 8 elements can hold the end of one row and the start of the next; in place too."""
+    x, res, w = make(40, width, torch.bfloat16, cuda_dev)
+    dy = rnd(40, width, dtype=torch.bfloat16, device=cuda_dev, seed=8)
+    keep = torch.arange(40, device=cuda_dev) % 3 != 1
+    x2, dy2 = x.clone(), dy.clone()
+    x2[~keep], dy2[~keep] = bad, bad
+    for quant in (None, "row"):
+        good, got = (pkg.norm.launch_add_norm(t, res.clone(), w, EPS, quant=quant) for t in (x, x2))
+        in_place = x2.clone()
+        again = pkg.norm.launch_add_norm(in_place, res, w, EPS, quant=quant, new_residual=in_place)
+        for a, b, c in zip(good, got, again):
+            assert torch.equal(a[keep].float(), b[keep].float()) and torch.equal(a[keep].float(), c[keep].float())
+        assert bool(got[0][~keep].float().isnan().all())
+    dx, dx2 = (pkg.norm.launch_add_norm_backward(g, t, w, EPS, d_new_residual=g)[0] for g, t in ((dy, x), (dy2, x2)))
+    assert torch.equal(dx[keep], dx2[keep]) and bool(dx2[~keep].isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_weights_of_odd_widths(pkg, cuda_dev, dtype):
+    """Weights of either type that begin on a 16-byte boundary and off it."""
+    x, res, w = make(9, 1003, dtype, cuda_dev)
+    for wt in (w, w.to(dtype)):
+        off = torch.cat([wt[:1], wt])[1:]
+        for weight in (wt, off):
+            ref.close(pkg.norm.launch_add_norm(x, res, weight, EPS)[0], *ref.add_norm(x, res, wt, EPS)[1], "y")
+            dx, dw = pkg.norm.launch_add_norm_backward(res, x, weight, EPS)
+            want_dx, want_dw = ref.add_norm(None, None, wt, EPS, dy=res, summed=x)
+            ref.close(dx, *want_dx, "dx")
+            ref.close(dw, *want_dw, "dw")
+
+
+@gpu
 def test_in_place(pkg, cuda_dev):
     x, res, w = make(33, 2048, torch.bfloat16, cuda_dev)
     y, r = pkg.norm.launch_add_norm(x, res, w, EPS)
