@@ -348,7 +348,8 @@ int gdn_scan_step_launch(const GdnScanArgs* args, int64_t tokens, void* stream);
  *               (the same rows, contiguous).  The norm is of the unrounded r.
  *   output      [rows, width] of `dtype`, or e4m3 codes
  *   scale       fp32 [rows] or [rows, width / 128] (width a multiple of 128):
- *               max(amax |y|, 1e-12) / 448; code = e4m3(y / scale), saturating;
+ *               max(amax |y|, 1e-12) / 448; code = e4m3(y / scale), saturating, of
+ *               the fp32 y and quotient (two roundings), by the scale as stored;
  *               NaN stays NaN, in the scale too
  * No reference counterpart (the reference has the recurrence alone). */
 typedef struct GdnAddNormArgs {

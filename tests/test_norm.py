@@ -505,3 +505,56 @@ def test_capi_refusals(pkg):
         assert fn(args(), grad(), p, need - 1, None) == WS
         assert fn(args(), grad(), None, need, None) == WS
     assert lib.gdn_add_norm_launch(None, None) == NULL and lib.gdn_gated_norm_launch(None, None) == NULL
+
+
+# ------------------------------------------------------- codes of a quotient --
+def _e4m3_of(y, scale):
+    """The codes by definition: torch's own fp32 division by the stored scales, then its conversion."""
+    return (y / scale[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn).float()
+
+
+def _scale_of(y):
+    # a tensor, since by a number torch multiplies with its reciprocal
+    return y.abs().amax(-1).clamp(min=1e-12) / torch.full((), 448.0, device=y.device)
+
+
+@gpu
+@pytest.mark.parametrize("quant,width", [("row", 4096), ("group", 4096), ("row", 1003), ("row", 250)])
+def test_codes_are_y_over_the_stored_scale(pkg, cuda_dev, quant, width):
+    """Every code of 33 million, at its ties too.  An fp32 output is the y that the codes are made of."""
+    x, res, w = make((1 << 25) // width, width, torch.float32, cuda_dev)
+    y, _ = pkg.norm.launch_add_norm(x, res, w, EPS)
+    q, _, s = pkg.norm.launch_add_norm(x, res, w, EPS, quant=quant)
+    per = y.unflatten(1, (s.shape[1], -1))
+    assert torch.equal(s, _scale_of(per))
+    assert torch.equal(q.float(), _e4m3_of(per, s).flatten(1))
+
+
+@gpu
+def test_gated_codes_are_y_over_the_stored_scale(pkg, cuda_dev):
+    x, z = (rnd(65536, 4, 128, device=cuda_dev, seed=k) for k in (1, 2))
+    w = 1 + rnd(128, device=cuda_dev, scale=0.1)
+    y = pkg.norm.launch_gated_norm(x, z, w, EPS)
+    q, s = pkg.norm.launch_gated_norm(x, z, w, EPS, quant=True)
+    assert torch.equal(s, _scale_of(y)) and torch.equal(q.float(), _e4m3_of(y, s))
+
+
+@gpu
+@pytest.mark.parametrize("quant", ["row", "group"])
+def test_codes_beside_an_infinite_output(pkg, cuda_dev, quant):
+    """A weight that overflows its column: that code is NaN, its neighbours' are 0 over an infinite scale; the
+    smallest and the largest finite scales hold too."""
+    x, res, w = make(5, 256, torch.float32, cuda_dev)
+    w[3] = 3e38
+    x[:, 3], res[:, 3] = 4.0, 4.0
+    q, _, s = pkg.norm.launch_add_norm(x, res, w, EPS, quant=quant)
+    assert bool(s[:, 0].isinf().all()) and bool(q[:, 3].float().isnan().all())
+    near = q[:, :128].float()
+    near[:, 3] = 0
+    assert not near.any()
+    for big in (1e-30, 1e-13, 1e-12, 3e36, 3e37):
+        v = rnd(256, device=cuda_dev).sign() * big
+        y, _ = pkg.norm.launch_add_norm(x[:, :], None, v, EPS)
+        q, _, s = pkg.norm.launch_add_norm(x, None, v, EPS, quant=quant)
+        per = y.unflatten(1, (s.shape[1], -1))
+        assert torch.equal(s, _scale_of(per)) and torch.equal(q.float(), _e4m3_of(per, s).flatten(1))
