@@ -882,6 +882,9 @@ extern "C" int gdn_gated_norm_backward_launch(const GdnGatedNormArgs* a, const G
         !aligned(workspace, 16))
         return GDN_ERR_WORKSPACE;
     if (int rc = check_device()) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->tokens == 0)  // no head to read, not even one that does not count
+        return cudaMemsetAsync(g->d_weight, 0, a->head_dim * sizeof(float), s) == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
     p.vec = p.vec && rows_vec(g->d_output, g->d_output_stride * es) && aligned(g->dx, 16) && aligned(g->dz, 16);
     GatedNormGradParams d;
     d.dy = g->d_output;
@@ -889,7 +892,6 @@ extern "C" int gdn_gated_norm_backward_launch(const GdnGatedNormArgs* a, const G
     d.dx = g->dx;
     d.dz = g->dz;
     d.part = static_cast<float*>(workspace);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e =
         a->dtype == GDN_DTYPE_F32   ? launch_gated_norm_backward<float>(p, d, a->head_dim, g->d_weight, s)
         : a->dtype == GDN_DTYPE_F16 ? launch_gated_norm_backward<__half>(p, d, a->head_dim, g->d_weight, s)

@@ -558,3 +558,22 @@ def test_codes_beside_an_infinite_output(pkg, cuda_dev, quant):
         q, _, s = pkg.norm.launch_add_norm(x, None, v, EPS, quant=quant)
         per = y.unflatten(1, (s.shape[1], -1))
         assert torch.equal(s, _scale_of(per)) and torch.equal(q.float(), _e4m3_of(per, s).flatten(1))
+
+
+@gpu
+@pytest.mark.parametrize("off", [0, 1])
+def test_norms_of_nothing(pkg, cuda_dev, off):
+    """No tokens or rows, with weights on a 16-byte boundary and off it: zeros, and nothing is read."""
+    n, w = pkg.norm, torch.ones(129, device=cuda_dev)[off:off + 128]
+    e = torch.empty(0, 3, 128, dtype=torch.bfloat16, device=cuda_dev)
+    dx, dz, dw = n.launch_gated_norm_backward(e, e, e, w, EPS)
+    assert dx.shape == dz.shape == e.shape and not dw.any()
+    assert n.launch_gated_norm(e, e, w, EPS).shape == e.shape
+    q, s = n.launch_gated_norm(e, e, w, EPS, quant=True)
+    assert q.shape == e.shape and s.shape == (0, 3)
+    r = e[:, 0]
+    dx, dw = n.launch_add_norm_backward(r, r, w, EPS, d_new_residual=r)
+    assert dx.shape == r.shape and not dw.any()
+    for quant in (None, "row", "group"):
+        assert n.launch_add_norm(r, r, w, EPS, quant=quant)[0].shape == r.shape
+    assert pkg.prefill.device_status(cuda_dev) == 0
