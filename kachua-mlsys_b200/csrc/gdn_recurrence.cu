@@ -192,6 +192,26 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// A bounded wait of the whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, tc05::mbar_wait(bar, parity));
+}
+// The last thing every thread of a scan does, also one that gave up a wait: no
+// CTA's shared memory goes while a CTA of its cluster can still send to it.
+// Where no wait ran out, all that was sent to this CTA has arrived, because it
+// waited for it; a warp that gave up stays for what is still on its way (sent
+// before the barrier, and under a microsecond from arriving).
+__device__ __forceinline__ void leave_cluster(bool gave_up) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (gave_up) {
+        record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+        constexpr uint64_t kStayNs = 100000;
+        const uint64_t t0 = tc05::globaltimer_ns();
+        for (uint32_t i = 0; i < tc05::kWaitMaxPolls && tc05::globaltimer_ns() - t0 < kStayNs; ++i) {}
+    }
+}
 // 16 bytes into the same shared address of CTA `rank` of the cluster, counted
 // by that CTA's mbarrier at the address of `bar`: neither side needs a fence.
 __device__ __forceinline__ void st_cluster_f4(uint32_t a, uint32_t bar, uint32_t rank, float4 v) {
@@ -570,11 +590,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     scan_empty_sequences(p, p.state, p.new_state, c0, c0 + me.kChannels, rank * blockDim.x + threadIdx.x, R * blockDim.x);
     cluster_wait();  // every CTA of the cluster runs and has its barriers
 
+    bool gave_up = false;
     if (warp == W) {
         F2 carry = splat2(0.0f);
         for (int k = 0; k < steps; ++k) {
             const int buf = k & 1, phase = k >> 1 & 1;
-            if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if ((gave_up = !warp_wait(full + 8 * buf, phase))) break;
             const float4* last = maps + (buf * kRows + kPiece - 1) * 32;  // a piece's whole map is its last token's
             float4* before = befores + buf * W * 32;
             F2 A = splat2(1.0f), H = splat2(0.0f);
@@ -605,7 +626,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
             // CTA's map of tile k + 1, sent after that CTA had read tile k's.
             for (int r = 0; r < R; ++r)
                 st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
-            if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if ((gave_up = !warp_wait(arrived + 8 * buf, phase))) break;
             if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
             const float4* all = ranks + buf * R * 32 + lane;
             F2 in = carry;
@@ -627,111 +648,111 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
                 if (ok1) p.ckpt[c + 1] = 0.0f;
             }
         }
-        return;
-    }
-
-    Spans span = {0, 0, 0, 0, 0};
-    uint32_t ends = 0;  // of the tile before
-    for (int k = 0; k <= steps; ++k) {
-        if (k < steps) {
-            const int w0 = (k * R + rank) * kTile + warp * kSpan, buf = k & 1;
-            token_spans<kSpan>(offsets, tokens, w0, span);
-            const uint32_t special = span.start | (~span.covered & kAllTokens<kSpan>);
-            float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
-            F2 A = splat2(1.0f), H = splat2(0.0f);  // the map up to each token
+    } else {
+        Spans span = {0, 0, 0, 0, 0};
+        uint32_t ends = 0;  // of the tile before
+        for (int k = 0; k <= steps; ++k) {
+            if (k < steps) {
+                const int w0 = (k * R + rank) * kTile + warp * kSpan, buf = k & 1;
+                token_spans<kSpan>(offsets, tokens, w0, span);
+                const uint32_t special = span.start | (~span.covered & kAllTokens<kSpan>);
+                float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
+                F2 A = splat2(1.0f), H = splat2(0.0f);  // the map up to each token
 #pragma unroll
-            for (int i = 0; i < kPiece; i += kBatch) {
-                F2 z[kBatch], u[kBatch];
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    z[j] = add2(raw_to_f2<T>(a[i + j]), dtb);
-                    u[j] = mul2(sigmoid2(raw_to_f2<T>(b[i + j])), raw_to_f2<T>(x[i + j]));
-                }
-                fetch(k + 1, i);
-                decays(z, rate);
-                auto put = [&](int j) {
-                    const float2 va = unpack2(A), vh = unpack2(H);
-                    m[(i + j) * 32] = make_float4(va.x, va.y, vh.x, vh.y);
-                };
-                if (special == 0) {
+                for (int i = 0; i < kPiece; i += kBatch) {
+                    F2 z[kBatch], u[kBatch];
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
-                        A = mul2(A, z[j]);
-                        H = fma2(z[j], H, u[j]);
-                        put(j);
+                        z[j] = add2(raw_to_f2<T>(a[i + j]), dtb);
+                        u[j] = mul2(sigmoid2(raw_to_f2<T>(b[i + j])), raw_to_f2<T>(x[i + j]));
                     }
-                } else {  // g and u for now
+                    fetch(k + 1, i);
+                    decays(z, rate);
+                    auto put = [&](int j) {
+                        const float2 va = unpack2(A), vh = unpack2(H);
+                        m[(i + j) * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                    };
+                    if (special == 0) {
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const float2 vg = unpack2(z[j]), vu = unpack2(u[j]);
-                        m[(i + j) * 32] = make_float4(vg.x, vg.y, vu.x, vu.y);
+                        for (int j = 0; j < kBatch; ++j) {
+                            A = mul2(A, z[j]);
+                            H = fma2(z[j], H, u[j]);
+                            put(j);
+                        }
+                    } else {  // g and u for now
+#pragma unroll
+                        for (int j = 0; j < kBatch; ++j) {
+                            const float2 vg = unpack2(z[j]), vu = unpack2(u[j]);
+                            m[(i + j) * 32] = make_float4(vg.x, vg.y, vu.x, vu.y);
+                        }
                     }
                 }
-            }
-            if (special) {
-                const uint32_t fresh = special >> me.strip * kPiece, covered = span.covered >> me.strip * kPiece;
-                A = splat2(1.0f);
-                H = splat2(0.0f);
+                if (special) {
+                    const uint32_t fresh = special >> me.strip * kPiece, covered = span.covered >> me.strip * kPiece;
+                    A = splat2(1.0f);
+                    H = splat2(0.0f);
 #pragma unroll 1
-                for (int j = 0; j < kPiece; ++j) {
-                    const float4 gu = m[j * 32];
-                    const F2 g = pack2(gu.x, gu.y), u = pack2(gu.z, gu.w);
-                    const F2 before = state_of_strips<STRIPS>(offsets, p.state, p.channels, span.start >> j, kPiece, w0 + j, c,
-                                                              me.strip, H);
-                    A = fresh >> j & 1 ? splat2(-0.0f) : mul2(A, g);
-                    H = covered >> j & 1 ? fma2(g, before, u) : splat2(0.0f);
-                    const float2 va = unpack2(A), vh = unpack2(H);
-                    m[j * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                    for (int j = 0; j < kPiece; ++j) {
+                        const float4 gu = m[j * 32];
+                        const F2 g = pack2(gu.x, gu.y), u = pack2(gu.z, gu.w);
+                        const F2 before = state_of_strips<STRIPS>(offsets, p.state, p.channels, span.start >> j, kPiece, w0 + j, c,
+                                                                  me.strip, H);
+                        A = fresh >> j & 1 ? splat2(-0.0f) : mul2(A, g);
+                        H = covered >> j & 1 ? fma2(g, before, u) : splat2(0.0f);
+                        const float2 va = unpack2(A), vh = unpack2(H);
+                        m[j * 32] = make_float4(va.x, va.y, vh.x, vh.y);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
+            }
+            if (k > 0) {
+                const int buf = (k - 1) & 1, w0 = ((k - 1) * R + rank) * kTile + warp * kSpan, t0 = w0 + me.strip * kPiece;
+                if ((gave_up = !warp_wait(ready + 8 * buf, (k - 1) >> 1 & 1))) break;
+                const float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
+                const float4 before = befores[(buf * W + warp) * 32 + lane];
+                const F2 tile_in = s_in[buf][lane];
+                F2 in = apply_map(before, tile_in), h[kPiece];
+                const bool finite = !__any_sync(0xffffffffu, !all_finite(tile_in) || !all_finite(in));
+                if (finite) {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) h[j] = apply_map(m[j * 32], in);
+                } else {
+                    in = apply_map_select(before, tile_in);
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
+                }
+                // the piece's token whose state is the next checkpoint, if it has one
+                const int kept = kScanCkpt - 1 - t0 % kScanCkpt;
+                if (p.ckpt && kept < kPiece && t0 + kept + 1 < tokens) {
+                    F2 v = h[0];
+#pragma unroll
+                    for (int j = 1; j < kPiece; ++j)
+                        if (j == kept) v = h[j];
+                    float* ck = p.ckpt + static_cast<int64_t>((t0 + kept + 1) / kScanCkpt) * p.channels + c;
+                    if (ok0) ck[0] = unpack2(v).x;
+                    if (ok1) ck[1] = unpack2(v).y;
+                }
+                T* out = row_at<T>(out0, t0, p.out_stride);
+                if (w0 + kSpan <= tokens && p.out_pairs && all_channels) {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) store_pair(row_at<T>(out, j, p.out_stride), h[j], true, true, true);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j)
+                        if (t0 + j < tokens) store_pair(row_at<T>(out, j, p.out_stride), h[j], p.out_pairs, ok0, ok1);
+                }
+#pragma unroll 1
+                for (uint32_t left = ends; left; left &= left - 1) {  // sequences that end here
+                    const int t = __ffs(left) - 1;
+                    store_state_of_strip(offsets, p.new_state, p.channels, w0 + t, c, me.strip == t / kPiece,
+                                         apply_map_select(m[t % kPiece * 32], in));
                 }
             }
-            __syncwarp();
-            if (lane == 0) tc05::mbar_arrive(full + 8 * buf);
+            ends = span.end;
         }
-        if (k > 0) {
-            const int buf = (k - 1) & 1, w0 = ((k - 1) * R + rank) * kTile + warp * kSpan, t0 = w0 + me.strip * kPiece;
-            if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-            const float4* m = maps + (buf * kRows + warp * kPiece) * 32 + lane;
-            const float4 before = befores[(buf * W + warp) * 32 + lane];
-            const F2 tile_in = s_in[buf][lane];
-            F2 in = apply_map(before, tile_in), h[kPiece];
-            const bool finite = !__any_sync(0xffffffffu, !all_finite(tile_in) || !all_finite(in));
-            if (finite) {
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) h[j] = apply_map(m[j * 32], in);
-            } else {
-                in = apply_map_select(before, tile_in);
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) h[j] = apply_map_select(m[j * 32], in);
-            }
-            // the piece's token whose state is the next checkpoint, if it has one
-            const int kept = kScanCkpt - 1 - t0 % kScanCkpt;
-            if (p.ckpt && kept < kPiece && t0 + kept + 1 < tokens) {
-                F2 v = h[0];
-#pragma unroll
-                for (int j = 1; j < kPiece; ++j)
-                    if (j == kept) v = h[j];
-                float* ck = p.ckpt + static_cast<int64_t>((t0 + kept + 1) / kScanCkpt) * p.channels + c;
-                if (ok0) ck[0] = unpack2(v).x;
-                if (ok1) ck[1] = unpack2(v).y;
-            }
-            T* out = row_at<T>(out0, t0, p.out_stride);
-            if (w0 + kSpan <= tokens && p.out_pairs && all_channels) {
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) store_pair(row_at<T>(out, j, p.out_stride), h[j], true, true, true);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j)
-                    if (t0 + j < tokens) store_pair(row_at<T>(out, j, p.out_stride), h[j], p.out_pairs, ok0, ok1);
-            }
-#pragma unroll 1
-            for (uint32_t left = ends; left; left &= left - 1) {  // sequences that end here
-                const int t = __ffs(left) - 1;
-                store_state_of_strip(offsets, p.new_state, p.channels, w0 + t, c, me.strip == t / kPiece,
-                                     apply_map_select(m[t % kPiece * 32], in));
-            }
-        }
-        ends = span.end;
     }
+    leave_cluster(gave_up);
 }
 
 // What the gates of a backward tile gave, per token and lane: log2 g, beta,
@@ -832,6 +853,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
     auto tile_start = [&](int k) { return (tiles - 1 - (k * R + rank)) * kTile; };
 
     F2 sum_A = splat2(0.0f), sum_dt = splat2(0.0f);
+    bool gave_up = false;
     if (warp == W) {
         F2 carry = splat2(0.0f);
         auto checkpoint = [&](int k) {
@@ -845,7 +867,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
             const int buf = k & 1, phase = k >> 1 & 1;
             const F2 state_in = state;
             state = checkpoint(k + 1);
-            if (!tc05::mbar_wait(full + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if ((gave_up = !warp_wait(full + 8 * buf, phase))) break;
             // In place: a piece's map makes way for what comes before it (a lane's
             // words are its own).
             auto chain = [&](float4* m, int step) {  // a word every `step`
@@ -887,7 +909,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
             for (int r = 0; r < R; ++r)
                 st_cluster_f4(to, arrived + 8 * buf, r, make_float4(va.x, va.y, vh.x, vh.y));
             if (STRIPS == 1) chain(first_state, me.kLanes);
-            if (!tc05::mbar_wait(arrived + 8 * buf, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if ((gave_up = !warp_wait(arrived + 8 * buf, phase))) break;
             if (lane == 0) tc05::mbar_expect_tx(arrived + 8 * buf, R * 512);
             const float4* every = ranks + buf * R * 32 + lane;
             F2 in = carry;
@@ -1009,7 +1031,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
             }
             if (k > 0 && tile_start(k - 1) >= 0) {
                 const int buf = (k - 1) & 1, w0 = tile_start(k - 1) + warp * kSpan, t0 = w0 + me.strip * kPiece;
-                if (!tc05::mbar_wait(ready + 8 * buf, (k - 1) >> 1 & 1)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+                if ((gave_up = !warp_wait(ready + 8 * buf, (k - 1) >> 1 & 1))) break;
                 const float4 ends = s_ends[buf][lane];
                 const F2 tile_h = pack2(ends.x, ends.y), tile_e = pack2(ends.z, ends.w);
                 const float4 hm = state_maps[(buf * W + warp) * 32 + lane], em = grad_maps[(buf * W + warp) * 32 + lane];
@@ -1108,7 +1130,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
     float4* sums = state_maps + lane;  // nobody reads the maps any more
     if (warp < W) sums[warp * 32] = part;
     __syncthreads();
-    if (warp != 0) return;
     auto add_up = [](const float4* v, int n) {
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int i = 0; i < n; ++i) {
@@ -1117,14 +1138,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
         }
         return s;
     };
-    st_cluster_f4(tc05::smem_u32(cta_sums + rank * 32 + lane), summed, 0, add_up(sums, W));
-    if (rank != 0) return;
-    if (!tc05::mbar_wait(summed, 0)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
-    const float4 s = add_up(cta_sums + lane, R);
-    if (me.strip != 0) return;
-    constexpr float kLn2 = 0.6931471805599453f;  // l = ln 2 log2 g
-    if (ok0) d.dA_log[c] = s.x * kLn2, d.ddt_bias[c] = s.z;
-    if (ok1) d.dA_log[c + 1] = s.y * kLn2, d.ddt_bias[c + 1] = s.w;
+    if (warp == 0) st_cluster_f4(tc05::smem_u32(cta_sums + rank * 32 + lane), summed, 0, add_up(sums, W));
+    if (warp == 0 && rank == 0) {
+        if (warp_wait(summed, 0)) {
+            const float4 s = add_up(cta_sums + lane, R);
+            constexpr float kLn2 = 0.6931471805599453f;  // l = ln 2 log2 g
+            if (me.strip == 0 && ok0) d.dA_log[c] = s.x * kLn2, d.ddt_bias[c] = s.z;
+            if (me.strip == 0 && ok1) d.dA_log[c + 1] = s.y * kLn2, d.ddt_bias[c + 1] = s.w;
+        } else {
+            gave_up = true;
+        }
+    }
+    leave_cluster(gave_up);
 }
 
 // One or a few tokens per sequence, V channels of one sequence per thread (4

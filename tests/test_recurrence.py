@@ -547,3 +547,35 @@ def test_bounds_follow_fp32(pkg):
     ref.close(h, *want["new_state"], "new_state")
     with pytest.raises(AssertionError):
         ref.close(y * (1 + 1e-4), *want["y"], "y")
+
+
+# --------------------------------------------------------- leaving a cluster --
+def _kernel_bodies(source):
+    """Bodies of the __global__ functions that use distributed shared memory, by name."""
+    out, at = {}, 0
+    while (at := source.find("__global__", at)) >= 0:
+        open_ = source.index("{", at)
+        depth, end = 1, open_ + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(source[end], 0)
+            end += 1
+        body = source[open_ + 1:end - 1]
+        if "st_cluster_f4" in body:
+            out[source[at:open_].split("(")[-2].split()[-1]] = body
+        at = end
+    return out
+
+
+def test_scans_leave_their_cluster_together(pkg):
+    """A wait that runs out is not forced on a GPU; that its CTA stays for its peers is held here.  No thread of a scan
+    ends but behind the cluster's barrier, the kernel's last statement, and every wait answers for its whole warp."""
+    source = (pkg._build.CSRC / "gdn_recurrence.cu").read_text()
+    bodies = _kernel_bodies(source)
+    assert set(bodies) == {"gdn_scan_kernel", "gdn_scan_backward_kernel"}
+    for name, body in bodies.items():
+        assert body.rstrip().endswith("leave_cluster(gave_up);") and body.count("leave_cluster") == 1, name
+        assert "return;" not in body and "return record_status" not in body, name
+        assert "mbar_wait" not in body and body.count("warp_wait(") == body.count("gave_up = !warp_wait(") + body.count("if (warp_wait("), name
+    leave = source[source.index("void leave_cluster"):]
+    leave = leave[:leave.index("\n}\n")]
+    assert leave.index("cluster_arrive") < leave.index("cluster_wait") < leave.index("record_status")
