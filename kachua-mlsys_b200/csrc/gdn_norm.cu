@@ -399,7 +399,14 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : kNormThreads) gdn_add_norm_b
         const T* dr = static_cast<const T*>(d.dr) + (d.dr ? row * d.dr_stride : 0);
         const T *ex = x, *edy = dy, *edr = dr;  // for the end of the last row
         if (MODE != kApart && p.stages > 0) {
-            if (!tc05::mbar_wait(bar + 8 * stage, phase)) return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            if (!tc05::mbar_wait(bar + 8 * stage, phase)) {
+                // the copies under way land (bounded again) before the shared memory goes
+                for (int i = 0; i < p.stages && row + static_cast<int64_t>(i) * gridDim.x < p.rows; ++i) {
+                    const int at = (stage + i) % p.stages;
+                    tc05::mbar_wait(bar + 8 * at, phase ^ (at < stage));
+                }
+                return record_status(32 /* GDN_ERR_DEVICE_TIMEOUT */);
+            }
             x = reinterpret_cast<const T*>(smem) + stage * 3 * slot_max + m;
             dy = x + slot_max;
             dr = dy + slot_max;

@@ -577,3 +577,23 @@ def test_norms_of_nothing(pkg, cuda_dev, off):
     for quant in (None, "row", "group"):
         assert n.launch_add_norm(r, r, w, EPS, quant=quant)[0].shape == r.shape
     assert pkg.prefill.device_status(cuda_dev) == 0
+
+
+def test_backward_waits_for_its_copies(pkg):
+    """A wait that runs out is not forced on a GPU; that the kernel then waits for every copy under way is held here:
+    the stage and phase that it waits for, for the rows that were asked for, are those of the main loop."""
+    source = (pkg._build.CSRC / "gdn_norm.cu").read_text()
+    body = source[source.index("gdn_add_norm_backward_kernel(const NormParams p"):]
+    body = body[:body.index("\n}\n")]
+    give_up = body[body.index("if (!tc05::mbar_wait(bar + 8 * stage, phase)) {"):body.index("return record_status")]
+    assert "(stage + i) % p.stages" in give_up and "phase ^ (at < stage)" in give_up and "< p.rows" in give_up
+    for stages in (2, 3):
+        for first in range(8):  # rows `first` .. of this block: the main loop's stage and phase of each
+            stage, phase, seen = 0, 0, []
+            for _ in range(first + stages):
+                seen.append((stage, phase))
+                stage = 0 if stage + 1 == stages else stage + 1
+                phase ^= stage == 0
+            at, ph = seen[first]
+            want = seen[first:first + stages]
+            assert [((at + i) % stages, ph ^ ((at + i) % stages < at)) for i in range(stages)] == want
