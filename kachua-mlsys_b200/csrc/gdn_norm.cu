@@ -669,15 +669,18 @@ static cudaError_t launch_add_norm_backward(NormParams p, const NormGradParams& 
     // Rows in flight for about 200 KB of an SM's shared memory over its CTAs;
     // fewer than two would not run ahead, and rows at any alignment cannot be
     // copied in bulk (65536 x 4096: 407 us, 536 without).
+    constexpr int kBudget = 200 << 10;
     const int per_sm = (grid + kSmCount - 1) / kSmCount;
     const size_t stage = 3 * 8 * static_cast<size_t>(row_vecs(p.width, p.mode)) * sizeof(T);
-    const int fit = static_cast<int>((200 << 10) / per_sm / stage);
+    const int fit = static_cast<int>(kBudget / per_sm / stage);
     p.stages = p.mode == kApart || fit < 2 ? 0 : fit < kNormStages ? fit : kNormStages;
     const int smem = static_cast<int>(p.stages * stage);
     cudaError_t e = cudaSuccess;
     with_row_shape(r.vpt, p.mode, [&](auto vpt, auto mode) {
         const auto kernel = gdn_add_norm_backward_kernel<T, vpt(), mode()>;
-        if (smem > (40 << 10)) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        // The limit belongs to the kernel, not to the call: one value for all
+        // widths, or another thread's call could lower it before this launch.
+        if (smem > (40 << 10)) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget);
         if (e == cudaSuccess) kernel<<<grid, r.threads, smem, s>>>(p, d);
     });
     if (e == cudaSuccess) e = cudaGetLastError();

@@ -1,5 +1,7 @@
 """The residual and the gated RMS norm against their definitions in 64 bits."""
 import ctypes
+import sys
+import threading
 
 import pytest
 import torch
@@ -597,3 +599,50 @@ def test_backward_waits_for_its_copies(pkg):
             at, ph = seen[first]
             want = seen[first:first + stages]
             assert [((at + i) % stages, ph ^ ((at + i) % stages < at)) for i in range(stages)] == want
+
+
+@gpu
+def test_backward_from_four_threads(pkg, cuda_dev):
+    """Host threads with a stream each, at two widths whose rows take different amounts of one kernel's shared memory;
+    then both widths in one graph.  Packed arguments, so that the threads spend their time inside the library."""
+    lib, C, rows = pkg._capi.load(), pkg._capi, 8
+    refused, calls, results = [], [], []
+    for k, width in enumerate((4096, 8192, 4096, 8192)):
+        x, _, w = make(rows, width, torch.bfloat16, cuda_dev, seed=k)
+        dy = rnd(rows, width, dtype=torch.bfloat16, device=cuda_dev, seed=8)
+        need = int(lib.gdn_add_norm_backward_workspace_size(rows, width))
+        t = [x, dy, w, torch.empty_like(x), torch.empty_like(w), torch.empty(need, dtype=torch.uint8, device=cuda_dev),
+             torch.cuda.Stream(cuda_dev)]
+        args = pkg.norm._pack_add(x.data_ptr(), 0, width, 0, w.data_ptr(), C.DTYPE_F32, C.DTYPE_BF16, 0, EPS, rows, width, 0, 0, 0)
+        grads = pkg.norm._pack_grad(dy.data_ptr(), width, 0, 0, t[3].data_ptr(), 0, t[4].data_ptr())
+        calls.append((args, grads, t[5].data_ptr(), need, t[6].cuda_stream))
+        results.append(t)
+    torch.cuda.synchronize()
+
+    def work(call):
+        torch.cuda.set_device(cuda_dev)
+        refused.extend(rc for rc in (lib.gdn_add_norm_backward_launch(*call) for _ in range(10000)) if rc)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    torch.cuda.synchronize()
+    assert not refused
+    for x, dy, w, dx, dw, *_ in results:
+        want_dx, want_dw = ref.add_norm(None, None, w, EPS, dy=dy, summed=x)
+        ref.close(dx, *want_dx, "dx")
+        ref.close(dw, *want_dw, "dweight")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = [pkg.norm.launch_add_norm_backward(t[1], t[0], t[2], EPS) for t in results[:2]]
+    g.replay()
+    torch.cuda.synchronize()
+    for (dx, dw), t in zip(captured, results):
+        assert torch.equal(dx, t[3]) and torch.equal(dw, t[4])
