@@ -398,7 +398,7 @@ __device__ __noinline__ Spans find_spans(Offsets o, int64_t tokens, int64_t t, i
     Spans s = {0, 0, 0, 0, 0};
     const int64_t stop = t + width < tokens ? t + width : tokens;
     if (t >= stop) return s;
-    for (int n = seq_of_token(o, t); n < o.seqs; n += 32) {
+    for (int n = seq_of_token(o, t); n < o.seqs;) {
         int64_t b = stop, e = stop;
         if (n + lane < o.seqs) b = o.at(n + lane), e = o.at(n + lane + 1);
         uint32_t st = 0, en = 0, cov = 0;
@@ -415,7 +415,12 @@ __device__ __noinline__ Spans find_spans(Offsets o, int64_t tokens, int64_t t, i
         s.covered |= __reduce_or_sync(0xffffffffu, cov);
         s.lo = max(s.lo, __reduce_max_sync(0xffffffffu, lo));
         s.hi = max(s.hi, __reduce_max_sync(0xffffffffu, hi));
-        if (__shfl_sync(0xffffffffu, b, 31) >= stop) break;
+        const int64_t last = __shfl_sync(0xffffffffu, b, 31);
+        if (last >= stop) break;
+        // On behind the 32, and behind all that are empty where the last of them
+        // begins: any number of those can lie at one token, and the other warps'
+        // waits are bounded.  So two searches a token at most.
+        n = max(n + 32, seq_of_token(o, last));
     }
     return s;
 }

@@ -1,4 +1,5 @@
 """The per-channel gated recurrence against its definition in 64 bits."""
+import bisect
 import ctypes
 
 import pytest
@@ -579,3 +580,72 @@ def test_scans_leave_their_cluster_together(pkg):
     leave = source[source.index("void leave_cluster"):]
     leave = leave[:leave.index("\n}\n")]
     assert leave.index("cluster_arrive") < leave.index("cluster_wait") < leave.index("record_status")
+
+
+# ---------------------------------------------- many empty sequences in a row --
+def _walk(ends, t, width, tokens):
+    """The warp's walk over the sequences of one piece (find_spans), in its order: starts, ends, covered, steps."""
+    starts, seqs, stop = [0] + ends[:-1], len(ends), min(t + width, tokens)
+    start = end = covered = steps = 0
+    n = bisect.bisect_right(ends, t)
+    while n < seqs:
+        steps += 1
+        for k in range(n, min(n + 32, seqs)):
+            b, e = starts[k], ends[k]
+            if e > b and b < stop and e > t:
+                start |= (b >= t) << max(b - t, 0)
+                end |= (e <= stop) << max(min(e, stop) - 1 - t, 0)
+                for j in range(max(b, t), min(e, stop)):
+                    covered |= 1 << (j - t)
+        last = starts[n + 31] if n + 31 < seqs else stop
+        if last >= stop:
+            break
+        n = max(n + 32, bisect.bisect_right(ends, last))
+    return start, end, covered, steps
+
+
+@pytest.mark.parametrize("width", [4, 8, 16])
+def test_walk_over_empty_sequences(pkg, width):
+    """The walk's steps are bounded by the piece's tokens, not by the sequences; nothing is missed."""
+    gen = torch.Generator().manual_seed(0)
+    for case in range(40):
+        lens = torch.randint(0, 3 + case % 5, (60,), generator=gen).tolist()
+        for k in torch.randint(0, 60, (4,), generator=gen).tolist():
+            lens[k:k] = [0] * int(torch.randint(0, 3000, (1,), generator=gen))
+        ends = torch.tensor(lens).cumsum(0).tolist()
+        tokens = ends[-1] + case % 3
+        first = {b for b, n in zip([0] + ends[:-1], lens) if n}
+        last = {e - 1 for e, n in zip(ends, lens) if n}
+        for t in range(0, tokens, width):
+            start, end, covered, steps = _walk(ends, t, width, tokens)
+            live = range(min(width, tokens - t))
+            assert start == sum(1 << j for j in live if t + j in first)
+            assert end == sum(1 << j for j in live if t + j in last)
+            assert covered == sum(1 << j for j in live if t + j < ends[-1])
+            assert steps <= width + 1
+
+
+@gpu
+@pytest.mark.parametrize("N", [900, 400_000])
+def test_scan_of_many_empty_sequences(pkg, cuda_dev, N):
+    """Offsets that repeat in the middle of a tile, with and without tokens of other sequences beside them: the bits of
+    the call without them, and their state rows passed on."""
+    C, gen = 24, torch.Generator().manual_seed(1)
+    i = make([101, 3, 1, 140], C, torch.bfloat16, cuda_dev)
+    at = [1, N // 3, N // 2 + 40, N + 3]  # where the four stand among the empty ones
+    lens = torch.zeros(N + 4, dtype=torch.int64)
+    lens[at] = torch.tensor(i["lens"])
+    state, dns = (torch.randn(N + 4, C, generator=gen).to(cuda_dev) for _ in range(2))
+    state[at], dns[at] = i["state"], i["dns"]
+    j = {**i, "cu": torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).to(cuda_dev), "state": state, "dns": dns}
+    for a, b in zip(check_forward(pkg, i), pkg.recurrence.launch_scan(*gates(j), j["cu"], j["state"])):
+        assert torch.equal(a, b if a.shape == b.shape else b[at])
+    ns = pkg.recurrence.launch_scan(*gates(j), j["cu"], j["state"])[1]
+    empty = torch.ones(N + 4, dtype=torch.bool, device=cuda_dev)
+    empty[at] = False
+    assert torch.equal(ns[empty], state[empty])
+    want, got = backward(pkg, i), backward(pkg, j)
+    for a, b in zip(want[:5], got[:5]):
+        assert torch.equal(a, b)
+    assert torch.equal(got[5][at], want[5]) and torch.equal(got[5][empty], dns[empty])
+    assert pkg.prefill.device_status(cuda_dev) == 0
