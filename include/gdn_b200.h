@@ -54,6 +54,7 @@ typedef enum gdn_status_t {
     GDN_ERR_CUDA = 5,              /* a CUDA runtime call failed */
     GDN_ERR_BAD_DTYPE = 6,         /* unsupported dtype code */
     GDN_ERR_NO_DEVICE = 7,         /* no usable sm_100 device is current */
+    GDN_ERR_OVERLAP = 8,           /* an output shares memory with an input or another output */
     GDN_ERR_DEVICE_BAD_SEQLENS = 16,  /* device status bit: cu_seqlens not monotone / out of range */
     GDN_ERR_DEVICE_TIMEOUT = 32       /* device status bit: a bounded wait expired */
 } gdn_status_t;
@@ -261,6 +262,13 @@ int gdn_prefill_launch_noalloc(const GdnPrefillArgs* args, void* stream);
 
 /* ---------------------------------------------- per-channel recurrence -- */
 
+/* The outputs of a call below, its workspace among them, share no memory with
+ * each other and none with its inputs, but for an output that is an input
+ * itself, row for row, where that is said (GDN_ERR_OVERLAP).  Column blocks of
+ * one buffer are apart.  Two tensors of different row strides whose rows lie
+ * among each other are taken to meet unless the strides' common divisor keeps
+ * them apart. */
+
 /* Element types of the operators below. */
 #define GDN_DTYPE_BF16 0
 #define GDN_DTYPE_F16 1
@@ -280,7 +288,7 @@ int gdn_prefill_launch_noalloc(const GdnPrefillArgs* args, void* stream);
  *   new_state   fp32 [N, C]
  *   checkpoints fp32 [gdn_scan_checkpoint_rows(T), C] or NULL: what the
  *               backward pass needs of the forward pass
- * The output must not overlap an input.  State and sums are fp32.  An empty
+ * No output may be an input.  State and sums are fp32.  An empty
  * sequence's new_state row is its state row.  Output rows (and gradients) of
  * tokens that belong to no sequence are written as zeros.  No reference
  * counterpart (the reference has the delta rule only). */
@@ -330,7 +338,7 @@ int gdn_scan_backward_launch(const GdnScanArgs* args, const GdnScanGradArgs* gra
 
 /* Decode: `tokens` >= 1 tokens for each of num_seqs sequences, total_tokens =
  * num_seqs * tokens rows in sequence order; cu_seqlens and checkpoints are not
- * read; state is required and may be new_state. */
+ * read; state is required and may be new_state, and x, a or b may be output. */
 int gdn_scan_step_launch(const GdnScanArgs* args, int64_t tokens, void* stream);
 
 /* ----------------------------------------------------------------- norms -- */
@@ -346,7 +354,8 @@ int gdn_scan_step_launch(const GdnScanArgs* args, int64_t tokens, void* stream);
  *   weight      [width], fp32 or `dtype` (weight_dtype)
  *   new_residual [rows, width]: r rounded to `dtype`; may be residual or x itself
  *               (the same rows, contiguous).  The norm is of the unrounded r.
- *   output      [rows, width] of `dtype`, or e4m3 codes
+ *   output      [rows, width] of `dtype` (may be x or residual itself, contiguous),
+ *               or e4m3 codes
  *   scale       fp32 [rows] or [rows, width / 128] (width a multiple of 128):
  *               max(amax |y|, 1e-12) / 448; code = e4m3(y / scale), saturating, of
  *               the fp32 y and quotient (two roundings), by the scale as stored;
@@ -376,7 +385,7 @@ int gdn_add_norm_launch(const GdnAddNormArgs* args, void* stream);
  *   x, z    [tokens, heads, head_dim] of `dtype`, *_stride elements between
  *           tokens, a token's heads contiguous
  *   weight  [head_dim], fp32 or `dtype`
- *   output  contiguous, of `dtype` (may be x itself when x is contiguous) or
+ *   output  contiguous, of `dtype` (may be x or z itself, contiguous) or
  *           e4m3 codes with scale fp32 [tokens, heads] (GDN_QUANT_GROUP) */
 typedef struct GdnGatedNormArgs {
     const void* x;
@@ -400,7 +409,7 @@ int gdn_gated_norm_launch(const GdnGatedNormArgs* args, void* stream);
  * of x; dx (and dz of the gated norm) contiguous, of `dtype`; d_weight fp32.
  * For gdn_add_norm args->x is the stored sum (new_residual), residual is not
  * read, and dx -- the gradient of x and of residual alike -- includes
- * d_new_residual (NULL: zero).  Sums are taken in a fixed order: the same
+ * d_new_residual (NULL: zero).  dx and dz may be contiguous inputs.  Sums are taken in a fixed order: the same
  * call gives the same bits.  The workspace (16-byte aligned) is free again
  * when the call's kernels have run; calls that overlap need one each. */
 typedef struct GdnNormGradArgs {

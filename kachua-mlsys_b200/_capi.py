@@ -17,6 +17,7 @@ from . import _build
 GDN_OK = 0
 GDN_SEQLENS_INT32 = 0
 GDN_SEQLENS_INT64 = 1
+GDN_ERR_OVERLAP = 8
 GDN_ERR_DEVICE_BAD_SEQLENS = 16
 GDN_ERR_DEVICE_TIMEOUT = 32
 

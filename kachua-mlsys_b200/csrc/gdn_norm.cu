@@ -799,6 +799,24 @@ static int gated_norm_setup(const GdnGatedNormArgs* a, GatedNormParams& p) {
     p.scale = a->scale;
     return GDN_OK;
 }
+
+// What the entry points of the two norms read.
+static Operands add_norm_inputs(const GdnAddNormArgs* a) {
+    const int64_t es = static_cast<int64_t>(dtype_bytes(a->dtype)), row = a->width * es;
+    Operands o;
+    o.read(a->x, a->rows, a->x_stride * es, row);
+    o.read(a->residual, a->rows, a->residual_stride * es, row);
+    o.read(a->weight, 1, 0, a->width * static_cast<int64_t>(dtype_bytes(a->weight_dtype)));
+    return o;
+}
+static Operands gated_norm_inputs(const GdnGatedNormArgs* a) {
+    const int64_t es = static_cast<int64_t>(dtype_bytes(a->dtype)), row = static_cast<int64_t>(a->heads) * a->head_dim * es;
+    Operands o;
+    o.read(a->x, a->tokens, a->x_stride * es, row);
+    o.read(a->z, a->tokens, a->z_stride * es, row);
+    o.read(a->weight, 1, 0, a->head_dim * static_cast<int64_t>(dtype_bytes(a->weight_dtype)));
+    return o;
+}
 }  // namespace gdn
 
 extern "C" int gdn_add_norm_launch(const GdnAddNormArgs* a, void* stream) {
@@ -806,6 +824,16 @@ extern "C" int gdn_add_norm_launch(const GdnAddNormArgs* a, void* stream) {
     if (int rc = add_norm_setup(a, p)) return rc;
     if (a->rows > 0 && (!a->output || (a->residual && !a->new_residual) || (a->quant && !a->scale)))
         return GDN_ERR_NULL_POINTER;
+    Operands o = add_norm_inputs(a);
+    const int64_t row = a->width * static_cast<int64_t>(dtype_bytes(a->dtype));
+    if (a->quant) {
+        o.write(a->output, a->rows, a->width, a->width);
+        o.write(a->scale, 1, 0, a->rows * (a->quant == GDN_QUANT_ROW ? 1 : a->width / kQuantGroup) * 4);
+    } else {
+        o.write(a->output, a->rows, row, row, true);
+    }
+    if (a->residual) o.write(a->new_residual, a->rows, row, row, true);
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     if (a->rows == 0) return GDN_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -840,6 +868,14 @@ extern "C" int gdn_add_norm_backward_launch(const GdnAddNormArgs* a, const GdnNo
     if (workspace == nullptr || workspace_bytes < gdn_add_norm_backward_workspace_size(a->rows, a->width) ||
         !aligned(workspace, 16))
         return GDN_ERR_WORKSPACE;
+    Operands o = add_norm_inputs(a);
+    const int64_t size = static_cast<int64_t>(es), row = a->width * size;
+    o.read(g->d_output, a->rows, g->d_output_stride * size, row);
+    o.read(g->d_new_residual, a->rows, g->d_new_residual_stride * size, row);
+    o.write(g->dx, a->rows, row, row, true);
+    o.write(g->d_weight, 1, 0, a->width * 4);
+    o.write(workspace, 1, 0, static_cast<int64_t>(workspace_bytes));
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     const int mode = row_mode(a->width, es, {{g->d_output, g->d_output_stride}, {g->d_new_residual, g->d_new_residual_stride},
                                              {g->dx, a->width}});
@@ -862,6 +898,15 @@ extern "C" int gdn_gated_norm_launch(const GdnGatedNormArgs* a, void* stream) {
     GatedNormParams p;
     if (int rc = gated_norm_setup(a, p)) return rc;
     if (a->tokens > 0 && (!a->output || (a->quant && !a->scale))) return GDN_ERR_NULL_POINTER;
+    Operands o = gated_norm_inputs(a);
+    const int64_t n = static_cast<int64_t>(a->heads) * a->head_dim, row = n * static_cast<int64_t>(dtype_bytes(a->dtype));
+    if (a->quant) {
+        o.write(a->output, a->tokens, n, n);
+        o.write(a->scale, 1, 0, a->tokens * a->heads * 4);
+    } else {
+        o.write(a->output, a->tokens, row, row, true);
+    }
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     if (a->tokens == 0) return GDN_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -891,6 +936,14 @@ extern "C" int gdn_gated_norm_backward_launch(const GdnGatedNormArgs* a, const G
     if (workspace == nullptr || workspace_bytes < gdn_gated_norm_backward_workspace_size(a->tokens, a->heads, a->head_dim) ||
         !aligned(workspace, 16))
         return GDN_ERR_WORKSPACE;
+    Operands o = gated_norm_inputs(a);
+    const int64_t size = static_cast<int64_t>(es), row = width * size;
+    o.read(g->d_output, a->tokens, g->d_output_stride * size, row);
+    o.write(g->dx, a->tokens, row, row, true);
+    o.write(g->dz, a->tokens, row, row, true);
+    o.write(g->d_weight, 1, 0, a->head_dim * 4);
+    o.write(workspace, 1, 0, static_cast<int64_t>(workspace_bytes));
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->tokens == 0)  // no head to read, not even one that does not count

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "gdn_common.cuh"
+#include "gdn_overlap.cuh"
 #include "tc05.cuh"
 
 namespace gdn {
@@ -1358,6 +1359,22 @@ static bool stride_ok(int64_t stride) { return stride >= 0 && stride <= (1 << 29
 // Every row starts on a boundary of two elements, so a pair is one access.
 static bool rows_in_pairs(const void* q, int64_t stride, uintptr_t es) { return aligned(q, 2 * es) && stride % 2 == 0; }
 
+static int64_t checkpoint_rows(int64_t tokens) { return (tokens + kScanCkpt - 1) / kScanCkpt; }
+
+// What the three entry points read.
+static Operands scan_inputs(const GdnScanArgs* a, bool step) {
+    const int64_t es = static_cast<int64_t>(dtype_bytes(a->dtype)), T = a->total_tokens, N = a->num_seqs, C = a->channels;
+    Operands o;
+    o.read(a->x, T, a->x_stride * es, C * es);
+    o.read(a->a, T, a->a_stride * es, C * es);
+    o.read(a->b, T, a->b_stride * es, C * es);
+    o.read(a->A_log, 1, 0, C * 4);
+    o.read(a->dt_bias, 1, 0, C * 4);
+    o.read(a->state, N, C * 4, C * 4);
+    if (!step) o.read(a->cu_seqlens, 1, 0, (N + 1) * (a->cu_seqlens_dtype == GDN_SEQLENS_INT64 ? 8 : 4));
+    return o;
+}
+
 // Argument checks shared by the three entry points, then the kernel parameters.
 static int scan_setup(const GdnScanArgs* a, ScanParams& p, bool step) {
     if (a == nullptr) return GDN_ERR_NULL_POINTER;
@@ -1412,6 +1429,12 @@ extern "C" int gdn_scan_launch(const GdnScanArgs* a, void* stream) {
     if (a->num_seqs > 0 && !a->new_state) return GDN_ERR_NULL_POINTER;
     if (a->total_tokens > 1 && a->output_stride < a->channels) return GDN_ERR_BAD_SIZE;
     if (a->state != nullptr && a->num_seqs > 0 && a->state == a->new_state) return GDN_ERR_BAD_SIZE;
+    Operands o = scan_inputs(a, false);
+    const int64_t es = static_cast<int64_t>(dtype_bytes(a->dtype)), C = a->channels;
+    o.write(a->output, a->total_tokens, a->output_stride * es, C * es);
+    o.write(a->new_state, a->num_seqs, C * 4, C * 4);
+    o.write(a->checkpoints, checkpoint_rows(a->total_tokens), C * 4, C * 4);
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     if (a->num_seqs == 0 && a->total_tokens == 0) return GDN_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1422,7 +1445,7 @@ extern "C" int gdn_scan_launch(const GdnScanArgs* a, void* stream) {
 }
 
 extern "C" int64_t gdn_scan_checkpoint_rows(int64_t total_tokens) {
-    return total_tokens < 0 ? 0 : (total_tokens + kScanCkpt - 1) / kScanCkpt;
+    return total_tokens < 0 ? 0 : checkpoint_rows(total_tokens);
 }
 
 extern "C" int gdn_scan_backward_launch(const GdnScanArgs* a, const GdnScanGradArgs* g, void* stream) {
@@ -1441,6 +1464,18 @@ extern "C" int gdn_scan_backward_launch(const GdnScanArgs* a, const GdnScanGradA
     if (!aligned(g->d_output, es) || !aligned(g->dx, es) || !aligned(g->da, es) || !aligned(g->db, es) ||
         !aligned(g->d_new_state, 4) || !aligned(g->d_state, 4) || !aligned(g->dA_log, 4) || !aligned(g->d_dt_bias, 4))
         return GDN_ERR_MISALIGNED;
+    Operands o = scan_inputs(a, false);
+    const int64_t size = static_cast<int64_t>(es), T = a->total_tokens, N = a->num_seqs, C = a->channels;
+    o.read(g->d_output, T, g->d_output_stride * size, C * size);
+    o.read(g->d_new_state, N, C * 4, C * 4);
+    o.read(a->checkpoints, checkpoint_rows(T), C * 4, C * 4);
+    o.write(g->dx, T, g->dx_stride * size, C * size);
+    o.write(g->da, T, g->da_stride * size, C * size);
+    o.write(g->db, T, g->db_stride * size, C * size);
+    o.write(g->dA_log, 1, 0, C * 4);
+    o.write(g->d_dt_bias, 1, 0, C * 4);
+    o.write(g->d_state, N, C * 4, C * 4);
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     ScanGradParams d;
     d.dy = g->d_output;
@@ -1472,6 +1507,11 @@ extern "C" int gdn_scan_step_launch(const GdnScanArgs* a, int64_t tokens, void* 
     if (a->num_seqs == 0) return check_device();
     if (!a->output || !a->state || !a->new_state) return GDN_ERR_NULL_POINTER;
     if (a->total_tokens > 1 && a->output_stride < a->channels) return GDN_ERR_BAD_SIZE;
+    Operands o = scan_inputs(a, true);
+    const int64_t es = static_cast<int64_t>(dtype_bytes(a->dtype)), C = a->channels;
+    o.write(a->output, a->total_tokens, a->output_stride * es, C * es, true);
+    o.write(a->new_state, a->num_seqs, C * 4, C * 4, true);
+    if (!o.apart()) return GDN_ERR_OVERLAP;
     if (int rc = check_device()) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = a->dtype == GDN_DTYPE_F32   ? launch_scan_step<float>(p, tokens, s)

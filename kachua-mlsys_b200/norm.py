@@ -11,7 +11,9 @@ scale), saturating.  The backward passes and the differentiable ``add_norm``
 and ``gated_norm`` are for training.  Inputs are bf16, fp16 or fp32, all of
 one type, the weight fp32 or that type; statistics and sums are fp32 and every
 output is rounded once.  Everything runs on the current torch stream,
-asynchronously; errors in arguments raise ``ValueError`` before a launch.
+asynchronously; errors in arguments raise ``ValueError`` before a launch.  An
+output of the inputs' type may be a contiguous input itself; no output may
+otherwise share memory with an input or another output.
 """
 from __future__ import annotations
 

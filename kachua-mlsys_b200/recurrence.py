@@ -83,6 +83,8 @@ def _call(fn, what: str, device, *args) -> None:
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
+    if rc == _capi.GDN_ERR_OVERLAP:
+        raise ValueError(f"{what}: an output must not overlap an input or another output")
     if rc:
         _capi.check(rc, what)
 
@@ -184,8 +186,8 @@ def launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None, output=None, ne
     ``new_state``; an empty sequence's ``new_state`` row is its ``state`` row.
     Output rows of tokens that belong to no sequence are zeros.
     ``checkpoints`` (``empty_checkpoints(x)``) is filled for the backward pass.
-    ``output`` may be row-strided (a column block of a wider buffer) and must
-    not overlap an input.
+    ``output`` may be row-strided (a column block of a wider buffer).  No
+    output may share memory with an input or another output.
     """
     T, C, strides = _inputs(x, A_log, a, dt_bias, b, True)
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device != x.device:
@@ -218,7 +220,8 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
     The arguments are those of the forward call and the ``checkpoints`` that it
     filled; ``d_output`` is ``[T, C]`` of ``x``'s type, ``d_new_state`` fp32
     ``[N, C]`` (``None``: zero).  ``dx``, ``da``, ``db`` may be given
-    (row-strided, e.g. column blocks of the projection's gradient); ``dA_log``
+    (row-strided, e.g. column blocks of the projection's gradient) and share no
+    memory with each other or an input; ``dA_log``
     and ``d_dt_bias`` are fp32 ``[C]``, ``d_state`` fp32 ``[N, C]`` (``None``
     when ``state`` is).  Sums are taken in a fixed order: the same call gives
     the same bits.
@@ -259,7 +262,8 @@ def launch_step(x, A_log, a, dt_bias, b, state, output=None, new_state=None):
 
     ``x``, ``a``, ``b`` are ``[B, C]``, or ``[B, T, C]`` for T tokens per
     sequence applied in order; ``state`` is ``[B, C]`` fp32 and may be
-    ``new_state`` (in-place update).
+    ``new_state`` (in-place update), and a contiguous ``x``, ``a`` or ``b``
+    may be ``output``.
     """
     if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3):
         raise ValueError("x must be a [B, C] or [B, T, C] tensor")
