@@ -205,6 +205,13 @@ class GdnError(RuntimeError):
         super().__init__(f"{what}: {status_string(status)} (status {status})")
 
 
+class GdnArgumentError(GdnError, ValueError):
+    """A status that says what is wrong with the call's arguments: nothing was launched."""
+
+
+# NULL_POINTER, BAD_SIZE, MISALIGNED, WORKSPACE, BAD_DTYPE, OVERLAP
+ARGUMENT_ERRORS = (1, 2, 3, 4, 6, GDN_ERR_OVERLAP)
+
 _lib = None
 _lock = threading.Lock()
 
@@ -289,7 +296,7 @@ def status_string(status: int) -> str:
 
 def check(status: int, what: str) -> None:
     if status != GDN_OK:
-        raise GdnError(status, what)
+        raise (GdnArgumentError if status in ARGUMENT_ERRORS else GdnError)(status, what)
 
 
 def read_device_status(stream_handle: int, clear: bool = True) -> int:

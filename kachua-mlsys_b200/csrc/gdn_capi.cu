@@ -49,7 +49,7 @@ extern "C" const char* gdn_status_string(int status) {
         case GDN_ERR_CUDA: return "a CUDA runtime call failed";
         case GDN_ERR_BAD_DTYPE: return "unsupported dtype code";
         case GDN_ERR_NO_DEVICE: return "no usable sm_100 device is current";
-        case GDN_ERR_OVERLAP: return "an output shares memory with an input or another output";
+        case GDN_ERR_OVERLAP: return "an output must not overlap an input or another output";
         case GDN_ERR_DEVICE_BAD_SEQLENS: return "device: cu_seqlens not monotone or out of range";
         case GDN_ERR_DEVICE_TIMEOUT: return "device: a bounded wait expired";
         default: return "unknown status";

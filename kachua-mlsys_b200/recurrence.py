@@ -26,6 +26,8 @@ import torch
 from . import _capi
 
 _pack_scan, _pack_scan_grad = _capi.packer(_capi.GdnScanArgs), _capi.packer(_capi.GdnScanGradArgs)
+# What the kernels' indices hold: elements between tokens, channels, tokens and sequences.
+MAX_STRIDE, MAX_CHANNELS, MAX_ROWS = 1 << 29, 1 << 20, 0x7FFF0000
 DTYPES = {torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16, torch.float32: _capi.DTYPE_F32}
 
 
@@ -58,6 +60,14 @@ def _rows(t, name: str, dtype, rows: int, width: int, device) -> int:
     return stride
 
 
+def _token_rows(t, name: str, dtype, rows: int, width: int, device) -> int:
+    """``_rows`` of a tensor that a scan or a step reads or writes."""
+    stride = _rows(t, name, dtype, rows, width, device)
+    if stride > MAX_STRIDE:
+        raise ValueError(f"{name} must have at most {MAX_STRIDE} elements between tokens, got {stride}")
+    return stride
+
+
 def _dense(t, name: str, dtype, shape, device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != shape:
         _fault(t, name, dtype, shape, device)
@@ -83,8 +93,6 @@ def _call(fn, what: str, device, *args) -> None:
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
-    if rc == _capi.GDN_ERR_OVERLAP:
-        raise ValueError(f"{what}: an output must not overlap an input or another output")
     if rc:
         _capi.check(rc, what)
 
@@ -103,17 +111,20 @@ def _inputs(x, A_log, a, dt_bias, b, require_cuda: bool):
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if dtype not in DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {dtype}")
-    if C < 1:
-        raise ValueError("x must have at least one channel")
+    if not 1 <= C <= MAX_CHANNELS:
+        raise ValueError(f"x must have 1 to {MAX_CHANNELS} channels, got {C}")
+    if T > MAX_ROWS:
+        raise ValueError(f"x must have at most {MAX_ROWS} tokens, got {T}")
     layout = x.stride()
-    stride = layout[0] if T > 1 and layout[1] == 1 and layout[0] >= C else _rows(x, "x", dtype, T, C, dev)
+    stride = (layout[0] if T > 1 and layout[1] == 1 and C <= layout[0] <= MAX_STRIDE
+              else _token_rows(x, "x", dtype, T, C, dev))
     strides = [stride]
     for t, name in ((a, "a"), (b, "b")):  # mostly in the layout of x
         if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.shape == shape
                 and t.stride() == layout):
             strides.append(stride)
         else:
-            strides.append(_rows(t, name, dtype, T, C, dev))
+            strides.append(_token_rows(t, name, dtype, T, C, dev))
     for t, name in ((A_log, "A_log"), (dt_bias, "dt_bias")):
         _dense(t, name, torch.float32, (C,), dev)
     return T, C, strides
@@ -133,6 +144,8 @@ def _seqlens(cu_seqlens, T: int, device, check: bool) -> int:
         _need(int(cu[0]) >= 0, "cu_seqlens[0] must be >= 0")
         _need(bool((cu[1:] >= cu[:-1]).all()), "cu_seqlens must be non-decreasing")
         _need(int(cu[-1]) <= T, f"cu_seqlens[-1]={int(cu[-1])} exceeds total tokens {T}")
+    if cu_seqlens.numel() - 1 > MAX_ROWS:
+        raise ValueError(f"cu_seqlens must have at most {MAX_ROWS} sequences")
     return cu_seqlens.numel() - 1
 
 
@@ -147,7 +160,7 @@ def validate(x, A_log, a, dt_bias, b, cu_seqlens, state, output, new_state, chec
     T, C, _ = _inputs(x, A_log, a, dt_bias, b, require_cuda)
     dev = x.device
     N = _seqlens(cu_seqlens, T, dev, check_seqlens)
-    _rows(output, "output", x.dtype, T, C, dev)
+    _token_rows(output, "output", x.dtype, T, C, dev)
     _dense(new_state, "new_state", torch.float32, (N, C), dev)
     if state is not None:
         _dense(state, "state", torch.float32, (N, C), dev)
@@ -166,6 +179,8 @@ def _checkpoint_rows(T: int) -> int:
 def empty_checkpoints(x) -> torch.Tensor:
     """The buffer that ``launch_scan`` fills for ``launch_scan_backward`` (one
     fp32 row of channels per 60 packed tokens)."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a [T, C] tensor")
     return x.new_empty((_checkpoint_rows(x.shape[0]), x.shape[1]), dtype=torch.float32)
 
 
@@ -196,7 +211,7 @@ def launch_scan(x, A_log, a, dt_bias, b, cu_seqlens, state=None, output=None, ne
     if output is None:
         output = _like(x)
     else:
-        _rows(output, "output", x.dtype, T, C, x.device)
+        _token_rows(output, "output", x.dtype, T, C, x.device)
         _need(T == 0 or output.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr()),
               "output must not overlap an input")
     if state is not None:
@@ -231,7 +246,7 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.device != dev:
         cu_seqlens = cu_seqlens.to(dev)
     N = _seqlens(cu_seqlens, T, dev, False)
-    dy_stride = _rows(d_output, "d_output", x.dtype, T, C, dev)
+    dy_stride = _token_rows(d_output, "d_output", x.dtype, T, C, dev)
     _dense(checkpoints, "checkpoints", torch.float32, (_checkpoint_rows(T), C), dev)
     if state is not None:
         _dense(state, "state", torch.float32, (N, C), dev)
@@ -243,7 +258,7 @@ def launch_scan_backward(d_output, x, A_log, a, dt_bias, b, cu_seqlens, state, c
             t = _like(x)
             grad_strides.append(C)
         else:
-            grad_strides.append(_rows(t, name, x.dtype, T, C, dev))
+            grad_strides.append(_token_rows(t, name, x.dtype, T, C, dev))
             _need(T == 0 or t.data_ptr() not in (x.data_ptr(), a.data_ptr(), b.data_ptr(), d_output.data_ptr()),
                   f"{name} must not overlap an input")
             _need(T == 0 or all(t.data_ptr() != u.data_ptr() for u in grads), f"{name} must not overlap another gradient")

@@ -649,3 +649,34 @@ def test_scan_of_many_empty_sequences(pkg, cuda_dev, N):
         assert torch.equal(a, b)
     assert torch.equal(got[5][at], want[5]) and torch.equal(got[5][empty], dns[empty])
     assert pkg.prefill.device_status(cuda_dev) == 0
+
+
+# ------------------------------------------------------------------- limits --
+def test_scan_refuses_what_its_indices_cannot_hold(pkg):
+    """As ``ValueError``, from ``validate`` and from the entry points alike."""
+    rec = pkg.recurrence
+    i = make([2], 4, torch.bfloat16)
+    far = torch.empty_strided((2, 4), (rec.MAX_STRIDE + 2, 1), dtype=torch.bfloat16)  # address space only
+    ok = dict(output=torch.empty_like(i["x"]), new_state=torch.empty(1, 4), require_cuda=False)
+    for k in ("x", "a", "b"):
+        with pytest.raises(ValueError, match=f"{k} must have at most"):
+            rec.validate(*gates({**i, k: far}), i["cu"], i["state"], **ok)
+    with pytest.raises(ValueError, match="output must have at most"):
+        rec.validate(*gates(i), i["cu"], i["state"], **{**ok, "output": far})
+    many = rec.MAX_CHANNELS + 1
+    x, v = torch.zeros(1, many), torch.zeros(many)
+    with pytest.raises(ValueError, match="channels"):
+        rec.validate(x, v, x, v, x, torch.tensor([0, 1]), None, torch.empty_like(x), torch.empty(1, many), require_cuda=False)
+    for x in (i["x"][0], i["x"][None], None):
+        with pytest.raises(ValueError, match="x must be a"):
+            rec.empty_checkpoints(x)
+        with pytest.raises(ValueError, match="x must be a"):
+            rec.gated_scan(x, *gates(i)[1:], i["cu"])
+
+
+def test_argument_statuses_are_value_errors(pkg):
+    C = pkg._capi
+    for status in range(1, 64):
+        with pytest.raises(C.GdnError) as e:
+            C.check(status, "call")
+        assert isinstance(e.value, ValueError) == (status in (1, 2, 3, 4, 6, 8)) and e.value.status == status
