@@ -85,6 +85,11 @@ __device__ __forceinline__ float max_keep_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float min_keep_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -146,6 +151,18 @@ __device__ __forceinline__ F2 sigmoid2(F2 b) {
     const float2 e = unpack2(mul2(b, splat2(-kLog2e)));
     const float2 d = unpack2(add2(pack2(ex2_approx(e.x), ex2_approx(e.y)), splat2(1.0f)));
     return pack2(rcp_approx(d.x), rcp_approx(d.y));
+}
+// sigmoid(b) and 1 - sigmoid(b), which the difference would lose from b = 17 on:
+// 1 / (1 + e) and e / (1 + e) with e = exp(-b).  Where that overflows, sigmoid(b)
+// is flushed to zero, and a finite e keeps its product with it a number.
+__device__ __forceinline__ F2 sigmoid2(F2 b, F2& rest) {
+    constexpr float kMost = 3.402823466e38f;
+    const float2 t = unpack2(mul2(b, splat2(-kLog2e)));
+    const F2 e = pack2(min_keep_nan(ex2_approx(t.x), kMost), min_keep_nan(ex2_approx(t.y), kMost));
+    const float2 d = unpack2(add2(e, splat2(1.0f)));
+    const F2 beta = pack2(rcp_approx(d.x), rcp_approx(d.y));
+    rest = mul2(e, beta);
+    return beta;
 }
 
 template <typename T>
@@ -761,48 +778,59 @@ __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanPar
     leave_cluster(gave_up);
 }
 
-// What the gates of a backward tile gave, per token and lane: log2 g, beta,
-// sigmoid(z) and the two inputs that are needed again, x and dy.  A thread
-// reads only what it wrote.
+// What the gates of a backward tile gave, per token and lane: log2 g, beta and
+// 1 - beta, sigmoid(z) and the two inputs that are needed again, x and dy, in 40
+// bytes.  A thread reads only what it wrote.
+constexpr size_t kGradTileBytes = 2 * kGradRows * 32 * 40;
 template <typename T>
-struct GradTile {  // 16-bit inputs: 32 bytes
-    static constexpr size_t kBytes = 2 * kGradRows * 32 * 32;
+struct GradTile {
     float4* base;
-    __device__ GradTile(unsigned char* smem, int lane) : base(reinterpret_cast<float4*>(smem) + lane) {}
-    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<T> x, RawPair<T> dy) {
+    float2* rests;
+    __device__ GradTile(unsigned char* smem, int lane)
+        : base(reinterpret_cast<float4*>(smem) + lane),
+          rests(reinterpret_cast<float2*>(smem + 2 * kGradRows * 32 * 32) + lane) {}
+    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 rest, F2 sig, RawPair<T> x, RawPair<T> dy) {
         const float2 a = unpack2(t), b = unpack2(beta), c = unpack2(sig);
         base[2 * i * 32] = make_float4(a.x, a.y, b.x, b.y);
         base[(2 * i + 1) * 32] = make_float4(c.x, c.y, __uint_as_float(x.bits), __uint_as_float(dy.bits));
+        rests[i * 32] = unpack2(rest);
     }
-    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& sig, F2& x, F2& dy) const {
+    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& rest, F2& sig, F2& x, F2& dy) const {
         const float4 a = base[2 * i * 32], b = base[(2 * i + 1) * 32];
+        const float2 c = rests[i * 32];
         t = pack2(a.x, a.y);
         beta = pack2(a.z, a.w);
+        rest = pack2(c.x, c.y);
         sig = pack2(b.x, b.y);
         x = raw_to_f2<T>({__float_as_uint(b.z)});
         dy = raw_to_f2<T>({__float_as_uint(b.w)});
     }
 };
+// With 8 bytes each for x and dy there is room (in clusters of any size) for
+// the smaller of beta and 1 - beta, which gives the other; its sign says which.
 template <>
-struct GradTile<float> {  // 40 bytes
-    static constexpr size_t kBytes = 2 * kGradRows * 32 * 40;
+struct GradTile<float> {
     float4* base;
     float2* sigs;
     __device__ GradTile(unsigned char* smem, int lane)
         : base(reinterpret_cast<float4*>(smem) + lane),
           sigs(reinterpret_cast<float2*>(smem + 2 * kGradRows * 32 * 32) + lane) {}
-    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 sig, RawPair<float> x, RawPair<float> dy) {
-        const float2 a = unpack2(t), b = unpack2(beta);
-        base[2 * i * 32] = make_float4(a.x, a.y, b.x, b.y);
+    static __device__ __forceinline__ float smaller(float beta, float rest) { return beta > rest ? -rest : beta; }
+    __device__ __forceinline__ void put(int i, F2 t, F2 beta, F2 rest, F2 sig, RawPair<float> x, RawPair<float> dy) {
+        const float2 a = unpack2(t), b = unpack2(beta), r = unpack2(rest);
+        base[2 * i * 32] = make_float4(a.x, a.y, smaller(b.x, r.x), smaller(b.y, r.y));
         base[(2 * i + 1) * 32] = make_float4(__uint_as_float(x.bits.x), __uint_as_float(x.bits.y),
                                              __uint_as_float(dy.bits.x), __uint_as_float(dy.bits.y));
         sigs[i * 32] = unpack2(sig);
     }
-    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& sig, F2& x, F2& dy) const {
+    __device__ __forceinline__ void get(int i, F2& t, F2& beta, F2& rest, F2& sig, F2& x, F2& dy) const {
         const float4 a = base[2 * i * 32], b = base[(2 * i + 1) * 32];
         const float2 c = sigs[i * 32];
+        const float lo0 = fabsf(a.z), lo1 = fabsf(a.w), hi0 = 1.0f - lo0, hi1 = 1.0f - lo1;
+        const bool rest0 = __float_as_int(a.z) < 0, rest1 = __float_as_int(a.w) < 0;
         t = pack2(a.x, a.y);
-        beta = pack2(a.z, a.w);
+        beta = pack2(rest0 ? hi0 : lo0, rest1 ? hi1 : lo1);
+        rest = pack2(rest0 ? lo0 : hi0, rest1 ? lo1 : hi1);
         sig = pack2(c.x, c.y);
         x = pack2(b.x, b.y);
         dy = pack2(b.z, b.w);
@@ -831,7 +859,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
     const int R = cluster_size(), rank = cluster_rank();
     GradTile<T> vals(smem, lane);
     const Strips<STRIPS> me;
-    float4* state_maps = reinterpret_cast<float4*>(smem + GradTile<T>::kBytes);  // [2][W][32], and then what precedes
+    float4* state_maps = reinterpret_cast<float4*>(smem + kGradTileBytes);  // [2][W][32], and then what precedes
     float4* grad_maps = state_maps + 2 * W * 32;                                 // [2][W][32], and then what follows
     float4* ranks = grad_maps + 2 * W * 32;                                      // [2][R][32]
     float4* cta_sums = ranks + 2 * R * 32;  // [R][32], the first CTA's: others write while it still works
@@ -990,8 +1018,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                     const float2 v = unpack2(z[j]), w = unpack2(e[j]);
                     const float2 q = make_float2(rcp_approx(1.0f + w.x), rcp_approx(1.0f + w.y));
                     const F2 sig = pack2(v.x < 0.0f ? w.x * q.x : q.x, v.y < 0.0f ? w.y * q.y : q.y);
-                    const F2 beta = sigmoid2(raw_to_f2<T>(b[j]));
-                    vals.put(buf * kRows + warp * kPiece + j, g[j], beta, sig, x[j], dy[j]);
+                    F2 rest;
+                    const F2 beta = sigmoid2(raw_to_f2<T>(b[j]), rest);
+                    vals.put(buf * kRows + warp * kPiece + j, g[j], beta, rest, sig, x[j], dy[j]);
                     z[j] = mul2(beta, raw_to_f2<T>(x[j]));
                 }
                 exp2_decays(g);
@@ -1006,10 +1035,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                     for (int j = kPiece - 1; j >= 0; --j) E = mul2(g[j], add2(raw_to_f2<T>(dy[j]), E));
                 } else {
                     const int at = me.strip * kPiece;
-                    F2 t, beta, sig, xs, dys;
+                    F2 t, beta, rest, sig, xs, dys;
 #pragma unroll 1
                     for (int j = 0; j < kPiece; ++j) {
-                        vals.get(buf * kRows + warp * kPiece + j, t, beta, sig, xs, dys);
+                        vals.get(buf * kRows + warp * kPiece + j, t, beta, rest, sig, xs, dys);
                         const bool covered = span.covered >> (at + j) & 1, start = span.start >> (at + j) & 1;
                         F2 g1[1] = {t};
                         exp2_decays(g1);
@@ -1019,7 +1048,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                     }
 #pragma unroll 1
                     for (int j = kPiece - 1; j >= 0; --j) {
-                        vals.get(buf * kRows + warp * kPiece + j, t, beta, sig, xs, dys);
+                        vals.get(buf * kRows + warp * kPiece + j, t, beta, rest, sig, xs, dys);
                         const bool covered = span.covered >> (at + j) & 1, end = span.end >> (at + j) & 1;
                         F2 g1[1] = {t};
                         exp2_decays(g1);
@@ -1051,20 +1080,20 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                 T* db = row_at<T>(static_cast<T*>(d.db) + c, t0, d.db_stride);
                 const int row0 = buf * kRows + warp * kPiece;
                 // one token's gradients from the state before it; e moves on to the token before
-                const auto token = [&](F2 g, F2 before, F2 t, F2 beta, F2 sig, F2 xs, F2 dys, F2& vx, F2& va, F2& vb) {
+                const auto token = [&](F2 g, F2 before, F2 beta, F2 rest, F2 sig, F2 xs, F2 dys, F2& vx, F2& va, F2& vb) {
                     const F2 G = add2(dys, e);
                     e = mul2(g, G);
                     const F2 dl = mul2(e, before);
                     vx = mul2(G, beta);
                     va = mul2(mul2(dl, minus_decay), sig);
-                    vb = mul2(mul2(vx, xs), fma2(beta, splat2(-1.0f), splat2(1.0f)));
+                    vb = mul2(mul2(vx, xs), rest);
                     return dl;
                 };
                 if ((done.start | done.end) == 0 && done.covered == kAllTokens<kSpan> && all_channels && d.grad_pairs) {
-                    F2 g[kPiece], t[kPiece], beta[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
+                    F2 g[kPiece], t[kPiece], beta[kPiece], rest[kPiece], sig[kPiece], xs[kPiece], dys[kPiece], before[kPiece];
 #pragma unroll
                     for (int j = 0; j < kPiece; ++j) {
-                        vals.get(row0 + j, t[j], beta[j], sig[j], xs[j], dys[j]);
+                        vals.get(row0 + j, t[j], beta[j], rest[j], sig[j], xs[j], dys[j]);
                         g[j] = t[j];
                     }
                     exp2_decays(g);
@@ -1076,7 +1105,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
 #pragma unroll
                     for (int j = kPiece - 1; j >= 0; --j) {
                         F2 vx, va, vb;
-                        const F2 dl = token(g[j], before[j], t[j], beta[j], sig[j], xs[j], dys[j], vx, va, vb);
+                        const F2 dl = token(g[j], before[j], beta[j], rest[j], sig[j], xs[j], dys[j], vx, va, vb);
                         sum_A = fma2(dl, t[j], sum_A);
                         sum_dt = add2(sum_dt, va);
                         store_pair(row_at<T>(dx, j, d.dx_stride), vx, true, true, true);
@@ -1085,10 +1114,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                     }
                 } else {
                     const int at = me.strip * kPiece;
-                    F2 before[kPiece], t, beta, sig, xs, dys;
+                    F2 before[kPiece], t, beta, rest, sig, xs, dys;
 #pragma unroll 1
                     for (int j = 0; j < kPiece; ++j) {
-                        vals.get(row0 + j, t, beta, sig, xs, dys);
+                        vals.get(row0 + j, t, beta, rest, sig, xs, dys);
                         F2 g[1] = {t};
                         exp2_decays(g);
                         h = state_of_strips<STRIPS>(offsets, p.state, p.channels, done.start >> j, kPiece, w0 + j, c, me.strip, h);
@@ -1097,11 +1126,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                     }
 #pragma unroll 1
                     for (int j = kPiece - 1; j >= 0; --j) {
-                        vals.get(row0 + j, t, beta, sig, xs, dys);
+                        vals.get(row0 + j, t, beta, rest, sig, xs, dys);
                         F2 g[1] = {t}, vx, va, vb;
                         exp2_decays(g);
                         e = state_of_strips<STRIPS>(offsets, d.d_new_state, p.channels, done.end >> j, kPiece, w0 + j, c, me.strip, e);
-                        const F2 dl = token(g[0], before[j], t, beta, sig, xs, dys, vx, va, vb);
+                        const F2 dl = token(g[0], before[j], beta, rest, sig, xs, dys, vx, va, vb);
                         if (done.covered >> (at + j) & 1) {
                             sum_A = fma2(dl, t, sum_A);
                             sum_dt = add2(sum_dt, va);
@@ -1330,7 +1359,7 @@ static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
     static int cache[2][64][kScanMaxCluster + 1];
-    const auto smem = [](int r) { return GradTile<T>::kBytes + (2 * 2 * kGradWarps + 3 * r) * 32 * sizeof(float4); };
+    const auto smem = [](int r) { return kGradTileBytes + (2 * 2 * kGradWarps + 3 * r) * 32 * sizeof(float4); };
     return launch_scan_clusters(gdn_scan_backward_kernel<T, 1>, gdn_scan_backward_kernel<T, 2>, cache, p.tokens, kGradRows,
                                 kGradThreads, p.channels, smem, s, p, d);
 }

@@ -680,3 +680,45 @@ def test_argument_statuses_are_value_errors(pkg):
         with pytest.raises(C.GdnError) as e:
             C.check(status, "call")
         assert isinstance(e.value, ValueError) == (status in (1, 2, 3, 4, 6, 8)) and e.value.status == status
+
+
+# ------------------------------------------------- gates far from the middle --
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("special", [False, True], ids=["inside", "starts"])
+def test_db_of_open_gates(pkg, cuda_dev, dtype, special):
+    """db = G x sigmoid(b) sigmoid(-b) for b from -60 to 60, where 1 - sigmoid(b) cannot be had by a difference.  Decays
+    of zero, so every token's gradient is its own, in pieces inside a sequence and in pieces where some start."""
+    T, C = 240, 32
+    i = make([1, 2, 3] * 40 if special else [T], C, dtype, cuda_dev, state=False)
+    i["b"] = torch.linspace(-60, 60, T * C, device=cuda_dev).view(T, C).to(dtype)
+    i["a"] += 300.0
+    x, dy, b = (i[k].double() for k in ("x", "dy", "b"))
+    beta, rest = torch.sigmoid(b), torch.sigmoid(-b)
+    dx, _, db = backward(pkg, i, dns=False)[:3]
+    # e = exp(-|b|): 2 U of the exponential and |b| U of its rounded argument; 1 / (1 + e): 2 U; 1 - e / (1 + e) adds U, and
+    # its argument's error times e, under U; three products
+    err = (12 + b.abs()) * ref.U
+    ref.close(dx, dy * beta, err * (dy * beta).abs(), "dx")
+    ref.close(db, dy * x * beta * rest, 2 * err * (dy * x * beta * rest).abs(), "db")
+
+
+@gpu
+def test_gates_past_the_exponents(pkg, cuda_dev):
+    """b and a at infinities and far out: gradients are the limits, and a NaN stays a NaN in its own channel."""
+    T, C = 150, 64
+    i = make([T], C, torch.float32, cuda_dev, memory="short", state=False)
+    for t, v in ((3, 100.0), (4, -100.0), (70, 1e4), (71, -1e4), (90, float("inf")), (91, -float("inf"))):
+        i["b"][t] = v
+    got = backward(pkg, i, dns=False)
+    fin = {**i, "b": i["b"].clamp(-500, 500)}
+    want = values(fin, dy=i["dy"], dns=None)
+    for g, name in zip(got, ("dx", "da", "db", "dA_log", "d_dt_bias")):
+        ref.close(g, *((v + (2.0 ** -126) * 16 if k else v) for k, v in enumerate(want[name])), name)  # flushed below 2^-126
+    j = {**i, "b": i["b"].clone()}
+    j["b"][40, 5] = float("nan")
+    bad = backward(pkg, j, dns=False)
+    keep = torch.arange(C, device=cuda_dev) != 5
+    for g, w in zip(bad[:3], got[:3]):
+        assert torch.equal(g[:, keep], w[:, keep])
+    assert bool(bad[2][40, 5].isnan())
