@@ -289,7 +289,8 @@ int gdn_prefill_launch_noalloc(const GdnPrefillArgs* args, void* stream);
  *   checkpoints fp32 [gdn_scan_checkpoint_rows(T), C] or NULL: what the
  *               backward pass needs of the forward pass
  * No output may be an input.  State and sums are fp32.  An empty
- * sequence's new_state row is its state row.  Output rows (and gradients) of
+ * sequence's new_state row is its state row.  An infinite state stays so until
+ * its sequence ends; gradients beside one are infinite or NaN.  Output rows (and gradients) of
  * tokens that belong to no sequence are written as zeros.  No reference
  * counterpart (the reference has the delta rule only). */
 typedef struct GdnScanArgs {

@@ -328,9 +328,15 @@ __device__ __forceinline__ bool scan_bounds(const ScanParams& p, int64_t n, int6
 // select.
 __device__ __forceinline__ bool is_start(float a) { return __float_as_uint(a) == 0x80000000u; }
 __device__ __forceinline__ F2 apply_map(float4 m, F2 h) { return fma2(pack2(m.x, m.y), h, pack2(m.z, m.w)); }
-__device__ __forceinline__ F2 apply_map_select(float4 m, F2 h) {
-    const float2 r = unpack2(apply_map(m, h));
-    return pack2(is_start(m.x) ? m.z : r.x, is_start(m.y) ? m.w : r.y);
+// Decays are positive, but a piece's product of them can fall below the least
+// float: an infinite state stays what it is (0 times it would be a NaN) until
+// the sequence ends.
+__device__ __forceinline__ float select_one(float A, float H, float h, float r) {
+    return is_start(A) ? H : fabsf(h) > 3.402823466e38f && A >= 0.0f ? h + H : r;
+}
+__device__ __noinline__ F2 apply_map_select(float4 m, F2 h) {
+    const float2 r = unpack2(apply_map(m, h)), v = unpack2(h);
+    return pack2(select_one(m.x, m.z, v.x, r.x), select_one(m.y, m.w, v.y, r.y));
 }
 struct Map2 {
     F2 A, H;

@@ -722,3 +722,27 @@ def test_gates_past_the_exponents(pkg, cuda_dev):
     for g, w in zip(bad[:3], got[:3]):
         assert torch.equal(g[:, keep], w[:, keep])
     assert bool(bad[2][40, 5].isnan())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("C", [64, 1024])
+@pytest.mark.parametrize("T", [5, 300, 3000])
+def test_infinite_states_stay(pkg, cuda_dev, T, C, dtype):
+    """An infinity, of the state before or of a token, is the state until the sequence ends, however small the product
+    of its decays; what follows is as without it."""
+    inf = float("inf")
+    i = make([T, 40, T], C, dtype, cuda_dev, memory="short")
+    good = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    i["state"][0, :8], i["state"][0, 8:16] = inf, -inf
+    at = T + 40 + T // 2
+    i["x"][at, 16:24], i["x"][at, 24:32] = inf, -inf
+    y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    want, want_ns = good[0].clone(), good[1].clone()
+    want[:T, :8], want[:T, 8:16], want_ns[0, :8], want_ns[0, 8:16] = inf, -inf, inf, -inf
+    want[at:, 16:24], want[at:, 24:32], want_ns[2, 16:24], want_ns[2, 24:32] = inf, -inf, inf, -inf
+    # infinities of two signs meet in a NaN
+    assert torch.equal(y, want) and torch.equal(ns, want_ns)
+    i["x"][T - 1, :8] = -inf
+    y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
+    assert bool(y[T - 1, :8].isnan().all()) and torch.equal(y[T:], want[T:]) and torch.equal(ns[1:], want_ns[1:])
