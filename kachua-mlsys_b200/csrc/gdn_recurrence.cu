@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "gdn_common.cuh"
+#include "gdn_once.cuh"
 #include "gdn_overlap.cuh"
 #include "tc05.cuh"
 
@@ -1288,25 +1289,25 @@ static cudaLaunchConfig_t scan_config(int cluster, unsigned groups, int threads,
     cfg.numAttrs = 1;
     return cfg;
 }
-// Clusters of `n` CTAs of `kernel` that run at once (-1: none), asked once per
-// device and size; the kernel's attributes are set with it, for `most` bytes of
-// shared memory.
+// Clusters of `n` CTAs of `kernel` that run at once (below 1: none, or not
+// known), asked once per device and size; the kernel's attributes are set with
+// it, for `most` bytes of shared memory.
+using ClusterCounts = std::atomic<int>[kScanMaxCluster + 1];
 template <typename Kernel>
-static int active_clusters(Kernel kernel, int n, int threads, size_t smem, size_t most, int (*cache)[kScanMaxCluster + 1]) {
+static int active_clusters(Kernel kernel, int n, int threads, size_t smem, size_t most, ClusterCounts* counts) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
-    if (cache[dev][n] == 0) {
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    return asked_once(counts[dev][n], [&] {
         cudaLaunchAttribute attr[1];
         const cudaLaunchConfig_t cfg = scan_config(n, 1, threads, smem, nullptr, attr);
         int got = 0;
-        const bool ok =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) == cudaSuccess &&
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) == cudaSuccess &&
             cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-            cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0;
-        if (!ok) (void)cudaGetLastError();
-        cache[dev][n] = ok ? got : -1;
-    }
-    return cache[dev][n];
+            cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess)
+            return got > 0 ? got : -1;
+        (void)cudaGetLastError();  // the query's own: the launch has to find none
+        return 0;
+    });
 }
 
 // CTAs per cluster, and the tiles that a CTA then walks one after another.  A
@@ -1336,7 +1337,7 @@ static ClusterShape scan_cluster(int64_t tiles, int64_t groups, Active active) {
 // 1024: 16 groups in clusters of 6 fill 96 SMs, 110 us; 32 in clusters of 4 fill
 // 128, 89 us).
 template <typename Smem, typename... Params, typename... Args>
-static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Params...), int (*cache)[64][kScanMaxCluster + 1],
+static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Params...), ClusterCounts (*counts)[64],
                                         int64_t tokens, int rows, int threads, int channels, Smem smem, cudaStream_t s, Args... args) {
     const int64_t groups[2] = {(channels + 63) / 64, (channels + 31) / 32};
     void (*const kernels[2])(Params...) = {one, two};
@@ -1344,7 +1345,7 @@ static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Para
     for (int i = 0; i < 2; ++i) {
         const int tile = rows * (i + 1);
         shape[i] = scan_cluster((tokens + tile - 1) / tile, groups[i], [&](int n) {
-            return active_clusters(kernels[i], n, threads, smem(n), smem(kScanMaxCluster), cache[i]);
+            return active_clusters(kernels[i], n, threads, smem(n), smem(kScanMaxCluster), counts[i]);
         });
     }
     const int i = shape[1].steps < shape[0].steps ? 1 : 0;
@@ -1357,16 +1358,16 @@ static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Para
 template <typename T>
 static cudaError_t launch_scan(const ScanParams& p, cudaStream_t s) {
     constexpr int kRows = kScanWarps * kScanPiece<T>;
-    static int cache[2][64][kScanMaxCluster + 1];
+    static ClusterCounts counts[2][64];
     const auto smem = [](int r) { return (2 * kRows + 2 * kScanWarps + 2 * r) * 32 * sizeof(float4); };
-    return launch_scan_clusters(gdn_scan_kernel<T, 1>, gdn_scan_kernel<T, 2>, cache, p.tokens, kRows, kScanThreads, p.channels, smem, s, p);
+    return launch_scan_clusters(gdn_scan_kernel<T, 1>, gdn_scan_kernel<T, 2>, counts, p.tokens, kRows, kScanThreads, p.channels, smem, s, p);
 }
 
 template <typename T>
 static cudaError_t launch_scan_backward(const ScanParams& p, const ScanGradParams& d, cudaStream_t s) {
-    static int cache[2][64][kScanMaxCluster + 1];
+    static ClusterCounts counts[2][64];
     const auto smem = [](int r) { return kGradTileBytes + (2 * 2 * kGradWarps + 3 * r) * 32 * sizeof(float4); };
-    return launch_scan_clusters(gdn_scan_backward_kernel<T, 1>, gdn_scan_backward_kernel<T, 2>, cache, p.tokens, kGradRows,
+    return launch_scan_clusters(gdn_scan_backward_kernel<T, 1>, gdn_scan_backward_kernel<T, 2>, counts, p.tokens, kGradRows,
                                 kGradThreads, p.channels, smem, s, p, d);
 }
 

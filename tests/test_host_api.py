@@ -1,5 +1,8 @@
 """Host-side behaviour of the two launch_gdn drop-ins that needs no GPU:
 argument checking (ValueError before any launch) and the input generators."""
+import ctypes
+import subprocess
+
 import pytest
 import torch
 
@@ -109,3 +112,28 @@ def test_config_shapes(pkg):
     assert len(lens) == 32 and min(lens) >= 64 and max(lens) <= 2048
     c3 = pkg.inputs.make_prefill_inputs(lens[:2], seed=0)
     assert c3.cu_seqlens.tolist() == [0, lens[0], lens[0] + lens[1]]
+
+
+def test_a_failed_query_is_asked_again(pkg, tmp_path):
+    """The scans' table of cluster counts keeps answers, not failures (host code, compiled here)."""
+    (tmp_path / "shim.cpp").write_text("""
+#include "gdn_once.cuh"
+#include <thread>
+#include <vector>
+static std::atomic<int> cell, asked;
+extern "C" int ask(int answer) { return gdn::asked_once(cell, [&] { ++asked; return answer; }); }
+extern "C" int times() { return asked; }
+extern "C" int from_threads(int n, int answer) {
+    std::vector<std::thread> all;
+    std::atomic<int> wrong{0};
+    for (int i = 0; i < n; ++i) all.emplace_back([&] { for (int k = 0; k < 1000; ++k) wrong += ask(answer) != answer; });
+    for (auto& t : all) t.join();
+    return wrong;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-pthread", f"-I{pkg._build.CSRC}", "-o", tmp_path / "shim.so",
+                    tmp_path / "shim.cpp"], check=True)
+    lib = ctypes.CDLL(str(tmp_path / "shim.so"))
+    assert [lib.ask(0), lib.ask(0), lib.times()] == [0, 0, 2]
+    assert lib.from_threads(8, 33) == 0 and 3 <= lib.times() <= 10
+    assert lib.ask(5) == 33 and lib.ask(0) == 33
