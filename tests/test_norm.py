@@ -646,3 +646,35 @@ def test_backward_from_four_threads(pkg, cuda_dev):
     torch.cuda.synchronize()
     for (dx, dw), t in zip(captured, results):
         assert torch.equal(dx, t[3]) and torch.equal(dw, t[4])
+
+
+# ----------------------------------------------- sums with one term to them --
+@gpu
+def test_gated_weight_gradient_of_one_head(pkg, cuda_dev):
+    """d_output in one head of many: the weight's gradient is that head's term, wherever it lies in the blocks' turns
+    (1184 blocks of 16 heads) and in the last, partial one."""
+    tokens, heads, dim = 9001, 5, 128
+    x, z, dy = (rnd(tokens, heads, dim, dtype=torch.bfloat16, device=cuda_dev, seed=s) for s in (1, 2, 3))
+    w = 1 + rnd(dim, device=cuda_dev, scale=0.1)
+    n = tokens * heads
+    for item in (0, 15, 16, 18943, 18944, 37887, 37888, 37888 + 7100, n - 6, n - 5, n - 1):
+        one = torch.zeros_like(dy).view(n, dim)
+        one[item] = dy.view(n, dim)[item]
+        dw = pkg.norm.launch_gated_norm_backward(one.view_as(dy), x, z, w, EPS)[2]
+        at = tuple(t.view(n, 1, dim)[item:item + 1] for t in (x, z, dy))
+        want, err = ref.gated_norm(*at[:2], w, EPS, dy=at[2])[2]
+        ref.close(dw, want, err, f"head {item}")
+
+
+@gpu
+@pytest.mark.parametrize("width", [250, 1003, 4096])
+def test_weight_gradient_of_one_row(pkg, cuda_dev, width):
+    rows = 2003
+    x, _, w = make(rows, width, torch.bfloat16, cuda_dev)
+    dy = rnd(rows, width, dtype=torch.bfloat16, device=cuda_dev, seed=8)
+    for row in (0, 1, 143, 144, 147, 148, 295, 296, 1183, 1184, 1999, 2000, 2002):
+        one = torch.zeros_like(dy)
+        one[row] = dy[row]
+        dw = pkg.norm.launch_add_norm_backward(one, x, w, EPS)[1]
+        want, err = ref.add_norm(None, None, w, EPS, dy=dy[row:row + 1], summed=x[row:row + 1])[1]
+        ref.close(dw, want, err, f"row {row}")

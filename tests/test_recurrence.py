@@ -746,3 +746,32 @@ def test_infinite_states_stay(pkg, cuda_dev, T, C, dtype):
     i["x"][T - 1, :8] = -inf
     y, ns = pkg.recurrence.launch_scan(*gates(i), i["cu"], i["state"])
     assert bool(y[T - 1, :8].isnan().all()) and torch.equal(y[T:], want[T:]) and torch.equal(ns[1:], want_ns[1:])
+
+
+# ----------------------------------------------- sums with one term to them --
+@gpu
+@pytest.mark.parametrize("lens", [[1000], [299, 1, 0, 700], [1] * 200], ids=["one", "ragged", "single"])
+@pytest.mark.parametrize("C", [40, 1024])
+def test_parameter_gradients_of_one_token(pkg, cuda_dev, lens, C):
+    """A gradient that enters at one token: the parameters' are then sums of the few terms before it, and a term that
+    is lost or counted twice, at a piece's or a tile's edge or at an end, is most of the answer."""
+    i = make(lens, C, torch.bfloat16, cuda_dev, memory="short")
+    T, U = sum(lens), ref.U
+    z = i["a"].double() + i["dt_bias"].double()
+    sp, sig = torch.logaddexp(z, torch.zeros_like(z)), torch.sigmoid(z)
+    dy = i["dy"]
+    # an exponential below 2^-126 is flushed to zero (a = 4.7 at rate 16: g = 2e-42), so a decay is off by that at most, and
+    # each of the T terms G g h rate sigmoid(z) by that times |G| |h| rate, |G| <= |dy|
+    h = max(float(v.abs().max()) for v in (i["state"], values(i)["y"][0]))
+    flush = 2.0 ** -126 * T * float(dy.abs().max()) * h * i["A_log"].double().exp()
+    for t in sorted({0, 1, 3, 4, 7, 8, 59, 60, 61, 119, 120, 151, 152, T - 121, T - 61, T - 60, T - 2, T - 1}):
+        i["dy"] = torch.zeros_like(dy)
+        i["dy"][t] = dy[t]
+        got = backward(pkg, i, dns=False)
+        da, err = values(i, dy=i["dy"], dns=None)["da"]
+        # a thread adds 4 tokens of each of its tiles (9 at most here), then 2 strips, 15 warps, 16 blocks: 71 roundings
+        depth = 100 * U
+        ref.close(got[4], da.sum(0), err.sum(0) + depth * da.abs().sum(0) + flush, f"d_dt_bias of token {t}")
+        # dA_log = sum of dl l = sum of da softplus / sigmoid; l has 8 U and its argument's rounding, sigmoid 8 U
+        dA, more = da * sp / sig, (32 + z.abs() * sig / sp) * U
+        ref.close(got[3], dA.sum(0), (err * sp / sig + (depth + more) * dA.abs()).sum(0) + flush * sp.amax(0), f"dA_log of token {t}")
