@@ -98,7 +98,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // constants are then in registers once for all of them), with
 // softplus(z) = max(z, 0) + log1p(u), u = exp(-|z|) in [0, 1].
 // log1p(u) / u is a polynomial, fitted by weighted least squares iterated to
-// the smallest maximal relative error (Lawson): 1.9e-7.  lg2.approx is not
+// the smallest maximal relative error (Lawson): 2.2e-7, its constants rounded to
+// floats.  lg2.approx is not
 // usable here: its error near 1 is absolute (2^-22), and softplus of a
 // strongly negative argument is a tiny number whose relative error the
 // recurrence multiplies by its memory.
@@ -125,7 +126,7 @@ __device__ __forceinline__ void log2_decays(F2 (&z)[N], F2 (&u)[N], F2 rate) {
 // place, but off in one direction (measured: by 0.05 of them on average at
 // -0.001, 0.2 at -0.01), which a decay's memory of a thousand tokens adds up to
 // 1e-5.  So decays above 2^-0.25 are 1 + t q(t), q fitted like the polynomial
-// above (3e-9; 0.4 units, 0.001 on average).
+// above (3.7e-9; evaluated in floats 0.4 units, 0.001 on average).
 template <int N>
 __device__ __forceinline__ void exp2_decays(F2 (&t)[N]) {
     constexpr float kExp2[4] = {0.693146824836731f, 0.24021293222904205f, 0.05534094199538231f, 0.008836725726723671f};

@@ -775,3 +775,23 @@ def test_parameter_gradients_of_one_token(pkg, cuda_dev, lens, C):
         # dA_log = sum of dl l = sum of da softplus / sigmoid; l has 8 U and its argument's rounding, sigmoid 8 U
         dA, more = da * sp / sig, (32 + z.abs() * sig / sp) * U
         ref.close(got[3], dA.sum(0), (err * sp / sig + (depth + more) * dA.abs()).sum(0) + flush * sp.amax(0), f"dA_log of token {t}")
+
+
+def test_gate_polynomials(pkg):
+    """The errors that the comments state are those of the constants as floats, in 64 bits."""
+    source = (pkg._build.CSRC / "gdn_recurrence.cu").read_text()
+
+    def constants(name):
+        at = source.index(name + "[")
+        text = source[source.index("{", at) + 1:source.index("}", at)]
+        return [float(torch.tensor(float(v.strip().rstrip("f")))) for v in text.split(",")]
+
+    def poly(c, x):
+        return sum(k * x ** n for n, k in enumerate(c))
+
+    u = torch.linspace(1e-4, 1, 1_000_001, dtype=torch.float64)
+    log1p = float((poly(constants("kLog1p"), u) * u / torch.log1p(u) - 1).abs().max())
+    t = torch.linspace(-0.25, 0, 1_000_001, dtype=torch.float64)
+    exp2 = float(((1 + t * poly(constants("kExp2"), t)) / torch.exp2(t) - 1).abs().max())
+    assert log1p <= 2.2e-7 and exp2 <= 3.7e-9
+    assert "2.2e-7" in source and "3.7e-9" in source
