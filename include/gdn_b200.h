@@ -406,6 +406,10 @@ typedef struct GdnGatedNormArgs {
 
 int gdn_gated_norm_launch(const GdnGatedNormArgs* args, void* stream);
 
+/* What gdn_gated_norm_launch would say of these arguments, without a device:
+ * for callers that launch something else first. */
+int gdn_gated_norm_check(const GdnGatedNormArgs* args);
+
 /* Gradients of either norm (quant = GDN_QUANT_NONE): d_output in the layout
  * of x; dx (and dz of the gated norm) contiguous, of `dtype`; d_weight fp32.
  * For gdn_add_norm args->x is the stored sum (new_residual), residual is not

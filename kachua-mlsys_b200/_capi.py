@@ -48,10 +48,11 @@ EXPORTED_SYMBOLS = (
     "gdn_add_norm_backward_workspace_size",
     "gdn_add_norm_backward_launch",
     "gdn_gated_norm_launch",
+    "gdn_gated_norm_check",
     "gdn_gated_norm_backward_workspace_size",
     "gdn_gated_norm_backward_launch",
 )
-ABI_VERSION = 10
+ABI_VERSION = 11
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 QUANT_NONE, QUANT_ROW, QUANT_GROUP = 0, 1, 2
 PATH_AUTO, PATH_RECURRENT, PATH_CHUNKED, PATH_SEGMENTED = 0, 1, 2, 3
@@ -277,6 +278,7 @@ def load(build_if_needed: bool = True) -> ctypes.CDLL:
                 ("gdn_add_norm_backward_workspace_size", size, [i64, i64]),
                 ("gdn_add_norm_backward_launch", ctypes.c_int, [norm, norm_grad, P, size, P]),
                 ("gdn_gated_norm_launch", ctypes.c_int, [gated, P]),
+                ("gdn_gated_norm_check", ctypes.c_int, [gated]),
                 ("gdn_gated_norm_backward_workspace_size", size, [i64, ctypes.c_int32, ctypes.c_int32]),
                 ("gdn_gated_norm_backward_launch", ctypes.c_int, [gated, norm_grad, P, size, P])):
             getattr(lib, name).restype = restype

@@ -37,7 +37,7 @@ static float resolve_scale(float s) { return s == 0.0f ? 1.0f / sqrtf((float)kD)
 
 using namespace gdn;
 
-extern "C" int gdn_abi_version(void) { return 10; }
+extern "C" int gdn_abi_version(void) { return 11; }
 
 extern "C" const char* gdn_status_string(int status) {
     switch (status) {

@@ -817,6 +817,20 @@ static Operands gated_norm_inputs(const GdnGatedNormArgs* a) {
     o.read(a->weight, 1, 0, a->head_dim * static_cast<int64_t>(dtype_bytes(a->weight_dtype)));
     return o;
 }
+// All that is checked of the forward call's arguments.
+static int gated_norm_checked(const GdnGatedNormArgs* a, GatedNormParams& p) {
+    if (int rc = gated_norm_setup(a, p)) return rc;
+    if (a->tokens > 0 && (!a->output || (a->quant && !a->scale))) return GDN_ERR_NULL_POINTER;
+    Operands o = gated_norm_inputs(a);
+    const int64_t n = static_cast<int64_t>(a->heads) * a->head_dim, row = n * static_cast<int64_t>(dtype_bytes(a->dtype));
+    if (a->quant) {
+        o.write(a->output, a->tokens, n, n);
+        o.write(a->scale, 1, 0, a->tokens * a->heads * 4);
+    } else {
+        o.write(a->output, a->tokens, row, row, true);
+    }
+    return o.apart() ? GDN_OK : GDN_ERR_OVERLAP;
+}
 }  // namespace gdn
 
 extern "C" int gdn_add_norm_launch(const GdnAddNormArgs* a, void* stream) {
@@ -894,19 +908,14 @@ extern "C" int gdn_add_norm_backward_launch(const GdnAddNormArgs* a, const GdnNo
     return e == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
 }
 
+extern "C" int gdn_gated_norm_check(const GdnGatedNormArgs* a) {
+    GatedNormParams p;
+    return gated_norm_checked(a, p);
+}
+
 extern "C" int gdn_gated_norm_launch(const GdnGatedNormArgs* a, void* stream) {
     GatedNormParams p;
-    if (int rc = gated_norm_setup(a, p)) return rc;
-    if (a->tokens > 0 && (!a->output || (a->quant && !a->scale))) return GDN_ERR_NULL_POINTER;
-    Operands o = gated_norm_inputs(a);
-    const int64_t n = static_cast<int64_t>(a->heads) * a->head_dim, row = n * static_cast<int64_t>(dtype_bytes(a->dtype));
-    if (a->quant) {
-        o.write(a->output, a->tokens, n, n);
-        o.write(a->scale, 1, 0, a->tokens * a->heads * 4);
-    } else {
-        o.write(a->output, a->tokens, row, row, true);
-    }
-    if (!o.apart()) return GDN_ERR_OVERLAP;
+    if (int rc = gated_norm_checked(a, p)) return rc;
     if (int rc = check_device()) return rc;
     if (a->tokens == 0) return GDN_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -172,8 +172,9 @@ def _gated_inputs(x, z, weight, eps):
     return x, z, _heads(x, "x", x.dtype, shape, dev), _heads(z, "z", x.dtype, shape, dev), _weight(weight, dim, x.dtype, dev)
 
 
-def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):
-    """Checks the arguments and makes the C ones; returns ``(launch, output, scale)``."""
+def _prepare_gated_norm(x, z, weight, eps, output, scale, quant, check: bool = False):
+    """Checks the arguments and makes the C ones; returns ``(launch, output, scale)``.
+    With ``check`` the library's checks, which are the launch's own, come now too."""
     shape = x.shape if isinstance(x, torch.Tensor) else None
     x, z, xs, zs, wdt = _gated_inputs(x, z, weight, eps)
     tokens, heads, dim = x.shape
@@ -196,6 +197,8 @@ def _prepare_gated_norm(x, z, weight, eps, output, scale, quant):
     args = _pack_gated(_ptr(x), _ptr(z), xs, zs, _ptr(weight), wdt, DTYPES[x.dtype],
                                   _capi.QUANT_GROUP if quant else _capi.QUANT_NONE, eps, tokens, heads, dim,
                                   _ptr(output), _ptr(scale))
+    if check:
+        _capi.check(_capi.load().gdn_gated_norm_check(args), "gdn_gated_norm_check")
 
     def launch():
         _call(_capi.load().gdn_gated_norm_launch, "gdn_gated_norm_launch", dev, args)
@@ -264,18 +267,21 @@ class OutputNorm:
     scale: torch.Tensor | None = None
 
     def prepare(self, output):
-        """Checks the norm against the ``output`` it will be applied to and
-        returns the call that launches it."""
+        """Checks the norm against the ``output`` it will be applied to, all of
+        it, so that nothing is refused once the recurrence has run, and returns
+        the call that launches it."""
         _need((self.codes is None) == (self.scale is None), "codes and scale go together")
         z = self.z
         _need(isinstance(z, torch.Tensor) and z.numel() == output.numel(), f"z must have the output's shape {tuple(output.shape)}")
         if z.shape != output.shape:  # [B, 1, heads, 128] for an output [B, heads, 128], or the other way round
             _need(z.is_contiguous(), "z must be contiguous unless it has the output's shape")
             z = z.view(output.shape)
+        _need(z.numel() == 0 or output.data_ptr() != z.data_ptr(), "output must not be z")
+        # in place, or at least none of the recurrence's output where the norm reads
+        launch = _prepare_gated_norm(output, z, self.weight, self.eps, output, None, False, check=True)[0]
         if self.codes is None:
-            return _prepare_gated_norm(output, z, self.weight, self.eps, output, None, False)[0]
-        _need(z.numel() == 0 or output.data_ptr() != z.data_ptr(), "z must not be the output")
-        return _prepare_gated_norm(output, z, self.weight, self.eps, self.codes, self.scale, True)[0]
+            return launch
+        return _prepare_gated_norm(output, z, self.weight, self.eps, self.codes, self.scale, True, check=True)[0]
 
 
 class _AddNorm(torch.autograd.Function):

@@ -202,3 +202,42 @@ def test_gated_norm_refuses_overlaps(pkg, cuda_dev):
         t = [dy.clone(), x.clone(), z.clone()]
         got = n.launch_gated_norm_backward(*t, w, EPS, dx=t[a], dz=t[b])
         assert all(torch.equal(g, want) for g, want in zip(got, grads))
+
+
+@gpu
+def test_out_norm_is_refused_before_the_recurrence(pkg, cuda_dev):
+    """Whatever the norm cannot take is found while an in-place state is still the state before."""
+    w = 1 + rnd(129, device=cuda_dev, scale=0.1)
+    dec = pkg.inputs.make_decode_inputs(5, seed=1).to(cuda_dev)
+    before = dec.state.clone()
+    buf = torch.zeros(6, 8, 128, dtype=torch.bfloat16, device=cuda_dev)
+    out, apart = buf[:5], torch.zeros(5, 8, 128, dtype=torch.bfloat16, device=cuda_dev)
+    codes = torch.zeros(5, 8, 128, dtype=torch.float8_e4m3fn, device=cuda_dev)
+    scale = torch.zeros(5, 8, device=cuda_dev)
+    N = pkg.norm.OutputNorm
+    for norm in (N(buf[1:], w[:128]), N(buf[1:], w[:128], codes=codes, scale=scale),
+                 N(apart, out.view(-1).view(torch.float32)[3:131]), N(apart, w[:128], codes=codes, scale=codes.view(-1)[:160].view(torch.float32).view(5, 8)),
+                 N(apart, w[:128], codes=apart.view(torch.float8_e4m3fn).view(-1)[:5120].view(5, 8, 128), scale=scale)):
+        with pytest.raises(ValueError, match="overlap"):
+            pkg.decode.launch_gdn(*dec.args(), output=out, new_state=dec.state, out_norm=norm)
+        assert torch.equal(dec.state, before) and not out.any()
+    z = rnd(5, 8, 128, dtype=torch.bfloat16, device=cuda_dev)
+    pkg.decode.launch_gdn(*dec.args(), output=out, new_state=dec.state, out_norm=N(z, w[1:]))
+    assert out.any() and not torch.equal(dec.state, before)
+
+
+def test_gated_norm_check(pkg):
+    """The check answers as the launch does where that refuses, and needs no device where it does not."""
+    lib, C = pkg._capi.load(), pkg._capi
+    buf = ctypes.create_string_buffer(1 << 14)
+    p = (ctypes.addressof(buf) + 4095) // 4096 * 4096
+    for want, kw in ((0, {}), (0, dict(output=p)), (0, dict(quant=2)), (0, dict(tokens=0, x=None, z=None, output=None)), (1, dict(z=None)),
+                     (1, dict(output=None)), (1, dict(quant=2, scale=None)), (2, dict(head_dim=96)), (2, dict(eps=-1.0)), (3, dict(z=p + 1)),
+                     (6, dict(dtype=5)), (8, dict(output=p + 512)), (8, dict(output=p, quant=2)), (8, dict(z=p + 4096, output=p + 4096 + 256))):
+        a = C.GdnGatedNormArgs(p, p + 1024, 256, 256, p + 2048, C.DTYPE_F32, C.DTYPE_BF16, 0, EPS, 2, 2, 128, p + 3072, p + 6144)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        assert lib.gdn_gated_norm_check(ctypes.byref(a)) == want, kw
+        if want:
+            assert lib.gdn_gated_norm_launch(ctypes.byref(a), None) == want, kw
+    assert lib.gdn_gated_norm_check(None) == 1
