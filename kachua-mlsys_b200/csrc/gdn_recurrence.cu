@@ -340,6 +340,12 @@ __device__ __noinline__ F2 apply_map_select(float4 m, F2 h) {
     const float2 r = unpack2(apply_map(m, h)), v = unpack2(h);
     return pack2(select_one(m.x, m.z, v.x, r.x), select_one(m.y, m.w, v.y, r.y));
 }
+// The same without that, for the backward pass: beside an infinity its gradients
+// are not finite either way.
+__device__ __forceinline__ F2 apply_map_start(float4 m, F2 h) {
+    const float2 r = unpack2(apply_map(m, h));
+    return pack2(is_start(m.x) ? m.z : r.x, is_start(m.y) ? m.w : r.y);
+}
 struct Map2 {
     F2 A, H;
 };
@@ -1080,8 +1086,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(cons
                 const float4 hm = state_maps[(buf * W + warp) * 32 + lane], em = grad_maps[(buf * W + warp) * 32 + lane];
                 F2 h = apply_map(hm, tile_h), e = apply_map(em, tile_e);
                 if (__any_sync(0xffffffffu, !all_finite(tile_h) || !all_finite(tile_e))) {
-                    h = apply_map_select(hm, tile_h);
-                    e = apply_map_select(em, tile_e);
+                    h = apply_map_start(hm, tile_h);
+                    e = apply_map_start(em, tile_e);
                 }
                 T* dx = row_at<T>(static_cast<T*>(d.dx) + c, t0, d.dx_stride);
                 T* da = row_at<T>(static_cast<T*>(d.da) + c, t0, d.da_stride);
