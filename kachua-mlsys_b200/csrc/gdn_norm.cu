@@ -13,9 +13,11 @@
 // All of it is one pass over the data: a row (or head) stays in registers
 // between its statistics and its output.  8 elements per thread and load
 // (one 16-byte vector of a 16-bit type), arithmetic on packed fp32 pairs.
-// HBM-bound: 65536 x 4096 bf16 with a residual 311 us (6.9 TB/s, the copy rate
-// is 6.6), to e4m3 by rows 294 us (6.4); backward 332 us (6.5); 32768 tokens of
-// 32 heads of 128 gated 128 us (6.3), backward 223 us (6.0).
+// HBM-bound.  Into outputs kept between calls, 65536 x 4096 bf16 with a residual
+// takes 311 us (6.9 TB/s; the rate of a copy is 6.6), to e4m3 by rows 299 us (6.3;
+// 316 to 330 into outputs that each call allocates), by groups 312 us (6.0);
+// backward 323 us (6.6); 32768 tokens of 32 heads of 128 gated 128 us (6.3), to
+// e4m3 135 us (5.0), backward 222 us (6.0).
 #include <cuda_fp8.h>
 
 #include <initializer_list>
@@ -87,8 +89,8 @@ constexpr int kApart = 0;  // any alignment: blockDim.x apart, so that a warp's 
 constexpr int kVec = 1;    // rows are whole 8-element vectors on 16-byte boundaries
 // Rows of 16 elements or more whose width is not a multiple of 8, contiguous or
 // apart by a multiple of 8 elements more: the vectors of the whole tensor, of
-// which a row's first and last are only partly its own (16384 x 5333 bf16: 145
-// us forward, 181 backward; dealt apart 300 and 385).
+// which a row's first and last are only partly its own (16384 x 5333 bf16: 147
+// to 154 us forward, 181 backward; dealt apart 301 and 378).
 constexpr int kShift = 2;
 struct Cols {
     int first, step, width;
@@ -175,8 +177,8 @@ __device__ __forceinline__ void store8(T* row, Cols c, const F2 (&f)[4]) {
 // The scale of values up to amax, and its reciprocal in two words: y over the
 // scale is y (inv + rest), the fp32 quotient, where y inv alone is off by a
 // unit or two and at a tie of two codes gives the other one.  (One multiply more:
-// 65536 x 4096 bf16 to e4m3 by rows 324 us a call, 318 without.)  An infinite amax has no second
-// word: finite values over it are 0, infinite ones NaN.
+// 65536 x 4096 bf16 to e4m3 by rows 299 us, 294 without.)  An infinite amax has no
+// second word: finite values over it are 0, infinite ones NaN.
 struct Scale {
     float scale, inv, rest;
     __device__ __forceinline__ explicit Scale(float amax) : scale(amax / kFp8Max), inv(kFp8Max / amax) {
@@ -602,11 +604,12 @@ struct RowShape {
 static RowShape row_shape(int vecs, int vpt) { return {((vecs + vpt - 1) / vpt + 31) / 32 * 32, vpt}; }
 // Forward.  Two vectors per thread halve the warps that a row's sum waits for
 // (32768 x 2048 bf16: 82.7 us, 93.0 with one); four where a scale per row adds
-// a second wait (65536 x 1024: 74.7 us, 82.9 with two); but fp32 takes two up to
-// 1024 vectors, for its occupancy (16384 x 4096 with a scale per row: 130 us, 146
-// with four; 16384 x 6144: 196 and 206; shifted 16384 x 4097: 185 and 232).  Rows
-// dealt apart hold twice the registers per vector, so fewer (16384 x 5333: 320 us
-// with two, 483 with four).
+// a second wait (65536 x 1024: 78.3 us, 84.6 with two); but fp32 takes two up to
+// 1024 vectors, for its occupancy (16384 x 4096 with a scale per row: 133 us, 150
+// with four; 16384 x 6144: 204 and 206; shifted 16384 x 4097: 183 and 236).  Rows
+// dealt apart hold twice the registers per vector, so fewer (16384 x 5333: 301 us
+// with two, 483 with four).  Eight spill up to 250 bytes a thread in fp32 and
+// apart (4096 x 32768 bf16: 208 us, 5.2 TB/s).
 static int row_vecs(int width, int mode) { return (width + (mode == kShift ? 14 : 7)) / 8; }
 static RowShape row_shape_forward(const NormParams& p, size_t elem) {
     const int vecs = row_vecs(p.width, p.mode);
@@ -641,8 +644,11 @@ static cudaError_t launch_add_norm(const NormParams& p, cudaStream_t s) {
 }
 
 // Backward: the weight and its gradient's share are held too, so two vectors at
-// most while they fit (65536 x 4096 bf16: 332 us, 407 with one on twice the
-// threads, whose sums wait for twice the warps).
+// most while they fit (65536 x 4096 bf16: 323 us, 407 with one on twice the
+// threads, whose sums wait for twice the warps).  A vector holds 40 floats (w, dw,
+// r, g, o), so the wider rows spill, with four about 1 KB a thread and with eight
+// 3 to 5 KB: 16384 x 12288 bf16 578 us, where the copy rate is 245; 8192 x 16384
+// 312 and 164; 4096 x 32768 1190 and 164.
 static RowShape row_shape_backward(int width, int mode) {
     const int vecs = row_vecs(width, mode);
     if (mode == kApart) return row_shape(vecs, vecs <= 1024 ? 1 : vecs <= 2048 ? 4 : 8);

@@ -556,11 +556,15 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
 //               order (the same bits on every run).
 // So the gates' arithmetic, which is what the kernel is made of, has a whole
 // tile's time to hide the cluster's exchange behind.
-// Bound by instruction issue: 83 warp instructions per token and pair of
-// channels, 64 % of the slots with five warps to a scheduler.  Measured (bf16):
-// 1 x 16384 x 4096 143 us, 3.8 TB/s of inputs and outputs, 57 % of the copy
-// rate; 1 x 40000 x 1024 98 us; 32 x 64..2048 x 2048 172 us.  A thread per
-// sequence and channel took 42 ms for the second.
+// 85 warp instructions per token and pair of channels, about 35 of them gates and
+// chains, which at full issue on every SM would take 79 us of the first case below.
+// It takes longer because clusters fill 128 of the 148 SMs and those issue in 63 %
+// of their slots: with five warps to a scheduler the fixed latencies of dependent
+// instructions (1.8 of a warp's stalls per issue; special-function pipe 1.1,
+// memory 0.5) are not all hidden.  Measured (bf16): 1 x 16384 x 4096 145 us, 3.7
+// TB/s of inputs and outputs, 56 % of the copy rate; 1 x 40000 x 1024 99 us; 32 x
+// 64..2048 x 2048 177 us.  A thread per sequence and channel took 42 ms for the
+// second.
 template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kScanThreads, 1) gdn_scan_kernel(const ScanParams p) {
     constexpr int W = kScanWarps, kPiece = kScanPiece<T>, kRows = W * kPiece, kTile = STRIPS * kRows;
@@ -859,9 +863,9 @@ struct GradTile<float> {
 // gates once, keeps what the gradients need of them in shared memory, and
 // writes its piece's gradients a tile later, when both ends are known.  The
 // sums over tokens stay in registers to the end, and are added over the CTA's
-// warps and the cluster's CTAs in order.  Bound by instruction issue like the
-// forward pass; measured (bf16): 1 x 16384 x 4096 279 us, 3.4 TB/s;
-// 8 x 4096 x 1024 177 us.
+// warps and the cluster's CTAs in order.  Bound like the forward pass: 160 warp
+// instructions per token and pair of channels in 63 % of the slots; measured
+// (bf16): 1 x 16384 x 4096 273 us, 3.4 TB/s; 8 x 4096 x 1024 184 us.
 template <typename T, int STRIPS>
 __global__ void __launch_bounds__(kGradThreads, 1) gdn_scan_backward_kernel(const ScanParams p, const ScanGradParams d) {
     constexpr int W = kGradWarps, kPiece = kGradPiece, kRows = kGradRows, kTile = STRIPS * kRows, kSpan = STRIPS * kPiece;
@@ -1341,8 +1345,8 @@ static ClusterShape scan_cluster(int64_t tiles, int64_t groups, Active active) {
 // A kernel with one and with two strips to a warp: `rows` tokens per strip and
 // tile, smem(r) bytes in clusters of r.  Two strips of 32 channels make twice
 // the groups and half the tiles: better clusters for few channels (1 x 40000 x
-// 1024: 16 groups in clusters of 6 fill 96 SMs, 110 us; 32 in clusters of 4 fill
-// 128, 89 us).
+// 1024: 16 groups in clusters of 6 fill 96 SMs, 32 in clusters of 4 fill 128; 110
+// and 89 us with 15 map warps and shorter gates, 99 with two strips as it is now).
 template <typename Smem, typename... Params, typename... Args>
 static cudaError_t launch_scan_clusters(void (*one)(Params...), void (*two)(Params...), ClusterCounts (*counts)[64],
                                         int64_t tokens, int rows, int threads, int channels, Smem smem, cudaStream_t s, Args... args) {

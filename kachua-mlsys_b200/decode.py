@@ -136,9 +136,10 @@ class PreparedLaunch:
 
     For serving loops that call the same buffers every step (and for CUDA
     graph capture): arguments are checked once here; ``__call__`` launches on
-    the current stream of the tensors' device.  Every form ``launch_gdn``
-    takes is accepted: T >= 1 tokens per sequence, an fp32 or (one token) a
-    bf16 state, any supported head counts; all go through
+    the current stream of the tensors' device.  Every form of the step that
+    ``launch_gdn`` takes is accepted: T >= 1 tokens per sequence, an fp32 or
+    (one token) a bf16 state, any supported head counts (an ``out_norm`` is a
+    launch of its own, ``norm.launch_gated_norm``, behind it); all go through
     ``gdn_decode_launch_heads``, which routes the reference's 4 / 8 heads to
     the same kernels as ``gdn_decode_launch``.
     """
