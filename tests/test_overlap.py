@@ -233,8 +233,8 @@ def test_gated_norm_check(pkg):
     p = (ctypes.addressof(buf) + 4095) // 4096 * 4096
     for want, kw in ((0, {}), (0, dict(output=p)), (0, dict(quant=2)), (0, dict(tokens=0, x=None, z=None, output=None)), (1, dict(z=None)),
                      (1, dict(output=None)), (1, dict(quant=2, scale=None)), (2, dict(head_dim=96)), (2, dict(eps=-1.0)), (3, dict(z=p + 1)),
-                     (6, dict(dtype=5)), (8, dict(output=p + 512)), (8, dict(output=p, quant=2)), (8, dict(z=p + 4096, output=p + 4096 + 256))):
-        a = C.GdnGatedNormArgs(p, p + 1024, 256, 256, p + 2048, C.DTYPE_F32, C.DTYPE_BF16, 0, EPS, 2, 2, 128, p + 3072, p + 6144)
+                     (6, dict(dtype=5)), (8, dict(output=p + 512)), (8, dict(output=p, quant=2)), (8, dict(z=p + 5120, output=p + 5120 + 256))):
+        a = C.GdnGatedNormArgs(p, p + 1024, 256, 256, p + 2048, C.DTYPE_F32, C.DTYPE_BF16, 0, EPS, 2, 2, 128, p + 4096, p + 6144)
         for k, v in kw.items():
             setattr(a, k, v)
         assert lib.gdn_gated_norm_check(ctypes.byref(a)) == want, kw
